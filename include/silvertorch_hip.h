@@ -483,6 +483,111 @@ int st_fused_kmean_ann_noalloc(const int64_t* cluster_offsets, int64_t num_offse
                                int64_t invalid_index_value, void* scores,
                                int32_t* indices, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Tables held in 4 bits.  No counterpart in the reference.
+ *
+ * A table [rows, dim] is packed uint8 [rows, ceil(dim / 32) * 16] (16-byte
+ * aligned; column 2j in the low half of a row's byte j, column 2j + 1 in the
+ * high half), scales [rows, groups] (scale_type) and zeros uint8 [rows,
+ * groups] or null (8 everywhere), with groups = ceil(dim / group_size) and
+ * group_size a positive multiple of 32: column d stands for
+ * scales[d / group_size] * (code - zeros[d / group_size]).  Types are
+ * ST_SCORE_F32, ST_SCORE_F16 or ST_SCORE_BF16.  Everything is contiguous.
+ *
+ * st_int4_quantize: weight [rows, dim] to packed, scales (of the weight's type)
+ * and zeros, in 32-bit arithmetic with IEEE division.  Symmetric: scale =
+ * max |w| / 7, zero 8, code = round(w / scale) + 8; else scale = (max(w, 0) -
+ * min(w, 0)) / 15, zero = round(-min(w, 0) / scale), code = round(w / scale)
+ * + zero; the scale is rounded to its type first, ties go to even, codes and
+ * zeros are kept in [0, 15].  A group of zeros has scale 0, one with a value
+ * that is not finite scale NaN.
+ *
+ * st_int4_matvec: y [queries, rows] (y_type) = x [queries, dim] (x_type) times
+ * the table transposed, summed in 32 bits and rounded once.
+ * ------------------------------------------------------------------------- */
+int st_int4_quantize(const void* weight, int weight_type, int64_t rows, int64_t dim,
+                     int64_t group_size, int symmetric, uint8_t* packed, void* scales,
+                     uint8_t* zeros, void* stream);
+int st_int4_matvec(const uint8_t* packed, const void* scales, int scale_type,
+                   const uint8_t* zeros, const void* x, int x_type, int64_t queries,
+                   int64_t rows, int64_t dim, int64_t group_size, void* y, int y_type,
+                   void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Log-probabilities of given documents, entropy and best alternatives, and
+ * their gradient.  No counterpart in the reference.
+ *
+ * logits [rows, columns] (ST_SCORE_F32, _F16 or _BF16; row r starts at element
+ * r * row_stride, columns < 2^31); mask: the packed search output (document d
+ * at bit 63 - d % 64 of word d / 64; row r's words start at r * mask_stride, so
+ * 0 shares one row; mask_words of a row are readable and cover the columns), or
+ * null.  A column whose bit is not set, or whose score is -inf, is excluded.
+ * With l = log sum e^(z / temperature) over the others and log p = z /
+ * temperature - l: logprobs[r] = log p of targets[r] (-inf for an excluded one
+ * and one outside the columns; 0 for -1, "no target"), entropy[r] = -sum p log
+ * p, lse[r] = l, top_ids / top_logprobs [rows, topk] the columns of largest
+ * score in order, equal ones by column, padded with -1 / -inf.  A row that
+ * excludes every column has entropy 0 and l = -inf.  A NaN or +inf among the
+ * others makes logprobs, entropy and lse NaN; NaN is never an alternative.
+ * stats [rows, 2] (or null) is what the backward call needs.  0 <= topk <= 128,
+ * 1e-6 <= temperature <= 1e6.  workspace: device memory of
+ * st_target_logprobs_workspace_bytes(rows, columns, topk) bytes (may be 0),
+ * 16-byte aligned.
+ *
+ * st_target_logprobs_backward: grad_logits [rows, columns] (score_type,
+ * contiguous) from the gradients of the four outputs, each float32 and null for
+ * zero; excluded columns get 0, and an excluded target gives none.
+ * ------------------------------------------------------------------------- */
+int64_t st_target_logprobs_workspace_bytes(int64_t rows, int64_t columns, int64_t topk);
+int st_target_logprobs(const void* logits, int score_type, int64_t rows, int64_t columns,
+                       int64_t row_stride, const int64_t* targets, const int64_t* mask,
+                       int64_t mask_stride, int64_t mask_words, int64_t topk,
+                       double temperature, void* workspace, float* logprobs, float* entropy,
+                       float* lse, int64_t* top_ids, float* top_logprobs, float* stats,
+                       void* stream);
+int st_target_logprobs_backward(const void* logits, int score_type, int64_t rows,
+                                int64_t columns, int64_t row_stride, const int64_t* targets,
+                                const int64_t* mask, int64_t mask_stride, int64_t mask_words,
+                                int64_t topk, double temperature, const float* entropy,
+                                const float* stats, const int64_t* top_ids,
+                                const float* grad_logprobs, const float* grad_entropy,
+                                const float* grad_lse, const float* grad_top_logprobs,
+                                void* grad_logits, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Routing rows to clusters, with the balance loss and its gradient.  No
+ * counterpart in the reference; the ids are what st_fused_kmean_ann takes.
+ *
+ * logits [rows, clusters] (ST_SCORE_F32, _F16 or _BF16; row r starts at element
+ * r * row_stride; 1 <= clusters <= 32768); valid uint8 [rows] or null.  Per
+ * valid row: lse = log sum e^z, cluster_ids [rows, probes] the clusters of
+ * largest score in order, equal ones by cluster (clusters at -inf or NaN are
+ * never chosen; padded with -1), weights = e^(z - lse) at them (padded with 0).
+ * Rows whose flag is 0, or with every score at -inf, have ids -1, weights 0,
+ * lse -inf and are not counted.  counts [clusters]: rows that chose each;
+ * loss = clusters * sum_e (counts_e / (probes * n)) (sum_rows p_e / n) over
+ * the n counted rows (0 without any).  stats [rows, 2] and slopes [clusters]
+ * are what the backward call needs.  1 <= probes <= 64.  workspace: device
+ * memory of st_cluster_route_workspace_bytes(rows, clusters) bytes, 16-byte
+ * aligned.  The same inputs give the same bits.
+ *
+ * st_cluster_route_backward: grad_logits [rows, clusters] (score_type,
+ * contiguous) from the gradients of weights, lse and loss, each float32 and
+ * null for zero (grad_weights at padding is ignored).  The counts are
+ * constants.
+ * ------------------------------------------------------------------------- */
+int64_t st_cluster_route_workspace_bytes(int64_t rows, int64_t clusters);
+int st_cluster_route(const void* logits, int score_type, int64_t rows, int64_t clusters,
+                     int64_t row_stride, int64_t probes, const uint8_t* valid, void* workspace,
+                     int64_t* cluster_ids, float* weights, float* lse, int64_t* counts,
+                     float* loss, float* stats, float* slopes, void* stream);
+int st_cluster_route_backward(const void* logits, int score_type, int64_t rows,
+                              int64_t clusters, int64_t row_stride, int64_t probes,
+                              const int64_t* cluster_ids, const float* weights,
+                              const float* stats, const float* slopes,
+                              const float* grad_weights, const float* grad_lse,
+                              const float* grad_loss, void* grad_logits, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

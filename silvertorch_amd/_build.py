@@ -54,10 +54,16 @@ LIB_SOURCES = [
     "filtered_topk.hip",
     "kmean_ann.hip",
     "fresh_topk.hip",
+    "int4_matvec.hip",
+    "target_logprobs.hip",
+    "cluster_route.hip",
     "search_plan.cpp",
     "host_pool.cpp",
     "expression_parser.cpp",
 ]
+
+# torch.ops.st.* registration
+EXT_SOURCES = ["torch_ops.cpp", "torch_head_ops.cpp"]
 
 
 def _run(cmd: list[str]) -> None:
@@ -124,11 +130,21 @@ def build_extension() -> Path:
     inc, libdirs = _torch_paths()
     py_inc = sysconfig.get_paths()["include"]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = [
-        "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+    flags = [
+        "-O2", "-std=c++17", "-fPIC",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         *[f"-I{p}" for p in inc], f"-I{py_inc}", "-I/opt/rocm/include",
-        str(CSRC / "torch_ops.cpp"),
+    ]
+
+    def compile_object(src: str) -> str:
+        obj = str(OBJ / (src + ".o"))
+        _run(["g++", *flags, "-c", str(CSRC / src), "-o", obj])
+        return obj
+
+    with ThreadPoolExecutor() as ex:
+        objs = list(ex.map(compile_object, EXT_SOURCES))
+    cmd = [
+        "g++", "-shared", *objs,
         f"-L{PKG}", "-lsilvertorch_hip",
         *[f"-L{d}" for d in libdirs], "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
         "-L/opt/rocm/lib", "-lamdhip64",

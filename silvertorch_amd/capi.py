@@ -57,6 +57,17 @@ SIGNATURES = {
     "st_fused_kmean_ann_noalloc": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, ctypes.c_int,
                                                   _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp,
                                                   _vp]),
+    "st_int4_quantize": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, ctypes.c_int, _vp, _vp, _vp, _vp]),
+    "st_int4_matvec": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, ctypes.c_int, _i64, _i64, _i64, _i64, _vp,
+                                      ctypes.c_int, _vp]),
+    "st_target_logprobs_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "st_target_logprobs": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
+                                          ctypes.c_double, *[_vp] * 8]),
+    "st_target_logprobs_backward": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
+                                                   ctypes.c_double, *[_vp] * 9]),
+    "st_cluster_route_workspace_bytes": (_i64, [_i64, _i64]),
+    "st_cluster_route": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, _i64, *[_vp] * 10]),
+    "st_cluster_route_backward": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, _i64, *[_vp] * 9]),
     "st_bloom_index_search_batch_counts": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
     "st_search_plan_partial_items": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp,
                                                     _i64p, _i64p]),

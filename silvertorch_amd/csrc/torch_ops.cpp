@@ -12,9 +12,6 @@
 // (expression_query_parser_cuda.cu:27-44).
 #include <ATen/ATen.h>
 #include <ATen/core/CachingHostAllocator.h>
-#include <c10/hip/HIPFunctions.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <Python.h>
 #include <torch/library.h>
 
@@ -27,27 +24,15 @@
 #include <string>
 #include <vector>
 
-#include "../../include/silvertorch_hip.h"
+#include "torch_common.hpp"
 
 namespace {
 
 using at::Tensor;
 
-void check_st(int rc, const char* what) {
-  TORCH_CHECK(rc == ST_OK, what, ": ", st_last_error());
-}
-
-void* current_stream(const Tensor& t) {
-  return static_cast<void*>(
-      c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream());
-}
-
-at::Device gpu_for_cpu_call() {
-  TORCH_CHECK(c10::hip::device_count() > 0,
-              "silvertorch_amd computes the bloom path with HIP kernels on an "
-              "MI355X; no GPU is visible to this process");
-  return at::Device(at::kCUDA, c10::hip::current_device());
-}
+using st_torch::check_st;
+using st_torch::current_stream;
+using st_torch::gpu_for_cpu_call;
 
 // ---------------------------------------------------------------- build
 
