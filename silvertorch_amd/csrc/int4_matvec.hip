@@ -9,6 +9,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <mutex>
+#include <type_traits>
 
 #include "score_ops.hpp"
 #include "st_errors.hpp"
@@ -19,6 +21,14 @@ int cu_count();
 namespace {
 
 constexpr int kBlock = 32;  // columns of 16 bytes
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kMaxTileColumns = 64;         // vectors' parts a pass takes
+constexpr int kVectorLds = 64 * 1024;       // the vectors' share of LDS
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct MatvecArgs {
   const uint8_t* packed;
@@ -26,7 +36,15 @@ struct MatvecArgs {
   const uint8_t* zeros;  // null: 8
   const void* x;
   void* y;
-  int64_t rows, dim, queries, group, groups, row_bytes;
+  int64_t rows, queries;
+  int dim, groups, row_bytes;
+  int blocks;            // of 32 columns
+  int group_blocks;      // a group's
+  uint32_t group_magic;  // block / group_blocks = block * magic >> 32
+  int parts;             // float16 parts a vector's element is split into
+  int queries_at_once;
+  int phase_blocks;      // blocks whose vectors are in LDS at once, a multiple of 16
+  int split;             // waves that share a row's columns
   int scale_type, x_type, y_type;
 };
 
@@ -45,24 +63,296 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, float v, int type)
     store_score<ST_SCORE_BF16>(p, i, v);
 }
 
-// A thread per table row and query.
-__global__ __launch_bounds__(256) void matvec_kernel(MatvecArgs a) {
-  const int64_t total = a.rows * a.queries;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t b = i / a.rows, n = i - b * a.rows;
-    float y = 0.0f;
-    for (int64_t g = 0; g < a.groups; ++g) {
-      const float zero = a.zeros != nullptr ? static_cast<float>(a.zeros[n * a.groups + g]) : 8.0f;
-      const int64_t end = min((g + 1) * a.group, a.dim);
-      const float scale = load_any(a.scales, n * a.groups + g, a.scale_type);
-      for (int64_t d = g * a.group; d < end; ++d) {
-        const uint32_t byte = a.packed[n * a.row_bytes + d / 2];
-        const float q = static_cast<float>((d & 1) ? byte >> 4 : byte & 15u);
-        y = fmaf((q - zero) * scale, load_any(a.x, b * a.dim + d, a.x_type), y);
+// Lane groups of 16 and registers transposed: register i of lane group g
+// becomes register g of lane group i.
+__device__ __forceinline__ u32x4 transpose4(u32x4 d) {
+  auto s02 = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false);
+  auto s13 = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
+  auto s01 = __builtin_amdgcn_permlane16_swap(s02[0], s13[0], false, false);
+  auto s23 = __builtin_amdgcn_permlane16_swap(s02[1], s13[1], false, false);
+  return u32x4{s01[0], s01[1], s23[0], s23[1]};
+}
+
+// Register i: the value of lane group i, in all four groups.
+__device__ __forceinline__ u32x4 broadcast4(uint32_t v) {
+  auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  auto a = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false);
+  auto b = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
+  return u32x4{a[0], a[1], b[0], b[1]};
+}
+
+__device__ __forceinline__ half2_t as_half2(uint32_t u) {
+  half2_t h;
+  __builtin_memcpy(&h, &u, 4);
+  return h;
+}
+
+// Eight codes less their zero point, exact in float16, in the order 0 4 1 5 2 6
+// 3 7.  A code put into the low bits of 1024.0 reads 1024 + q, one four bits
+// further up 1024 + 16 q.  low = -(1024 + zero), high = -(64 + zero).
+__device__ __forceinline__ half8_t codes_of(uint32_t w, half2_t low, half2_t high) {
+  const half2_t sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
+  const uint32_t v = w >> 8;
+  const half2_t a = as_half2((w & 0x000F000Fu) | 0x64006400u) + low;
+  const half2_t b = __builtin_elementwise_fma(as_half2((w & 0x00F000F0u) | 0x64006400u), sixteenth, high);
+  const half2_t c = as_half2((v & 0x000F000Fu) | 0x64006400u) + low;
+  const half2_t d = __builtin_elementwise_fma(as_half2((v & 0x00F000F0u) | 0x64006400u), sixteenth, high);
+  return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// The power of two that brings a vector's largest finite element into [2^14,
+// 2^15), as an exponent.
+__device__ __forceinline__ int shift_of(float largest) {
+  if (largest == 0.0f) return 0;
+  int e;
+  frexpf(largest, &e);
+  return min(15 - e, 126);
+}
+
+// Part `part` of an element (x 2^shift): its float16, or what that leaves out
+// times 2^11.
+__device__ __forceinline__ _Float16 part_of(float x, int part) {
+  const _Float16 h = static_cast<_Float16>(x);
+  if (part == 0) return h;
+  const float left = x - static_cast<float>(h);
+  return static_cast<_Float16>(__builtin_isfinite(left) ? left * 2048.0f : 0.0f);
+}
+
+// A step's weights of one wave: T tiles of 16 rows by J times 128 columns.
+// Lane l reads row l % 16, 16 bytes at block 4 j + l / 16.
+template <int T, int J>
+struct Step {
+  u32x4 w[T][J];
+  uint32_t scale[T][J];  // as stored
+  uint32_t zero[T][J];
+};
+
+// Products on the matrix cores: a wave takes 16 table rows as the columns of a
+// 16x16x32 product and up to 16 vectors' parts (C tiles of them) as its rows.
+// Vectors are held in LDS as float16: scaled by a power of two (undone at the
+// end) so that bfloat16 values stay exact down to 2^-28 of the largest, and
+// float32 ones split in two parts, which leaves 2^-22 of each out; they lie in
+// the order that the codes come in.  Codes less zero points are exact in
+// float16; each block of 32 columns (COARSE: each group, of whole 128 columns)
+// is summed by the matrix core in 32 bits and added to the row's sum times its
+// scale in 32 bits.
+// A row's 16 bytes at a time would leave a wave's load scattered, so four
+// blocks are read per row and lane groups exchange registers (transpose4).
+// SPREAD: with few columns they are spread over the product's rows so that a
+// lane finds its own in element 0 (SPREAD 4), or 0 and 2 (SPREAD 2).
+// `split` waves share a row's columns and their sums meet in LDS.
+template <bool COARSE, bool WIDE, int T, int J, int C, int SPREAD>
+__global__ __launch_bounds__(kThreads, 2) void matvec_kernel(MatvecArgs a) {
+  extern __shared__ __align__(16) uint8_t lds_raw[];
+  __shared__ float largest[kMaxTileColumns];
+  u32x4* xs = reinterpret_cast<u32x4*>(lds_raw);  // [block][l / 16][column]
+  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, row16 = lane % 16, quarter = lane / 16;
+  const int64_t first_query = static_cast<int64_t>(blockIdx.y) * a.queries_at_once;
+  const int queries = static_cast<int>(min(static_cast<int64_t>(a.queries_at_once), a.queries - first_query));
+  const int columns = queries * a.parts;
+  const int steps4 = (a.blocks + 3) / 4;  // of 128 columns
+  const int phases = (a.blocks + a.phase_blocks - 1) / a.phase_blocks;
+
+  if (a.x_type != ST_SCORE_F16) {
+    for (int q = wave; q < queries; q += kWaves) {
+      float top = 0.0f;
+      for (int d = lane; d < a.dim; d += 64) {
+        const float v = fabsf(load_any(a.x, (first_query + q) * a.dim + d, a.x_type));
+        if (v < __builtin_inff()) top = fmaxf(top, v);
+      }
+      top = wave_max(top);
+      if (lane == 0) largest[q] = top;
+    }
+    __syncthreads();
+  }
+
+  float* sums = reinterpret_cast<float*>(xs + static_cast<int64_t>(min(a.phase_blocks, steps4 * 4)) * 4 * columns);
+
+  auto fill = [&](int phase) {
+    const int first = phase * a.phase_blocks;
+    const int count = min(a.phase_blocks, steps4 * 4 - first);
+    for (int i = tid; i < count * 4 * columns; i += kThreads) {
+      const int c = i % columns, at = i / columns;
+      const int q = c / a.parts, part = c - q * a.parts;
+      const int d0 = first * kBlock + at * 8;
+      const int shift = a.x_type == ST_SCORE_F16 ? 0 : shift_of(largest[q]);
+      half8_t h;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int from = (k >> 1) + 4 * (k & 1);
+        const float v = d0 + from < a.dim ? load_any(a.x, (first_query + q) * a.dim + d0 + from, a.x_type) : 0.0f;
+        h[k] = part_of(ldexpf(v, shift), part);
+      }
+      u32x4 raw;
+      __builtin_memcpy(&raw, &h, 16);
+      xs[i] = raw;
+    }
+  };
+
+  const int row_waves = kWaves / a.split;
+  const int mine = wave / a.split, turn = wave % a.split;
+  const int64_t rows_at_once = static_cast<int64_t>(row_waves) * T * 16;
+  const half2_t low8 = as_half2(0xE408E408u), high8 = as_half2(0xD480D480u);  // -(1024 + 8), -(64 + 8)
+
+  auto load = [&](int64_t base, int step, Step<T, J>& s) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const int64_t row = min(base + t * 16 + row16, a.rows - 1);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int block = min((step * J + j) * 4 + quarter, a.blocks - 1);
+        s.w[t][j] = *reinterpret_cast<const u32x4*>(a.packed + row * a.row_bytes + block * 16);
+        const uint32_t of = COARSE ? min((step * J + j) * 4, a.blocks - 1) : block;
+        const int64_t at = row * a.groups + (a.group_blocks == 1 ? of : __umulhi(of, a.group_magic));
+        s.scale[t][j] = WIDE ? static_cast<const uint32_t*>(a.scales)[at] : static_cast<const uint16_t*>(a.scales)[at];
+        if (a.zeros != nullptr) s.zero[t][j] = a.zeros[at];
       }
     }
-    store_any(a.y, i, y, a.y_type);
+  };
+
+  auto scale_of = [&](uint32_t raw) {
+    if constexpr (WIDE) return __uint_as_float(raw);
+    return a.scale_type == ST_SCORE_F16 ? score_of_bits<ST_SCORE_F16>(raw) : score_of_bits<ST_SCORE_BF16>(raw);
+  };
+
+  f32x4 acc[T][C];
+  auto compute = [&](int step, int first_block, const Step<T, J>& s) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int block0 = (step * J + j) * 4;
+      if (block0 >= a.blocks) break;
+      f32x4 part[T][C];
+      u32x4 w[T], zero[T], scale[T];
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        w[t] = transpose4(s.w[t][j]);
+        if constexpr (!COARSE) {
+          scale[t] = broadcast4(__float_as_uint(scale_of(s.scale[t][j])));
+          if (a.zeros != nullptr) zero[t] = broadcast4(s.zero[t][j] * 0x00010001u);
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) part[t][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int block = block0 + i;
+        if (block >= a.blocks) break;
+        half8_t x[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const int column = min(c * 16 + row16 / SPREAD, columns - 1);
+          const u32x4 raw = xs[((block - first_block) * 4 + quarter) * columns + column];
+          __builtin_memcpy(&x[c], &raw, 16);
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          half2_t low = low8, high = high8;
+          if (a.zeros != nullptr) {
+            const uint32_t z = COARSE ? s.zero[t][j] * 0x00010001u : zero[t][i];
+            low = as_half2(z | 0xE400E400u);
+            high = low + half2_t{static_cast<_Float16>(960.0f), static_cast<_Float16>(960.0f)};
+          }
+          const half8_t q = codes_of(w[t][i], low, high);
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            if constexpr (COARSE) {
+              part[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[c], q, part[t][c], 0, 0, 0);
+            } else {
+              const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[c], q, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+              for (int e = 0; e < 4; e += SPREAD)
+                acc[t][c][e] = fmaf(__uint_as_float(scale[t][i]), p[e], acc[t][c][e]);
+            }
+          }
+        }
+      }
+      if constexpr (COARSE) {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; e += SPREAD) acc[t][c][e] = fmaf(scale_of(s.scale[t][j]), part[t][c][e], acc[t][c][e]);
+      }
+    }
+  };
+
+  // y of the wave's tiles from its sums
+  auto store = [&](int64_t base) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const int64_t row = base + t * 16 + row16;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int e = 0; e < 4; e += SPREAD) {
+          const int column = c * 16 + (quarter * 4 + e) / SPREAD;
+          if (a.parts == 2 && (column & 1)) continue;
+          const int q = column / a.parts;
+          if (q >= queries || row >= a.rows) continue;
+          float v = acc[t][c][e];
+          if constexpr (SPREAD < 4)
+            if (a.parts == 2) v = fmaf(acc[t][c][(e + SPREAD) % 4], 1.0f / 2048.0f, v);
+          if (a.x_type != ST_SCORE_F16) v = ldexpf(v, -shift_of(largest[q]));
+          store_any(a.y, (first_query + q) * a.rows + row, v, a.y_type);
+        }
+      }
+    }
+  };
+
+  if (phases == 1) {
+    fill(0);
+    __syncthreads();
+  }
+  for (int64_t base0 = static_cast<int64_t>(blockIdx.x) * rows_at_once; base0 < a.rows;
+       base0 += static_cast<int64_t>(gridDim.x) * rows_at_once) {
+    const int64_t base = base0 + static_cast<int64_t>(mine) * T * 16;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int c = 0; c < C; ++c) acc[t][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int phase = 0; phase < phases; ++phase) {
+      if (phases > 1) {
+        __syncthreads();
+        fill(phase);
+        __syncthreads();
+      }
+      const int first_block = phase * a.phase_blocks;
+      const int end_block = min(first_block + a.phase_blocks, a.blocks);
+      const int first_step = first_block / (4 * J), end_step = (end_block + 4 * J - 1) / (4 * J);
+      for (int step = first_step + turn; step < end_step; step += a.split) {
+        Step<T, J> s;
+        load(base, step, s);
+        compute(step, first_block, s);
+      }
+    }
+    if (a.split == 1) {
+      store(base);
+    } else {
+      // the sums of the waves that share the rows, added in order by the first
+      constexpr int kEach = T * C * 4;
+      float* own = sums + wave * 64 * kEach;
+      if (turn > 0) {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) own[((t * C + c) * 4 + e) * 64 + lane] = acc[t][c][e];
+      }
+      __syncthreads();
+      if (turn == 0) {
+        for (int w = 1; w < a.split; ++w)
+#pragma unroll
+          for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[t][c][e] += own[w * 64 * kEach + ((t * C + c) * 4 + e) * 64 + lane];
+        store(base);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -135,6 +425,67 @@ void check_launch(const char* what) {
   if (e != hipSuccess) throw Error(ST_ERR_HIP, cat(what, " launch failed: ", hipGetErrorString(e)));
 }
 
+template <bool COARSE, bool WIDE, int T, int J, int C, int SPREAD>
+void launch_shape(const MatvecArgs& a, int columns, hipStream_t s) {
+  const int64_t rows_at_once = static_cast<int64_t>(kWaves / a.split) * T * 16;
+  const int64_t passes = (a.queries + a.queries_at_once - 1) / a.queries_at_once;
+  const int64_t grid = std::min<int64_t>((a.rows + rows_at_once - 1) / rows_at_once, 2 * cu_count());
+  const int lds_blocks = std::min(a.phase_blocks, (a.blocks + 3) / 4 * 4);
+  size_t lds = static_cast<size_t>(lds_blocks) * 64 * columns;
+  if (a.split > 1) lds += sizeof(float) * kWaves * 64 * T * C * 4;
+  const auto kernel = matvec_kernel<COARSE, WIDE, T, J, C, SPREAD>;
+  if (lds > 48 * 1024) {
+    static std::once_flag once;
+    std::call_once(once, [&] {
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+      if (e != hipSuccess) throw Error(ST_ERR_HIP, cat("hipFuncSetAttribute failed: ", hipGetErrorString(e)));
+    });
+  }
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid), static_cast<unsigned>(passes)),
+                     dim3(kThreads), lds, s, a);
+}
+
+template <bool COARSE, bool WIDE, int T, int J>
+void launch_columns(const MatvecArgs& a, int columns, hipStream_t s) {
+  if (columns <= 4 && a.parts == 1)
+    launch_shape<COARSE, WIDE, T, J, 1, 4>(a, columns, s);
+  else if (columns <= 8)
+    launch_shape<COARSE, WIDE, T, J, 1, 2>(a, columns, s);
+  else if (columns <= 16)
+    launch_shape<COARSE, WIDE, T, J, 1, 1>(a, columns, s);
+  else if (columns <= 32)
+    launch_shape<COARSE, WIDE, T, J, 2, 1>(a, columns, s);
+  else
+    launch_shape<COARSE, WIDE, T, J, 4, 1>(a, columns, s);
+}
+
+void launch_matvec(MatvecArgs& a, hipStream_t s) {
+  a.parts = a.x_type == ST_SCORE_F32 ? 2 : 1;
+  a.queries_at_once = static_cast<int>(std::min<int64_t>(a.queries, kMaxTileColumns / a.parts));
+  const int columns = a.queries_at_once * a.parts;
+  // block / group_blocks: the reciprocal rounded up is exact while block *
+  // group_blocks stays below 2^32 (blocks are at most 2^16); 1 has none
+  a.group_magic = a.group_blocks == 1 ? 0 : static_cast<uint32_t>((0x100000000ull + a.group_blocks - 1) / a.group_blocks);
+  a.phase_blocks = std::max(16, kVectorLds / (64 * columns) / 16 * 16);
+  const bool coarse = a.group_blocks % 4 == 0;
+  const bool is_long = a.blocks > 8;
+  a.split = 1;
+  if (is_long)
+    while (a.split < kWaves && (a.rows + 15) / 16 * a.split < 16 * cu_count()) a.split *= 2;
+  const bool wide = a.scale_type == ST_SCORE_F32;
+  auto launch = [&](auto coarse_, auto wide_) {
+    if (is_long)
+      launch_columns<coarse_(), wide_(), 1, 4>(a, columns, s);
+    else
+      launch_columns<coarse_(), wide_(), 4, 1>(a, columns, s);
+  };
+  if (coarse)
+    wide ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
+  else
+    wide ? launch(std::false_type{}, std::true_type{}) : launch(std::false_type{}, std::false_type{});
+}
+
 void check_type(int type, const char* what) {
   ST_CHECK(type == ST_SCORE_F32 || type == ST_SCORE_F16 || type == ST_SCORE_BF16, what,
            " must be float32, float16 or bfloat16");
@@ -142,7 +493,7 @@ void check_type(int type, const char* what) {
 
 void check_table(int64_t rows, int64_t dim, int64_t group) {
   ST_CHECK(rows >= 0 && dim >= 1, "a table has at least one column, got ", rows, " x ", dim);
-  ST_CHECK(dim < (1ll << 31), "columns must be below 2^31, got ", dim);
+  ST_CHECK(dim <= (1ll << 21), "columns must be at most 2^21, got ", dim);
   ST_CHECK(group >= kBlock && group % kBlock == 0, "group_size must be a positive multiple of ", kBlock, ", got ", group);
 }
 
@@ -180,14 +531,27 @@ extern "C" int st_int4_matvec(const uint8_t* packed, const void* scales, int sca
     check_type(x_type, "x");
     check_type(y_type, "the result");
     check_table(rows, dim, group_size);
-    ST_CHECK(queries >= 0, "negative sizes");
+    ST_CHECK(queries >= 0 && queries <= (1ll << 20), "vectors must be between 0 and 2^20, got ", queries);
     if (rows == 0 || queries == 0) return;
     ST_CHECK(packed && scales && x && y, "null device pointer");
     ST_CHECK(reinterpret_cast<uintptr_t>(packed) % 16 == 0, "the packed table must be 16-byte aligned");
-    MatvecArgs a{packed, scales, zeros, x, y, rows, dim, queries, group_size, (dim + group_size - 1) / group_size,
-                 (dim + kBlock - 1) / kBlock * (kBlock / 2), scale_type, x_type, y_type};
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((rows * queries + 255) / 256, 1 << 22));
-    hipLaunchKernelGGL(matvec_kernel, dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    MatvecArgs a{};
+    a.packed = packed;
+    a.scales = scales;
+    a.zeros = zeros;
+    a.x = x;
+    a.y = y;
+    a.rows = rows;
+    a.queries = queries;
+    a.dim = static_cast<int>(dim);
+    a.groups = static_cast<int>((dim + group_size - 1) / group_size);
+    a.blocks = static_cast<int>((dim + kBlock - 1) / kBlock);
+    a.row_bytes = a.blocks * (kBlock / 2);
+    a.group_blocks = static_cast<int>(std::min<int64_t>(group_size / kBlock, a.blocks));
+    a.scale_type = scale_type;
+    a.x_type = x_type;
+    a.y_type = y_type;
+    launch_matvec(a, static_cast<hipStream_t>(stream));
     check_launch("matvec_kernel");
   });
 }
