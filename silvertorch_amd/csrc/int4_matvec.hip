@@ -24,7 +24,8 @@ constexpr int kBlock = 32;  // columns of 16 bytes
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTileColumns = 64;         // vectors' parts a pass takes
-constexpr int kVectorLds = 64 * 1024;       // the vectors' share of LDS
+constexpr int kVectorLds = 64 * 1024;       // the vectors' share of LDS, in phases
+constexpr int kWholeVectorLds = 128 * 1024;  // or, if they fit at once
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
@@ -90,13 +91,15 @@ __device__ __forceinline__ half2_t as_half2(uint32_t u) {
 // Eight codes less their zero point, exact in float16, in the order 0 4 1 5 2 6
 // 3 7.  A code put into the low bits of 1024.0 reads 1024 + q, one four bits
 // further up 1024 + 16 q.  low = -(1024 + zero), high = -(64 + zero).
-__device__ __forceinline__ half8_t codes_of(uint32_t w, half2_t low, half2_t high) {
+// `base` is 0x64006400 in a vector register: with the mask in a scalar one, and
+// and or are one instruction.
+__device__ __forceinline__ half8_t codes_of(uint32_t w, uint32_t base, half2_t low, half2_t high) {
   const half2_t sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
   const uint32_t v = w >> 8;
-  const half2_t a = as_half2((w & 0x000F000Fu) | 0x64006400u) + low;
-  const half2_t b = __builtin_elementwise_fma(as_half2((w & 0x00F000F0u) | 0x64006400u), sixteenth, high);
-  const half2_t c = as_half2((v & 0x000F000Fu) | 0x64006400u) + low;
-  const half2_t d = __builtin_elementwise_fma(as_half2((v & 0x00F000F0u) | 0x64006400u), sixteenth, high);
+  const half2_t a = as_half2((w & 0x000F000Fu) | base) + low;
+  const half2_t b = __builtin_elementwise_fma(as_half2((w & 0x00F000F0u) | base), sixteenth, high);
+  const half2_t c = as_half2((v & 0x000F000Fu) | base) + low;
+  const half2_t d = __builtin_elementwise_fma(as_half2((v & 0x00F000F0u) | base), sixteenth, high);
   return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
@@ -108,6 +111,9 @@ __device__ __forceinline__ int shift_of(float largest) {
   frexpf(largest, &e);
   return min(15 - e, 126);
 }
+
+// 2^e for e in [-126, 127]
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 // Part `part` of an element (x 2^shift): its float16, or what that leaves out
 // times 2^11.
@@ -138,74 +144,157 @@ struct Step {
 // scale in 32 bits.
 // A row's 16 bytes at a time would leave a wave's load scattered, so four
 // blocks are read per row and lane groups exchange registers (transpose4).
-// SPREAD: with few columns they are spread over the product's rows so that a
-// lane finds its own in element 0 (SPREAD 4), or 0 and 2 (SPREAD 2).
+// SPREAD 4: up to four columns are spread over the product's rows so that a
+// lane finds its own in element 0 alone.
 // `split` waves share a row's columns and their sums meet in LDS.
-template <bool COARSE, bool WIDE, int T, int J, int C, int SPREAD>
+template <bool COARSE, bool WIDE, bool ZEROS, int T, int J, int C, int SPREAD>
 __global__ __launch_bounds__(kThreads, 2) void matvec_kernel(MatvecArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
-  __shared__ float largest[kMaxTileColumns];
+  __shared__ uint32_t largest[kMaxTileColumns];
   u32x4* xs = reinterpret_cast<u32x4*>(lds_raw);  // [block][l / 16][column]
-  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, row16 = lane % 16, quarter = lane / 16;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, row16 = lane % 16, quarter = lane / 16;
   const int64_t first_query = static_cast<int64_t>(blockIdx.y) * a.queries_at_once;
   const int queries = static_cast<int>(min(static_cast<int64_t>(a.queries_at_once), a.queries - first_query));
   const int columns = queries * a.parts;
   const int steps4 = (a.blocks + 3) / 4;  // of 128 columns
   const int phases = (a.blocks + a.phase_blocks - 1) / a.phase_blocks;
 
-  if (a.x_type != ST_SCORE_F16) {
-    for (int q = wave; q < queries; q += kWaves) {
-      float top = 0.0f;
-      for (int d = lane; d < a.dim; d += 64) {
-        const float v = fabsf(load_any(a.x, (first_query + q) * a.dim + d, a.x_type));
-        if (v < __builtin_inff()) top = fmaxf(top, v);
-      }
-      top = wave_max(top);
-      if (lane == 0) largest[q] = top;
-    }
-    __syncthreads();
-  }
-
   float* sums = reinterpret_cast<float*>(xs + static_cast<int64_t>(min(a.phase_blocks, steps4 * 4)) * 4 * columns);
 
-  auto fill = [&](int phase) {
-    const int first = phase * a.phase_blocks;
-    const int count = min(a.phase_blocks, steps4 * 4 - first);
-    for (int i = tid; i < count * 4 * columns; i += kThreads) {
-      const int c = i % columns, at = i / columns;
-      const int q = c / a.parts, part = c - q * a.parts;
-      const int d0 = first * kBlock + at * 8;
-      const int shift = a.x_type == ST_SCORE_F16 ? 0 : shift_of(largest[q]);
+  // Eight elements of vector q from column d on, 0 past the last.
+  auto load_x = [&](int q, int d, float v[8]) {
+    const int64_t at = (first_query + q) * a.dim + d;
+    if (d + 8 <= a.dim) {
+      if (a.x_type == ST_SCORE_F32)
+        unpack8<ST_SCORE_F32>(load_raw8<ST_SCORE_F32>(a.x, at), v);
+      else if (a.x_type == ST_SCORE_F16)
+        unpack8<ST_SCORE_F16>(load_raw8<ST_SCORE_F16>(a.x, at), v);
+      else
+        unpack8<ST_SCORE_BF16>(load_raw8<ST_SCORE_BF16>(a.x, at), v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = d + i < a.dim ? load_any(a.x, at + i, a.x_type) : 0.0f;
+    }
+  };
+
+  auto top_of = [](const float v[8]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float x = fabsf(v[k]);
+      top = x < __builtin_inff() ? fmaxf(top, x) : top;
+    }
+    return top;
+  };
+  // Puts unit i (eight elements of a vector, vectors fastest) of a phase into
+  // LDS as its parts.
+  auto put = [&](int i, int q, const float v[8]) {
+    const float scale = a.x_type == ST_SCORE_F16 ? 1.0f : power_of_two(shift_of(__uint_as_float(largest[q])));
+    for (int part = 0; part < a.parts; ++part) {
       half8_t h;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int from = (k >> 1) + 4 * (k & 1);
-        const float v = d0 + from < a.dim ? load_any(a.x, (first_query + q) * a.dim + d0 + from, a.x_type) : 0.0f;
-        h[k] = part_of(ldexpf(v, shift), part);
-      }
+      for (int k = 0; k < 8; ++k) h[k] = part_of(v[(k >> 1) + 4 * (k & 1)] * scale, part);
       u32x4 raw;
       __builtin_memcpy(&raw, &h, 16);
-      xs[i] = raw;
+      xs[i * a.parts + part] = raw;
     }
+  };
+  auto fill = [&](int phase) {
+    const int first = phase * a.phase_blocks;
+    const int count = min(a.phase_blocks, steps4 * 4 - first) * 4 * queries;
+    for (int i = tid; i < count; i += kThreads) {
+      const int at = i / queries, q = i - at * queries;
+      float v[8];
+      load_x(q, first * kBlock + at * 8, v);
+      put(i, q, v);
+    }
+  };
+  // Each vector's largest finite element goes to largest[] (floats that are
+  // not negative are in the order of their bits), and, where one phase takes
+  // them all, the vectors to LDS: from registers, if they fit.
+  auto prepare = [&] {
+    constexpr int kHeld = 4;
+    const int units = steps4 * 16 * queries;
+    const bool held = phases == 1 && units <= kHeld * kThreads;
+    const bool scaled = a.x_type != ST_SCORE_F16;
+    float v[kHeld][8];
+    if (scaled) {
+      if (tid < queries) largest[tid] = 0;
+      __syncthreads();
+    }
+    if (held) {
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) {
+        const int i = tid + h * kThreads, at = i / queries;
+        if (i < units) load_x(i - at * queries, at * 8, v[h]);
+      }
+    }
+    if (scaled) {
+      if (held && queries == 1) {
+        float top = 0.0f;
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h)
+          if (tid + h * kThreads < units) top = fmaxf(top, top_of(v[h]));
+        top = wave_max(top);
+        if (lane == 0) atomicMax(&largest[0], __float_as_uint(top));
+      } else if (held) {
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h) {
+          const int i = tid + h * kThreads;
+          if (i < units) atomicMax(&largest[i % queries], __float_as_uint(top_of(v[h])));
+        }
+      } else {
+        for (int i = tid; i < units; i += kThreads) {
+          const int at = i / queries, q = i - at * queries;
+          float w[8];
+          load_x(q, at * 8, w);
+          atomicMax(&largest[q], __float_as_uint(top_of(w)));
+        }
+      }
+      __syncthreads();
+    }
+    if (held) {
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) {
+        const int i = tid + h * kThreads;
+        if (i < units) put(i, i % queries, v[h]);
+      }
+    } else if (phases == 1) {
+      fill(0);
+    }
+    __syncthreads();
   };
 
   const int row_waves = kWaves / a.split;
   const int mine = wave / a.split, turn = wave % a.split;
   const int64_t rows_at_once = static_cast<int64_t>(row_waves) * T * 16;
+  uint32_t base1024 = 0x64006400u;
+  asm volatile("" : "+v"(base1024));
   const half2_t low8 = as_half2(0xE408E408u), high8 = as_half2(0xD480D480u);  // -(1024 + 8), -(64 + 8)
 
+  // Addresses are a scalar base and a 32-bit offset per lane.  Rows and blocks
+  // past the last are read as the last, so that every load is issued on every
+  // path: a load behind a branch would make the compiler wait for all of them.
   auto load = [&](int64_t base, int step, Step<T, J>& s) {
+    const int64_t from = min(base, a.rows - 1);
+    const uint32_t last = static_cast<uint32_t>(min(a.rows - 1 - from, static_cast<int64_t>(T * 16)));
+    const uint8_t* packed = a.packed + from * a.row_bytes;
+    const int64_t scale0 = from * a.groups;
+    const uint8_t* scales = static_cast<const uint8_t*>(a.scales) + scale0 * (WIDE ? 4 : 2);
+    const uint8_t* zeros = a.zeros + scale0;
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      const int64_t row = min(base + t * 16 + row16, a.rows - 1);
+      const uint32_t row = min(static_cast<uint32_t>(t * 16 + row16), last);
+      const uint32_t bytes = __umul24(row, a.row_bytes), groups = __umul24(row, a.groups);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const int block = min((step * J + j) * 4 + quarter, a.blocks - 1);
-        s.w[t][j] = *reinterpret_cast<const u32x4*>(a.packed + row * a.row_bytes + block * 16);
+        const uint32_t block = min((step * J + j) * 4 + quarter, a.blocks - 1);
+        s.w[t][j] = *reinterpret_cast<const u32x4*>(packed + (bytes + block * 16));
         const uint32_t of = COARSE ? min((step * J + j) * 4, a.blocks - 1) : block;
-        const int64_t at = row * a.groups + (a.group_blocks == 1 ? of : __umulhi(of, a.group_magic));
-        s.scale[t][j] = WIDE ? static_cast<const uint32_t*>(a.scales)[at] : static_cast<const uint16_t*>(a.scales)[at];
-        if (a.zeros != nullptr) s.zero[t][j] = a.zeros[at];
+        const uint32_t at = groups + (a.group_blocks == 1 ? of : __umulhi(of, a.group_magic));
+        s.scale[t][j] = WIDE ? *reinterpret_cast<const uint32_t*>(scales + at * 4)
+                             : *reinterpret_cast<const uint16_t*>(scales + at * 2);
+        if constexpr (ZEROS) s.zero[t][j] = zeros[at];
       }
     }
   };
@@ -228,7 +317,7 @@ __global__ __launch_bounds__(kThreads, 2) void matvec_kernel(MatvecArgs a) {
         w[t] = transpose4(s.w[t][j]);
         if constexpr (!COARSE) {
           scale[t] = broadcast4(__float_as_uint(scale_of(s.scale[t][j])));
-          if (a.zeros != nullptr) zero[t] = broadcast4(s.zero[t][j] * 0x00010001u);
+          if constexpr (ZEROS) zero[t] = broadcast4(s.zero[t][j] * 0x00010001u);
         }
 #pragma unroll
         for (int c = 0; c < C; ++c) part[t][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -247,12 +336,12 @@ __global__ __launch_bounds__(kThreads, 2) void matvec_kernel(MatvecArgs a) {
 #pragma unroll
         for (int t = 0; t < T; ++t) {
           half2_t low = low8, high = high8;
-          if (a.zeros != nullptr) {
+          if constexpr (ZEROS) {
             const uint32_t z = COARSE ? s.zero[t][j] * 0x00010001u : zero[t][i];
             low = as_half2(z | 0xE400E400u);
             high = low + half2_t{static_cast<_Float16>(960.0f), static_cast<_Float16>(960.0f)};
           }
-          const half8_t q = codes_of(w[t][i], low, high);
+          const half8_t q = codes_of(w[t][i], base1024, low, high);
 #pragma unroll
           for (int c = 0; c < C; ++c) {
             if constexpr (COARSE) {
@@ -277,36 +366,87 @@ __global__ __launch_bounds__(kThreads, 2) void matvec_kernel(MatvecArgs a) {
     }
   };
 
+  // The wave's steps in order: row groups, phases, steps of 4 J blocks.  The
+  // next step's weights are loaded before a step is computed (the first ones
+  // before the vectors are in LDS).
+  struct Place {
+    int64_t base0;
+    int phase, step;
+  };
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * rows_at_once;
+  auto first_step = [&](int phase) { return phase * (a.phase_blocks / (4 * J)) + turn; };
+  auto end_step = [&](int phase) {
+    return (min((phase + 1) * a.phase_blocks, a.blocks) + 4 * J - 1) / (4 * J);
+  };
+  auto settle = [&](Place& p) {  // the first step at or after p
+    while (p.base0 < a.rows && p.step >= end_step(p.phase)) {
+      if (++p.phase == phases) {
+        p.phase = 0;
+        p.base0 += stride;
+      }
+      p.step = first_step(p.phase);
+    }
+  };
+  const int64_t tile0 = static_cast<int64_t>(mine) * T * 16;
+  Step<T, J> next;
+  Place ahead{static_cast<int64_t>(blockIdx.x) * rows_at_once, 0, first_step(0)};
+  settle(ahead);
+  load(ahead.base0 + tile0, ahead.step, next);
+
+  prepare();
+  // what undoes the scaling of the vectors whose sums this lane holds
+  float unscale[C][4];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; e += SPREAD) {
+      const int q = min((c * 16 + (quarter * 4 + e) / SPREAD) / a.parts, queries - 1);
+      unscale[c][e] = a.x_type == ST_SCORE_F16 ? 1.0f : power_of_two(-shift_of(__uint_as_float(largest[q])));
+    }
+
   // y of the wave's tiles from its sums
+  const bool y_wide = a.y_type == ST_SCORE_F32;
+  char* const y = static_cast<char*>(a.y) + first_query * a.rows * (y_wide ? 4 : 2);
+  auto put_y = [&](char* at, float v) {
+    if (y_wide)
+      *reinterpret_cast<float*>(at) = v;
+    else
+      *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(
+          a.y_type == ST_SCORE_F16 ? score_bits<ST_SCORE_F16>(v) : score_bits<ST_SCORE_BF16>(v));
+  };
   auto store = [&](int64_t base) {
+    if constexpr (T == 4 && C == 1 && SPREAD == 4) {
+      // one vector: every lane group has its sums, and stores one tile of the
+      // four, so that a wave stores 64 adjacent results
+      if (columns == 1) {
+        float v = 0.0f;
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-      const int64_t row = base + t * 16 + row16;
+        for (int t = 0; t < T; ++t) v = quarter == t ? static_cast<float>(acc[t][0][0]) : v;
+        if (base + lane < a.rows) put_y(y + (base + lane) * (y_wide ? 4 : 2), v * unscale[0][0]);
+        return;
+      }
+    }
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
+    for (int c = 0; c < C; ++c) {
 #pragma unroll
-        for (int e = 0; e < 4; e += SPREAD) {
-          const int column = c * 16 + (quarter * 4 + e) / SPREAD;
-          if (a.parts == 2 && (column & 1)) continue;
-          const int q = column / a.parts;
-          if (q >= queries || row >= a.rows) continue;
+      for (int e = 0; e < 4; e += SPREAD) {
+        const int column = c * 16 + (quarter * 4 + e) / SPREAD;
+        const int q = a.parts == 2 ? column >> 1 : column;
+        const bool mine_ = (a.parts == 1 || (column & 1) == 0) && q < queries;
+        char* at = y + (q * a.rows + base + row16) * (y_wide ? 4 : 2);
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
           float v = acc[t][c][e];
-          if constexpr (SPREAD < 4)
-            if (a.parts == 2) v = fmaf(acc[t][c][(e + SPREAD) % 4], 1.0f / 2048.0f, v);
-          if (a.x_type != ST_SCORE_F16) v = ldexpf(v, -shift_of(largest[q]));
-          store_any(a.y, (first_query + q) * a.rows + row, v, a.y_type);
+          if constexpr (SPREAD == 1)
+            if (a.parts == 2) v = fmaf(acc[t][c][(e + 1) % 4], 1.0f / 2048.0f, v);
+          if (mine_ && base + t * 16 + row16 < a.rows) put_y(at + t * 16 * (y_wide ? 4 : 2), v * unscale[c][e]);
         }
       }
     }
   };
 
-  if (phases == 1) {
-    fill(0);
-    __syncthreads();
-  }
-  for (int64_t base0 = static_cast<int64_t>(blockIdx.x) * rows_at_once; base0 < a.rows;
-       base0 += static_cast<int64_t>(gridDim.x) * rows_at_once) {
-    const int64_t base = base0 + static_cast<int64_t>(mine) * T * 16;
+  for (int64_t base0 = static_cast<int64_t>(blockIdx.x) * rows_at_once; base0 < a.rows; base0 += stride) {
+    const int64_t base = base0 + tile0;
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
@@ -317,13 +457,12 @@ __global__ __launch_bounds__(kThreads, 2) void matvec_kernel(MatvecArgs a) {
         fill(phase);
         __syncthreads();
       }
-      const int first_block = phase * a.phase_blocks;
-      const int end_block = min(first_block + a.phase_blocks, a.blocks);
-      const int first_step = first_block / (4 * J), end_step = (end_block + 4 * J - 1) / (4 * J);
-      for (int step = first_step + turn; step < end_step; step += a.split) {
-        Step<T, J> s;
-        load(base, step, s);
-        compute(step, first_block, s);
+      for (int step = first_step(phase); step < end_step(phase); step += a.split) {
+        const Step<T, J> now = next;
+        ahead.step += a.split;
+        settle(ahead);
+        load(ahead.base0 + tile0, ahead.step, next);
+        compute(step, phase * a.phase_blocks, now);
       }
     }
     if (a.split == 1) {
@@ -425,39 +564,44 @@ void check_launch(const char* what) {
   if (e != hipSuccess) throw Error(ST_ERR_HIP, cat(what, " launch failed: ", hipGetErrorString(e)));
 }
 
-template <bool COARSE, bool WIDE, int T, int J, int C, int SPREAD>
+template <bool COARSE, bool WIDE, bool ZEROS, int T, int J, int C, int SPREAD>
 void launch_shape(const MatvecArgs& a, int columns, hipStream_t s) {
   const int64_t rows_at_once = static_cast<int64_t>(kWaves / a.split) * T * 16;
   const int64_t passes = (a.queries + a.queries_at_once - 1) / a.queries_at_once;
-  const int64_t grid = std::min<int64_t>((a.rows + rows_at_once - 1) / rows_at_once, 2 * cu_count());
   const int lds_blocks = std::min(a.phase_blocks, (a.blocks + 3) / 4 * 4);
   size_t lds = static_cast<size_t>(lds_blocks) * 64 * columns;
   if (a.split > 1) lds += sizeof(float) * kWaves * 64 * T * C * 4;
-  const auto kernel = matvec_kernel<COARSE, WIDE, T, J, C, SPREAD>;
+  const auto kernel = matvec_kernel<COARSE, WIDE, ZEROS, T, J, C, SPREAD>;
   if (lds > 48 * 1024) {
     static std::once_flag once;
     std::call_once(once, [&] {
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 512);
       if (e != hipSuccess) throw Error(ST_ERR_HIP, cat("hipFuncSetAttribute failed: ", hipGetErrorString(e)));
     });
   }
+  // as many workgroups as a CU holds, by registers and LDS
+  static const int by_registers = [&] {
+    int n = 0;
+    const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, 0);
+    return e == hipSuccess && n > 0 ? n : 1;
+  }();
+  const int64_t per_cu = std::max<int64_t>(1, std::min<int64_t>(by_registers, 160 * 1024 / (lds + 512)));
+  const int64_t grid = std::min<int64_t>((a.rows + rows_at_once - 1) / rows_at_once, per_cu * cu_count());
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid), static_cast<unsigned>(passes)),
                      dim3(kThreads), lds, s, a);
 }
 
-template <bool COARSE, bool WIDE, int T, int J>
+template <bool COARSE, bool WIDE, bool ZEROS, int T, int J>
 void launch_columns(const MatvecArgs& a, int columns, hipStream_t s) {
   if (columns <= 4 && a.parts == 1)
-    launch_shape<COARSE, WIDE, T, J, 1, 4>(a, columns, s);
-  else if (columns <= 8)
-    launch_shape<COARSE, WIDE, T, J, 1, 2>(a, columns, s);
+    launch_shape<COARSE, WIDE, ZEROS, T, J, 1, 4>(a, columns, s);
   else if (columns <= 16)
-    launch_shape<COARSE, WIDE, T, J, 1, 1>(a, columns, s);
+    launch_shape<COARSE, WIDE, ZEROS, T, J, 1, 1>(a, columns, s);
   else if (columns <= 32)
-    launch_shape<COARSE, WIDE, T, J, 2, 1>(a, columns, s);
+    launch_shape<COARSE, WIDE, ZEROS, T, J, 2, 1>(a, columns, s);
   else
-    launch_shape<COARSE, WIDE, T, J, 4, 1>(a, columns, s);
+    launch_shape<COARSE, WIDE, ZEROS, T == 4 ? 2 : T, T == 4 ? 2 : J, 4, 1>(a, columns, s);
 }
 
 void launch_matvec(MatvecArgs& a, hipStream_t s) {
@@ -467,23 +611,23 @@ void launch_matvec(MatvecArgs& a, hipStream_t s) {
   // block / group_blocks: the reciprocal rounded up is exact while block *
   // group_blocks stays below 2^32 (blocks are at most 2^16); 1 has none
   a.group_magic = a.group_blocks == 1 ? 0 : static_cast<uint32_t>((0x100000000ull + a.group_blocks - 1) / a.group_blocks);
-  a.phase_blocks = std::max(16, kVectorLds / (64 * columns) / 16 * 16);
+  const int whole = (a.blocks + 15) / 16 * 16;
+  a.phase_blocks = whole * 64 * columns <= kWholeVectorLds ? whole : std::max(16, kVectorLds / (64 * columns) / 16 * 16);
   const bool coarse = a.group_blocks % 4 == 0;
   const bool is_long = a.blocks > 8;
   a.split = 1;
   if (is_long)
-    while (a.split < kWaves && (a.rows + 15) / 16 * a.split < 16 * cu_count()) a.split *= 2;
-  const bool wide = a.scale_type == ST_SCORE_F32;
-  auto launch = [&](auto coarse_, auto wide_) {
+    while (a.split < kWaves && (a.rows + 15) / 16 * a.split < 8 * cu_count()) a.split *= 2;
+  auto launch = [&](auto coarse_, auto wide_, auto zeros_) {
     if (is_long)
-      launch_columns<coarse_(), wide_(), 1, 4>(a, columns, s);
+      launch_columns<coarse_(), wide_(), zeros_(), 1, 4>(a, columns, s);
     else
-      launch_columns<coarse_(), wide_(), 4, 1>(a, columns, s);
+      launch_columns<coarse_(), wide_(), zeros_(), 4, 1>(a, columns, s);
   };
-  if (coarse)
-    wide ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
-  else
-    wide ? launch(std::false_type{}, std::true_type{}) : launch(std::false_type{}, std::false_type{});
+  auto with = [](bool b, auto f) { b ? f(std::true_type{}) : f(std::false_type{}); };
+  with(coarse, [&](auto c) {
+    with(a.scale_type == ST_SCORE_F32, [&](auto w) { with(a.zeros != nullptr, [&](auto z) { launch(c, w, z); }); });
+  });
 }
 
 void check_type(int type, const char* what) {
