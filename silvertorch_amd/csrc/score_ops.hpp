@@ -160,20 +160,6 @@ __device__ __forceinline__ SoftStats soft_rebase(SoftStats a, float to, float c)
   return {to, a.s * scale, (a.t + a.s * d) * scale};
 }
 
-__device__ __forceinline__ SoftStats soft_join(const SoftStats& a, const SoftStats& b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  const SoftStats x = soft_rebase(a, m, c), y = soft_rebase(b, m, c);
-  return {m, x.s + y.s, x.t + y.t};
-}
-
-template <int LANES>
-__device__ __forceinline__ SoftStats soft_wave_join(SoftStats a, float c) {
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1)
-    a = soft_join(a, {__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.t, o)}, c);
-  return a;
-}
-
 // A float moved between lanes by DPP; lanes outside the row mask keep theirs.
 template <int CONTROL, int ROWS = 0xF>
 __device__ __forceinline__ float dpp_move(float x) {
@@ -206,6 +192,12 @@ __device__ __forceinline__ float wave_sum(float x) {
   const float r0 = __int_as_float(__builtin_amdgcn_readlane(i, 0)), r1 = __int_as_float(__builtin_amdgcn_readlane(i, 16));
   const float r2 = __int_as_float(__builtin_amdgcn_readlane(i, 32)), r3 = __int_as_float(__builtin_amdgcn_readlane(i, 48));
   return (r0 + r1) + (r2 + r3);
+}
+
+// The statistics of all lanes' scores, in every lane.
+__device__ __forceinline__ SoftStats soft_wave_join(SoftStats a, float c) {
+  a = soft_rebase(a, wave_max(a.m), c);
+  return {a.m, wave_sum(a.s), wave_sum(a.t)};
 }
 
 }  // namespace st

@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "score_ops.hpp"
 #include "st_errors.hpp"
@@ -28,8 +29,8 @@ constexpr int kUnit = 8;              // columns a thread takes at once
 constexpr int kMaxAlternatives = 128;
 constexpr int kMaxChunks = 256;       // parts of a row
 constexpr int kRoundUnits = 256;      // units examined for candidates at a time
-constexpr int kCandidates = kRoundUnits * kUnit + 256;
-constexpr int kJoinThreads = 256;
+constexpr int kCandidates = kRoundUnits * kUnit + 192;
+constexpr int kJoinThreads = 512;
 constexpr int kBackwardThreads = 256;
 constexpr int kBackwardUnits = 4;     // units per thread
 constexpr unsigned kMaxGrid = 1u << 22;
@@ -51,13 +52,13 @@ struct LogprobsArgs {
   float* stats;                       // [rows, 2] or null: m and s, what the gradient needs
 };
 
-// Scores of an 8-column unit with the excluded ones at -inf: bit 7 - i of
+// Scores of an 8-column unit with the excluded ones at `fill`: bit 7 - i of
 // `pass` lets score i through.
-__device__ __forceinline__ void exclude8(float v[8], uint32_t pass) {
+__device__ __forceinline__ void exclude8(float v[8], uint32_t pass, float fill) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint32_t keep = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(pass), 7 - i, 1));
-    v[i] = __uint_as_float((__float_as_uint(v[i]) & keep) | (0xFF800000u & ~keep));
+    v[i] = __uint_as_float((__float_as_uint(v[i]) & keep) | (__float_as_uint(fill) & ~keep));
   }
 }
 
@@ -76,24 +77,108 @@ __device__ __forceinline__ void load_unit(const void* row, const uint64_t* mask,
 #pragma unroll
     for (int i = 0; i < kUnit; ++i) v[i] = i < n ? load_score<DT>(row, col + i) : kMinusInf;
   }
-  if constexpr (MASKED) exclude8(v, pass_byte(mask, col / kUnit));
+  if constexpr (MASKED) exclude8(v, pass_byte(mask, col / kUnit), kMinusInf);
 }
 
-// Adds a unit's scores to a thread's statistics; true when they hold a new
-// maximum.
-__device__ __forceinline__ bool take_unit(SoftStats& a, const float v[8], float c) {
-  float top = fmaxf(fmaxf(v[0], v[1]), v[2]);
-  top = fmaxf(fmaxf(top, v[3]), v[4]);
-  top = fmaxf(fmaxf(top, v[5]), fmaxf(v[6], v[7]));
-  const bool higher = top > a.m;
-  if (higher) a = soft_rebase(a, top, c);
+// A thread's running statistics.  In the loop they are kept relative to k =
+// round(m c) instead of m c: then e^((z-m)/T) is 2^(z c - k), one multiply-add
+// and the exponential, and t adds up e (z c - k).  What the rounding of k moved
+// is put back once at the end (rest = m c - k is exact).
+struct Running {
+  SoftStats a;      // a.m: the maximum itself, -inf before any
+  float least, k;   // max(m, -1e29) and its k
+};
+
+constexpr float kFast = -1e29f;  // maxima outside (kFast, -kFast] are kept relative to m c
+constexpr float kFill = -1e30f;  // stands in an excluded column: 2^(kFill c - k) is 0
+
+__device__ __forceinline__ Running running_none(float c) { return {soft_none(), kFast, kFast * c}; }
+
+// To the reference m (t in units of z) and back.
+__device__ __forceinline__ SoftStats settled(const Running& r, float c) {
+  if (!(r.a.m > kFast && r.a.m <= -kFast)) return r.a;
+  const float rest = fmaf(r.a.m, c, -r.k);
+  const float back = __builtin_amdgcn_exp2f(-rest);
+  return {r.a.m, r.a.s * back, (r.a.t - rest * r.a.s) * back / c};
+}
+
+__device__ __forceinline__ Running running_of(const SoftStats& a, float c) {
+  Running r{a, fmaxf(a.m, kFast), 0.0f};
+  r.k = r.least * c;
+  if (a.m > kFast && a.m <= -kFast) {
+    const float rest = fmaf(a.m, c, -r.k), on = __builtin_amdgcn_exp2f(rest);
+    r.a.s = a.s * on;
+    r.a.t = (a.t * c + rest * a.s) * on;
+  }
+  return r;
+}
+
+// Adds eight scores of any size, -inf for none, to statistics relative to m.
+__device__ __forceinline__ SoftStats take_any(SoftStats a, const float v[8], float top, float c) {
+  if (top > a.m) a = soft_rebase(a, top, c);
   const float m = a.m == kMinusInf ? 0.0f : a.m;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float d = v[i] - m;
     const float e = __builtin_amdgcn_exp2f(d * c);
     a.s += e;
-    a.t = fmaf(e, fmaxf(d, -1e30f), a.t);  // an excluded score's d is -inf and its e 0
+    a.t = fmaf(e, fmaxf(d, -1e30f), a.t);  // -inf: e is 0
+  }
+  return a;
+}
+
+__device__ __forceinline__ float max8(const float v[8]) {
+  const float a = fmaxf(fmaxf(v[0], v[1]), v[2]), b = fmaxf(fmaxf(v[3], v[4]), v[5]);
+  return fmaxf(fmaxf(a, b), fmaxf(v[6], v[7]));
+}
+
+__device__ __forceinline__ float min8(const float v[8]) {
+  const float a = fminf(fminf(v[0], v[1]), v[2]), b = fminf(fminf(v[3], v[4]), v[5]);
+  return fminf(fminf(a, b), fminf(v[6], v[7]));
+}
+
+// Adds a unit's scores, those that `pass` excludes (MASKED) left out, to a
+// thread's statistics; true when they hold a new maximum.
+template <bool MASKED>
+__device__ __forceinline__ bool take_unit(Running& r, float v[8], uint32_t pass, float c) {
+  const float low = min8(v);
+  if constexpr (MASKED) exclude8(v, pass, kFill);
+  float top = max8(v);
+  if (__any(!(low > kFast) || fmaxf(top, r.least) > -kFast)) {
+    if constexpr (MASKED) {
+      exclude8(v, pass, kMinusInf);
+      top = max8(v);
+    }
+    // Maxima that are not ordinary take the general way; -inf and very low
+    // scores beside ordinary ones count as excluded ones do (their e is 0).
+    const bool general = fmaxf(top, r.a.m) > -kFast || (top > kMinusInf && top <= kFast && !(r.a.m > kFast));
+    if (__any(general)) {
+      const float before = r.a.m;
+      r = running_of(take_any(settled(r, c), v, top, c), c);
+      return r.a.m > before;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = v[i] < kFill ? kFill : v[i];
+  }
+  const bool higher = top > r.least;
+  if (higher) {
+    const float k = top * c;
+    if (r.a.m > kFast) {
+      const float d = r.k - k, scale = __builtin_amdgcn_exp2f(d);
+      r.a.t = scale == 0.0f ? 0.0f : (r.a.t + r.a.s * d) * scale;
+      r.a.s *= scale;
+    } else {
+      r.a = soft_rebase(r.a, top, c);  // nothing yet, or scores too low to count
+    }
+    r.a.m = r.least = top;
+    r.k = k;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float d = fmaf(v[i], c, -r.k);
+    const float e = __builtin_amdgcn_exp2f(d);
+    r.a.s += e;
+    r.a.t = fmaf(e, d, r.a.t);
   }
   return higher;
 }
@@ -106,25 +191,59 @@ struct SelectLds {
   uint16_t segment[1024];
 };
 
-// Writes the k largest of keys[0, n) to top, largest first and 0 past the
-// last; every thread of the workgroup calls it.  A key's place is the number
-// of keys above it.
+// Writes the k largest of keys[0, n) to top (zeroed before); every thread of
+// the workgroup calls it, after a barrier that follows the last key.  A key's
+// place is the number of keys above it, counted by four lanes.
 template <int T>
 __device__ __forceinline__ void rank_keys(SelectLds& l, uint32_t n, int k) {
-  const int tid = threadIdx.x;
-  if (tid < k) l.top[tid] = 0;
-  if (tid == 0) l.keys[n] = 0;
-  __syncthreads();
-  for (uint32_t i = tid; i < n; i += T) {
+  const uint32_t part = threadIdx.x % 4;
+  for (uint32_t i = threadIdx.x / 4; i < n; i += T / 4) {
     const uint64_t key = l.keys[i];
-    uint32_t above = 0;
-    for (uint32_t j = 0; j < n; j += 2) {
-      above += l.keys[j] > key ? 1u : 0u;
-      above += l.keys[j + 1] > key ? 1u : 0u;
-    }
-    if (above < static_cast<uint32_t>(k)) l.top[above] = key;
+    int above = 0;
+#pragma unroll 8
+    for (uint32_t j = part; j < n; j += 4) above += l.keys[j] > key ? 1 : 0;
+    above += __builtin_amdgcn_update_dpp(0, above, 0xB1, 0xF, 0xF, false);  // the quad's sum
+    above += __builtin_amdgcn_update_dpp(0, above, 0x4E, 0xF, 0xF, false);
+    if (part == 0 && above < k) l.top[above] = key;
   }
   __syncthreads();
+}
+
+// A bound that exactly k of the wave's 64 N distinct keys reach (0 if fewer
+// are above 0), found bit by bit from the top: first the scores' half, then,
+// where more scores are equal than may count, the columns'.
+template <int N>
+__device__ __forceinline__ uint64_t wave_kth(const uint64_t key[N], int k) {
+  auto search = [&](auto part, int want, auto takes_part) {
+    uint32_t bound = 0;
+    for (int b = 31; b >= 0; --b) {
+      const uint32_t t = bound | (1u << b);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) n += __popcll(__ballot(takes_part(i) && part(i) >= t));
+      if (n >= want) bound = t;
+      if (n == want) break;
+    }
+    return bound;
+  };
+  const uint32_t high = search([&](int i) { return static_cast<uint32_t>(key[i] >> 32); }, k, [](int) { return true; });
+  int above = 0, reach = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t h = static_cast<uint32_t>(key[i] >> 32);
+    above += __popcll(__ballot(h > high));
+    reach += __popcll(__ballot(h >= high));
+  }
+  uint32_t low = 0;
+  if (reach > k && high != 0)
+    low = search([&](int i) { return static_cast<uint32_t>(key[i]); }, k - above,
+                 [&](int i) { return static_cast<uint32_t>(key[i] >> 32) == high; });
+  return (static_cast<uint64_t>(high) << 32) | low;
+}
+
+__device__ __forceinline__ void push_key(SelectLds& l, uint64_t key) {
+  const uint32_t at = atomicAdd(&l.count, 1u);
+  if (at < kCandidates) l.keys[at] = key;
 }
 
 // After a round of pushes: when another round might not fit, keeps the best k
@@ -133,13 +252,16 @@ template <int T>
 __device__ __forceinline__ void make_room(SelectLds& l, int k) {
   const uint32_t n = l.count;
   __syncthreads();  // every thread has read the count before the next round's pushes
-  if (n <= kCandidates - 1 - kRoundUnits * kUnit) return;
+  if (n <= kCandidates - kRoundUnits * kUnit) return;
   rank_keys<T>(l, n, k);
   const int tid = threadIdx.x;
-  if (tid < k) l.keys[tid] = l.top[tid];
+  if (tid < k) {
+    l.keys[tid] = l.top[tid];
+    l.top[tid] = 0;
+  }
   if (tid == 0) {
     l.count = k;  // more than k keys were there
-    l.threshold = l.top[k - 1];
+    l.threshold = l.keys[k - 1];
   }
   __syncthreads();
 }
@@ -148,71 +270,114 @@ __device__ __forceinline__ void make_room(SelectLds& l, int k) {
 // t, t + T, ... and knows its largest score and the first unit that holds it.
 // The k-th largest of disjoint groups' maxima bounds the k-th best score from
 // below, so only threads whose maximum reaches it hold candidates, and their
-// units are read again: about k threads of T, whose scores are in the caches.
-// Rounds of 256 units keep the candidates' list bounded whatever the scores.
-template <int DT, bool MASKED, int T>
+// units are read again: few more than k threads of T, whose scores are in the
+// caches.  That is done in one go; should more scores reach the bound than
+// there is room for, again in rounds of 256 units that keep the best k so far.
+// `ready` runs before the first barrier.
+template <int DT, bool MASKED, int T, typename F>
 __device__ void select_top(SelectLds& l, const void* row, const uint64_t* mask, int64_t first, int64_t columns,
-                           float top, uint32_t top_unit, int k) {
+                           float top, uint32_t top_unit, int k, F ready) {
   const int tid = threadIdx.x;
   const uint32_t units = static_cast<uint32_t>((columns + kUnit - 1) / kUnit);
   // The lowest key that a score of this value has in this unit.
   const uint64_t mine =
       top > kMinusInf ? score_key(top, static_cast<uint32_t>(first) + top_unit * kUnit + (kUnit - 1)) : 0;
-  // Twice as many groups as alternatives leave few candidates more than k.
-  const int groups = k <= 32 ? 64 : 256;
   l.keys[tid] = mine;
+  if (tid < kMaxAlternatives) l.top[tid] = 0;
   if (tid == 0) {
     l.threshold = 0;
     l.count = 0;
     l.segments = 0;
   }
+  ready();
   __syncthreads();
-  uint64_t group = 0;
-  if (tid < groups)
-    for (int j = tid; j < T; j += groups) group = l.keys[j] > group ? l.keys[j] : group;
-  __syncthreads();
-  if (tid < groups) l.keys[tid] = group;
-  __syncthreads();
-  if (tid < groups && group != 0) {
-    int above = 0;
-    for (int j = 0; j < groups; j += 2) {
-      above += l.keys[j] > group ? 1 : 0;
-      above += l.keys[j + 1] > group ? 1 : 0;
+  // One wave finds the bound; twice as many groups as alternatives leave few
+  // candidates more than k.
+  auto bound_of = [&](auto groups) {
+    constexpr int N = groups();
+    uint64_t group[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      group[i] = 0;
+#pragma unroll
+      for (int j = 64 * i; j < T; j += 64 * N) group[i] = l.keys[j + tid] > group[i] ? l.keys[j + tid] : group[i];
     }
-    if (above == k - 1) l.threshold = group;
+    const uint64_t bound = wave_kth<N>(group, k);
+    if (tid == 0) l.threshold = bound;
+  };
+  if (tid < 64) {
+    if (k <= 32)
+      bound_of(std::integral_constant<int, 1>{});
+    else
+      bound_of(std::integral_constant<int, 4>{});
   }
   __syncthreads();
   const uint64_t bound = l.threshold;
-  if (mine != 0 && mine >= bound) l.segment[atomicAdd(&l.segments, 1u)] = static_cast<uint16_t>(tid);
-  __syncthreads();
   const uint32_t per = (units + T - 1) / T;
-  const uint32_t pairs = l.segments * per;
-  for (uint32_t base = 0; base < pairs; base += kRoundUnits) {
-    const uint32_t p = base + tid;
-    if (tid < kRoundUnits && p < pairs) {
-      const uint32_t u = l.segment[p / per] + T * (p % per);
-      if (u < units) {
-        const int64_t col = first + static_cast<int64_t>(u) * kUnit;
-        const int64_t left = first + columns - col;
-        float v[8];
-        load_unit<DT, MASKED>(row, mask, col, left < kUnit ? static_cast<int>(left) : kUnit, v);
-        const uint64_t least = l.threshold;
+  auto push_unit = [&](uint32_t u, uint64_t least) {
+    const int64_t col = first + static_cast<int64_t>(u) * kUnit;
+    const int64_t left = first + columns - col;
+    float v[8];
+    load_unit<DT, MASKED>(row, mask, col, left < kUnit ? static_cast<int>(left) : kUnit, v);
 #pragma unroll
-        for (int i = 0; i < kUnit; ++i) {
-          const uint64_t key = score_key(v[i], static_cast<uint32_t>(col) + i);
-          if (v[i] > kMinusInf && key >= least) l.keys[atomicAdd(&l.count, 1u)] = key;
-        }
-      }
+    for (int i = 0; i < kUnit; ++i) {
+      const uint64_t key = score_key(v[i], static_cast<uint32_t>(col) + i);
+      if (v[i] > kMinusInf && key >= least) push_key(l, key);
     }
+  };
+  if (per == 1) {  // each thread has its own unit
+    if (mine != 0 && mine >= bound) push_unit(tid, bound);
+  } else {
+    if (mine != 0 && mine >= bound) l.segment[atomicAdd(&l.segments, 1u)] = static_cast<uint16_t>(tid);
     __syncthreads();
-    make_room<T>(l, k);
+    const uint32_t pairs = l.segments * per;
+    for (uint32_t p = tid; p < pairs; p += T) {
+      const uint32_t u = l.segment[p / per] + T * (p % per);
+      if (u < units) push_unit(u, bound);
+    }
   }
-  rank_keys<T>(l, l.count, k);
+  __syncthreads();
+  uint32_t n = l.count;
+  if (n > kCandidates) {
+    __syncthreads();
+    if (per == 1) {  // nobody has listed the threads yet
+      if (mine != 0 && mine >= bound) l.segment[atomicAdd(&l.segments, 1u)] = static_cast<uint16_t>(tid);
+    }
+    if (tid == 0) l.count = 0;
+    __syncthreads();
+    const uint32_t pairs = l.segments * per;
+    for (uint32_t base = 0; base < pairs; base += kRoundUnits) {
+      const uint32_t p = base + tid;
+      if (tid < kRoundUnits && p < pairs) {
+        const uint32_t u = l.segment[p / per] + T * (p % per);
+        if (u < units) push_unit(u, l.threshold);
+      }
+      __syncthreads();
+      make_room<T>(l, k);
+    }
+    n = l.count;
+  }
+  rank_keys<T>(l, n, k);
+}
+
+// The row's target: its score, or -inf where it is excluded.  The id is read
+// before the row's scores, the score after them, so that neither is waited for.
+struct Target {
+  float z;
+  bool none;  // -1: no target
+};
+
+template <int DT>
+__device__ __forceinline__ Target find_target(const LogprobsArgs& a, int64_t row, int64_t target) {
+  Target t{kMinusInf, target == -1};
+  if (target >= 0 && target < a.columns &&
+      (a.mask == nullptr || ((a.mask[row * a.mask_stride + (target >> 6)] >> (63 - (target & 63))) & 1) != 0))
+    t.z = load_score<DT>(static_cast<const char*>(a.logits) + row * a.row_stride * kScoreBytes<DT>, target);
+  return t;
 }
 
 // The row's outputs from its statistics, by one thread.
-template <int DT>
-__device__ void finish_row(const LogprobsArgs& a, int64_t row, const SoftStats& st) {
+__device__ void finish_row(const LogprobsArgs& a, int64_t row, const Target& target, const SoftStats& st) {
   const bool none = st.m == kMinusInf && st.s == 0.0f;
   const float log_s = logf(st.s);
   a.lse[row] = none ? kMinusInf : fmaf(st.m, a.inv_t, log_s);
@@ -222,16 +387,8 @@ __device__ void finish_row(const LogprobsArgs& a, int64_t row, const SoftStats& 
     a.stats[2 * row] = st.m;
     a.stats[2 * row + 1] = st.s;
   }
-  const int64_t target = a.targets[row];
-  float lp = kMinusInf;
-  if (target == -1) {
-    lp = 0.0f;
-  } else if (!none && target >= 0 && target < a.columns) {
-    const bool pass =
-        a.mask == nullptr || ((a.mask[row * a.mask_stride + (target >> 6)] >> (63 - (target & 63))) & 1) != 0;
-    const float z = load_score<DT>(static_cast<const char*>(a.logits) + row * a.row_stride * kScoreBytes<DT>, target);
-    if (pass && z != kMinusInf) lp = fmaf(z - st.m, a.inv_t, -log_s);
-  }
+  float lp = target.none ? 0.0f : kMinusInf;
+  if (!none && target.z != kMinusInf) lp = fmaf(target.z - st.m, a.inv_t, -log_s);
   a.logprobs[row] = lp;
 }
 
@@ -244,25 +401,27 @@ __device__ __forceinline__ void finish_alternative(const LogprobsArgs& a, int64_
       key == 0 ? kMinusInf : fmaf(score_from_ordered(static_cast<uint32_t>(key >> 32)) - st.m, a.inv_t, -logf(st.s));
 }
 
-// The workgroup's statistics, in every thread.
+// The workgroup's statistics: each wave leaves its own, and after a barrier
+// any thread can join them.
 template <int T>
-__device__ __forceinline__ SoftStats join_workgroup(SoftStats st, float c) {
-  __shared__ SoftStats waves[T / 64];
-  st = soft_wave_join<64>(st, c);
-  if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = st;
-  __syncthreads();
-  st = waves[0];
-#pragma unroll
-  for (int w = 1; w < T / 64; ++w) st = soft_join(st, waves[w], c);
-  __syncthreads();
-  return st;
-}
+struct WorkgroupStats {
+  SoftStats waves[T / 64];
+  __device__ __forceinline__ void put(SoftStats st, float c) {
+    st = soft_wave_join(st, c);
+    if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = st;
+  }
+  __device__ __forceinline__ SoftStats get(float c) const {
+    const int w = threadIdx.x % 64;
+    return soft_wave_join(w < T / 64 ? waves[w] : soft_none(), c);
+  }
+};
 
 // One workgroup per row, or per part of a row.
 template <int DT, bool MASKED, int T>
-__global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a) {
+__global__ __launch_bounds__(T, T == 256 ? 4 : 8) void logprobs_kernel(LogprobsArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
   SelectLds& l = *reinterpret_cast<SelectLds*>(lds_raw);
+  __shared__ WorkgroupStats<T> joined;
   const int tid = threadIdx.x;
   const int64_t items = a.rows * a.chunks;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
@@ -272,13 +431,15 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a) {
     const char* row = static_cast<const char*>(a.logits) + r * a.row_stride * kScoreBytes<DT>;
     const uint64_t* mask = MASKED ? a.mask + r * a.mask_stride : nullptr;
     const uint32_t full = static_cast<uint32_t>(columns / kUnit);
-    SoftStats st = soft_none();
+    const int64_t target_id = tid == 0 && a.chunks == 1 ? a.targets[r] : -1;
+    Running run = running_none(a.c);
     uint32_t top_unit = 0;
-    constexpr int kAhead = DT == ST_SCORE_F32 ? 2 : 4;  // 64 bytes a thread in flight
+    // units a thread has in flight: 64 bytes, half that beside the filter's registers
+    constexpr int kAhead = (DT == ST_SCORE_F32 ? 2 : 4) / (MASKED ? 2 : 1);
     uint32_t u = tid;
     for (; u + (kAhead - 1) * T < full; u += kAhead * T) {
       Raw8<DT> raw[kAhead];
-      uint32_t pass[kAhead];
+      uint32_t pass[kAhead] = {};
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int64_t col = first + static_cast<int64_t>(u + i * T) * kUnit;
@@ -289,25 +450,32 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a) {
       for (int i = 0; i < kAhead; ++i) {
         float v[8];
         unpack8<DT>(raw[i], v);
-        if constexpr (MASKED) exclude8(v, pass[i]);
-        if (take_unit(st, v, a.c)) top_unit = u + i * T;
+        if (take_unit<MASKED>(run, v, pass[i], a.c)) top_unit = u + i * T;
       }
     }
     const uint32_t units = static_cast<uint32_t>((columns + kUnit - 1) / kUnit);
     for (; u < units; u += T) {
       const int64_t col = first + static_cast<int64_t>(u) * kUnit;
       float v[8];
-      load_unit<DT, MASKED>(row, mask, col, u < full ? kUnit : static_cast<int>(columns % kUnit), v);
-      if (take_unit(st, v, a.c)) top_unit = u;
+      load_unit<DT, false>(row, mask, col, u < full ? kUnit : static_cast<int>(columns % kUnit), v);
+      uint32_t pass = 0xFFu;
+      if constexpr (MASKED) pass = pass_byte(mask, col / kUnit);
+      if (take_unit<MASKED>(run, v, pass, a.c)) top_unit = u;
     }
-    if (a.topk > 0)
-      select_top<DT, MASKED, T>(l, row, mask, first, columns, st.m, top_unit, a.topk);
-    st = join_workgroup<T>(st, a.c);
+    SoftStats st = settled(run, a.c);
+    const Target target = find_target<DT>(a, r, target_id);  // one thread's
+    if (a.topk > 0) {
+      select_top<DT, MASKED, T>(l, row, mask, first, columns, st.m, top_unit, a.topk, [&] { joined.put(st, a.c); });
+    } else {
+      joined.put(st, a.c);
+      __syncthreads();
+    }
+    st = joined.get(a.c);
     if (a.chunks > 1) {
       if (tid == 0) a.part_stats[item] = st;
       if (tid < a.topk) a.part_keys[item * a.topk + tid] = l.top[tid];
     } else {
-      if (tid == 0) finish_row<DT>(a, r, st);
+      if (tid == 0) finish_row(a, r, target, st);
       if (tid < a.topk) finish_alternative(a, r, tid, l.top[tid], st);
     }
     __syncthreads();
@@ -317,48 +485,67 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a) {
 // Joins a row's parts: one workgroup per row.  The parts' lists are in order,
 // so their j-th entries bound the k-th best key from below: with j = ceil(2k /
 // parts), ceil(k / j) lists have at least k keys at or above the
-// ceil(k / j)-th largest of them.
+// ceil(k / j)-th largest of them.  Everything is read at the start, the first
+// kRoundUnits * kUnit entries into registers.
 template <int DT>
 __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobsArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
   SelectLds& l = *reinterpret_cast<SelectLds*>(lds_raw);
+  __shared__ WorkgroupStats<kJoinThreads> joined;
+  constexpr int kEach = kRoundUnits * kUnit / kJoinThreads;
   const int tid = threadIdx.x;
   const int k = a.topk;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const uint64_t* lists = a.part_keys + r * a.chunks * k;
+    const int64_t entries = static_cast<int64_t>(a.chunks) * k;
+    const int depth = k > 0 ? min(k, (2 * k + a.chunks - 1) / a.chunks) : 0;
+    SoftStats st = tid < a.chunks ? a.part_stats[r * a.chunks + tid] : soft_none();
+    uint64_t head[kMaxChunks / 64] = {};  // of the first wave
+    if (k > 0 && tid < 64) {
+#pragma unroll
+      for (int i = 0; i < kMaxChunks / 64; ++i) {
+        const int chunk = tid + 64 * i;
+        if (chunk < a.chunks) head[i] = lists[static_cast<int64_t>(chunk) * k + depth - 1];
+      }
+    }
+    uint64_t key[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int64_t e = i * kJoinThreads + tid;
+      key[i] = e < entries ? lists[e] : 0;
+    }
+    const Target target = find_target<DT>(a, r, tid == 0 ? a.targets[r] : -1);
+    joined.put(st, a.c);
     if (k > 0) {
-      const int depth = min(k, (2 * k + a.chunks - 1) / a.chunks);
       const int need = (k + depth - 1) / depth;  // <= chunks
-      uint64_t mine = tid < a.chunks ? lists[static_cast<int64_t>(tid) * k + depth - 1] : 0;
-      l.keys[tid] = mine;
-      if (tid == 0) {
-        l.threshold = 0;
-        l.count = 0;
+      if (tid < kMaxAlternatives) l.top[tid] = 0;
+      if (tid < 64) {
+        const uint64_t bound = wave_kth<kMaxChunks / 64>(head, need);
+        if (tid == 0) {
+          l.threshold = bound;
+          l.count = 0;
+        }
       }
       __syncthreads();
-      if (mine != 0) {
-        int above = 0;
-        for (int j = 0; j < a.chunks; ++j) above += l.keys[j] > mine ? 1 : 0;
-        if (above == need - 1) l.threshold = mine;
-      }
-      __syncthreads();
-      const int64_t entries = static_cast<int64_t>(a.chunks) * k;
       for (int64_t base = 0; base < entries; base += kRoundUnits * kUnit) {
         const uint64_t least = l.threshold;
 #pragma unroll
-        for (int i = 0; i < kRoundUnits * kUnit / kJoinThreads; ++i) {
-          const int64_t e = base + i * kJoinThreads + tid;
-          const uint64_t key = e < entries ? lists[e] : 0;
-          if (key != 0 && key >= least) l.keys[atomicAdd(&l.count, 1u)] = key;
+        for (int i = 0; i < kEach; ++i) {
+          if (base > 0) {
+            const int64_t e = base + i * kJoinThreads + tid;
+            key[i] = e < entries ? lists[e] : 0;
+          }
+          if (key[i] != 0 && key[i] >= least) push_key(l, key[i]);
         }
         __syncthreads();
         make_room<kJoinThreads>(l, k);
       }
       rank_keys<kJoinThreads>(l, l.count, k);
+    } else {
+      __syncthreads();
     }
-    SoftStats st = tid < a.chunks ? a.part_stats[r * a.chunks + tid] : soft_none();
-    st = join_workgroup<kJoinThreads>(st, a.c);
-    if (tid == 0) finish_row<DT>(a, r, st);
+    st = joined.get(a.c);
+    if (tid == 0) finish_row(a, r, target, st);
     if (tid < k) finish_alternative(a, r, tid, l.top[tid], st);
     __syncthreads();
   }
@@ -495,16 +682,24 @@ void check_launch(const char* what) {
   if (e != hipSuccess) throw Error(ST_ERR_HIP, cat(what, " launch failed: ", hipGetErrorString(e)));
 }
 
-// Parts of a row: enough workgroups of 1,024 threads for two on every CU, each
-// with at least 8,192 columns (a unit per thread).
+// Parts of a row.  One workgroup reads up to 64K columns sooner than a second
+// launch joins parts (one row of 40,000 with 10 alternatives: 10.3 us whole,
+// 12.6 us in parts; of 100,000: 12.3 and 12.1; 256 rows of 50,000: 10.1 and
+// 15.9).  Longer rows: two workgroups of 1,024 threads for every CU, each with
+// at least 8,192 columns, a unit per thread (100,000 columns, 1 row: 12.1 us
+// against 14.0 with 32,768).
 int row_chunks(int64_t rows, int64_t columns) {
+  if (columns <= 65536) return 1;
   const int64_t want = (2 * cu_count() + rows - 1) / std::max<int64_t>(rows, 1);
   const int64_t most = (columns + 8191) / 8192;
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxChunks})));
 }
 
-// Workgroups of 256 threads, eight on a CU, once rows fill them.
-bool small_groups(int64_t rows) { return rows >= 8 * cu_count(); }
+// Threads of a row's workgroup: as few as let the rows fill every CU's 2,048.
+int row_threads(int64_t rows, int chunks) {
+  if (chunks > 1 || rows <= 2 * cu_count()) return 1024;
+  return rows <= 4 * cu_count() ? 512 : 256;
+}
 
 unsigned grid_of(int64_t items) { return static_cast<unsigned>(std::min<int64_t>(items, kMaxGrid)); }
 
@@ -512,8 +707,11 @@ template <int DT, bool MASKED>
 void launch_forward(const LogprobsArgs& a, hipStream_t s) {
   const size_t lds = a.topk > 0 ? sizeof(SelectLds) : 0;
   const unsigned grid = grid_of(a.rows * a.chunks);
-  if (a.chunks == 1 && small_groups(a.rows))
+  const int threads = row_threads(a.rows, a.chunks);
+  if (threads == 256)
     hipLaunchKernelGGL((logprobs_kernel<DT, MASKED, 256>), dim3(grid), dim3(256), lds, s, a);
+  else if (threads == 512)
+    hipLaunchKernelGGL((logprobs_kernel<DT, MASKED, 512>), dim3(grid), dim3(512), lds, s, a);
   else
     hipLaunchKernelGGL((logprobs_kernel<DT, MASKED, 1024>), dim3(grid), dim3(1024), lds, s, a);
   check_launch("logprobs_kernel");
