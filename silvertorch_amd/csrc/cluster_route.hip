@@ -250,9 +250,11 @@ __device__ __forceinline__ double sum_workgroup(double x, double* red) {
   for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
   if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = x;
   __syncthreads();
-  x = 0.0;
-  if (threadIdx.x == 0)
-    for (int w = 0; w < T / 64; ++w) x += red[w];
+  x = threadIdx.x < T / 64 ? red[threadIdx.x] : 0.0;
+  if (threadIdx.x < 64) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) x += __shfl_xor(x, o);  // at most 16 waves
+  }
   return x;
 }
 
@@ -278,7 +280,7 @@ __global__ __launch_bounds__((kThreads<LPR, U>), (kWavesPerSimd<LPR, U>)) void r
   extern __shared__ __align__(16) uint8_t lds_raw[];
   uint64_t* lists = reinterpret_cast<uint64_t*>(lds_raw);  // [kRows or kWaves][kList]
   uint32_t* hist = reinterpret_cast<uint32_t*>(lists + (LPR > 64 ? kRows : kWaves) * kList);  // [clusters]
-  float* sums = reinterpret_cast<float*>(hist + a.clusters);  // [clusters], with kRows > 1
+  float* sums = reinterpret_cast<float*>(hist + (a.clusters + 7) / 8 * 8);  // likewise, with kRows > 1
   __shared__ float maxima[LPR > 64 ? kRows * 64 : 1];
   __shared__ float part_sum[kWaves], row_bound[kRows], row_top[kRows];
   __shared__ uint32_t list_n[2][kRows];
@@ -578,9 +580,15 @@ __global__ __launch_bounds__((kThreads<LPR, U>), (kWavesPerSimd<LPR, U>)) void r
     for (int w = 0; w < kTurns; ++w) {
       if (turn == w && (LPR >= 64 || lane < LPR)) {
 #pragma unroll
-        for (int i = 0; i < U * 8; ++i) {
-          const int col = column_of<LPR>(in_row * 8, i);
-          if (col < clusters) sums[col] = w == 0 ? acc[i] : sums[col] + acc[i];
+        for (int u = 0; u < U; ++u) {
+          const int col = column_of<LPR>(in_row * 8, u * 8);
+          if (col >= clusters) continue;
+          float* at = sums + col;  // whole units: there is room for eight past the last
+          float old[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) old[i] = w == 0 ? 0.0f : at[i];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) at[i] = old[i] + acc[u * 8 + i];
         }
       }
       __syncthreads();
@@ -624,25 +632,27 @@ __global__ __launch_bounds__(kFinishThreads) void route_finish_kernel(FinishArgs
   __shared__ double sums[kSlices][kFinishColumns];
   __shared__ uint32_t counts[kSlices][kFinishColumns];
   __shared__ double red[kFinishThreads / 64];
+  __shared__ uint32_t all_rows;
   __shared__ bool last;
   const int tid = threadIdx.x, slice = tid / kFinishColumns, column = tid % kFinishColumns;
   const int e = blockIdx.x * kFinishColumns + column;
   double sum = 0.0;
   uint32_t count = 0, rows = 0;
   if (e < a.clusters) {
-#pragma unroll 4
+#pragma unroll 8
     for (int g = slice; g < a.groups; g += kSlices) {
       sum += a.part_sums[static_cast<int64_t>(g) * a.clusters + e];
       count += a.part_counts[static_cast<int64_t>(g) * a.clusters + e];
     }
   }
   for (int g = tid; g < a.groups; g += kFinishThreads) rows += a.part_rows[g];
+  if (tid == 0) all_rows = 0;
   sums[slice][column] = sum;
   counts[slice][column] = count;
-  const double all = sum_workgroup<kFinishThreads>(rows, red);
-  if (tid == 0) red[0] = all;
   __syncthreads();
-  const double scale = loss_scale(a.clusters, a.probes, red[0]);
+  if (rows != 0) atomicAdd(&all_rows, rows);
+  __syncthreads();
+  const double scale = loss_scale(a.clusters, a.probes, all_rows);
   double part = 0.0;
   if (slice == 0 && e < a.clusters) {
     double p = 0.0;
@@ -855,7 +865,7 @@ RouteShape route_shape(int64_t clusters) {
     constexpr int T = kThreads<lpr(), units()>;
     s.rows = T / lpr();
     s.per_cu = std::max(1, kWavesPerSimd<lpr(), units()> * 4 * 64 / T);
-    s.lds = (lpr() > 64 ? s.rows * kRowList : T / 64 * kWaveList) * 8 + clusters * 4 * (s.rows > 1 ? 2 : 1);
+    s.lds = (lpr() > 64 ? s.rows * kRowList : T / 64 * kWaveList) * 8 + (clusters + 7) / 8 * 8 * 4 * (s.rows > 1 ? 2 : 1);
   });
   return s;
 }
