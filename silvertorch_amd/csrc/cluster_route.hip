@@ -36,14 +36,12 @@ constexpr int kFinishColumns = 16;  // clusters per workgroup of the second kern
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kRowList = 512, kWaveList = 128;  // candidates of a row of several waves, of one
 
-// Waves that a SIMD is to hold, and threads of a workgroup: rows of one wave or
-// less leave registers for more waves, which hide each other's latencies (two
-// workgroups fill a CU); rows of more waves want few workgroups, whose sums are
-// written.
-template <int LPR, int U>
-constexpr int kWavesPerSimd = LPR <= 64 && U == 1 ? 5 : 4;
-template <int LPR, int U>
-constexpr int kThreads = LPR > 64 ? 1024 : kWavesPerSimd<LPR, U> * 128;
+// Threads of a workgroup, four waves a SIMD: rows of one wave or less take two
+// workgroups a CU (five or six waves a SIMD measured the same or slower: 65,536
+// x 64 18.6 and 17.1 us against 16.8); rows of more waves want few workgroups,
+// whose sums are written.
+template <int LPR>
+constexpr int kThreads = LPR > 64 ? 1024 : 512;
 
 struct RouteArgs {
   const void* logits;
@@ -270,13 +268,16 @@ __device__ __forceinline__ double loss_scale(int clusters, int probes, double ro
 // multiply-add each; p = e / sum e does not depend on ref, and lse takes it
 // back as it is.  The next row's scores are loaded before a row is worked on.
 template <int DT, int LPR, int U>
-__global__ __launch_bounds__((kThreads<LPR, U>), (kWavesPerSimd<LPR, U>)) void route_kernel(RouteArgs a) {
-  constexpr int T = kThreads<LPR, U>;
+__global__ __launch_bounds__(kThreads<LPR>, 4) void route_kernel(RouteArgs a) {
+  constexpr int T = kThreads<LPR>;
   constexpr int kWaves = T / 64;
   constexpr int kRows = T / LPR;  // rows at a time
   constexpr int kWavesPerRow = LPR > 64 ? LPR / 64 : 1;
   constexpr int kList = LPR > 64 ? kRowList : kWaveList;  // keys of a row
-  constexpr bool kAhead = DT != ST_SCORE_F32 || U < 4;  // registers for the next row's scores
+  // Whether registers are left for the next row's scores: once a register is
+  // spilled, its reload waits for them too (16,001 x 5,000 float32: 162 us with
+  // them, 134 us without).
+  constexpr bool kAhead = U < (LPR == 64 && DT != ST_SCORE_F32 ? 4 : 3);
   extern __shared__ __align__(16) uint8_t lds_raw[];
   uint64_t* lists = reinterpret_cast<uint64_t*>(lds_raw);  // [kRows or kWaves][kList]
   uint32_t* hist = reinterpret_cast<uint32_t*>(lists + (LPR > 64 ? kRows : kWaves) * kList);  // [clusters]
@@ -700,10 +701,10 @@ struct RouteBackwardArgs {
 // chosen.  A row's scores and what belongs to it are loaded while the one
 // before is worked on.
 template <int DT, int LPR, int U>
-__global__ __launch_bounds__((kThreads<LPR, U>)) void route_backward_kernel(RouteBackwardArgs a) {
-  constexpr int kRows = kThreads<LPR, U> / LPR;
+__global__ __launch_bounds__(kThreads<LPR>) void route_backward_kernel(RouteBackwardArgs a) {
+  constexpr int kRows = kThreads<LPR> / LPR;
   constexpr int kOwn = LPR < kMaxProbes ? kMaxProbes / LPR : 1;  // chosen clusters of a lane
-  __shared__ float red_sum[2][kThreads<LPR, U> / 64];
+  __shared__ float red_sum[2][kThreads<LPR> / 64];
   const int tid = threadIdx.x;
   const int group = tid / LPR, in_row = tid % LPR;
   const int clusters = a.clusters, k = a.probes;
@@ -862,9 +863,9 @@ struct RouteShape {
 RouteShape route_shape(int64_t clusters) {
   RouteShape s{};
   for_shape(clusters, [&](auto lpr, auto units) {
-    constexpr int T = kThreads<lpr(), units()>;
+    constexpr int T = kThreads<lpr()>;
     s.rows = T / lpr();
-    s.per_cu = std::max(1, kWavesPerSimd<lpr(), units()> * 4 * 64 / T);
+    s.per_cu = 1024 / T;
     s.lds = (lpr() > 64 ? s.rows * kRowList : T / 64 * kWaveList) * 8 + (clusters + 7) / 8 * 8 * 4 * (s.rows > 1 ? 2 : 1);
   });
   return s;
@@ -893,7 +894,7 @@ void launch_route(const RouteArgs& a, int groups, hipStream_t s) {
         if (e != hipSuccess) throw Error(ST_ERR_HIP, cat("hipFuncSetAttribute failed: ", hipGetErrorString(e)));
       });
     }
-    hipLaunchKernelGGL(kernel, dim3(groups), dim3((kThreads<lpr(), units()>)), lds, s, a);
+    hipLaunchKernelGGL(kernel, dim3(groups), dim3(kThreads<lpr()>), lds, s, a);
     check_launch("route_kernel");
   });
 }
@@ -901,10 +902,10 @@ void launch_route(const RouteArgs& a, int groups, hipStream_t s) {
 template <int DT>
 void launch_route_backward(const RouteBackwardArgs& a, hipStream_t s) {
   for_shape(a.clusters, [&](auto lpr, auto units) {
-    const int64_t n = kThreads<lpr(), units()> / lpr();
+    const int64_t n = kThreads<lpr()> / lpr();
     const int64_t grid = std::min<int64_t>((a.rows + n - 1) / n, (lpr() > 64 ? 1 : 2) * cu_count());
     hipLaunchKernelGGL((route_backward_kernel<DT, lpr(), units()>), dim3(static_cast<unsigned>(grid)),
-                       dim3((kThreads<lpr(), units()>)), 0, s, a);
+                       dim3(kThreads<lpr()>), 0, s, a);
     check_launch("route_backward_kernel");
   });
 }
