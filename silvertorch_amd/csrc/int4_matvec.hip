@@ -147,7 +147,7 @@ struct Step {
 // SPREAD 4: up to four columns are spread over the product's rows so that a
 // lane finds its own in element 0 alone.
 // `split` waves share a row's columns and their sums meet in LDS.
-template <bool COARSE, bool WIDE, bool ZEROS, int T, int J, int C, int SPREAD>
+template <bool COARSE, bool WIDE, bool ZEROS, int T, int J, int C, int SPREAD, bool STREAMED>
 __global__ __launch_bounds__(kThreads, 2) void matvec_kernel(MatvecArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
   __shared__ uint32_t largest[kMaxTileColumns];
@@ -289,7 +289,8 @@ __global__ __launch_bounds__(kThreads, 2) void matvec_kernel(MatvecArgs a) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const uint32_t block = min((step * J + j) * 4 + quarter, a.blocks - 1);
-        s.w[t][j] = *reinterpret_cast<const u32x4*>(packed + (bytes + block * 16));
+        const u32x4* w = reinterpret_cast<const u32x4*>(packed + (bytes + block * 16));
+        s.w[t][j] = STREAMED ? __builtin_nontemporal_load(w) : *w;
         const uint32_t of = COARSE ? min((step * J + j) * 4, a.blocks - 1) : block;
         const uint32_t at = groups + (a.group_blocks == 1 ? of : __umulhi(of, a.group_magic));
         s.scale[t][j] = WIDE ? *reinterpret_cast<const uint32_t*>(scales + at * 4)
@@ -408,38 +409,47 @@ __global__ __launch_bounds__(kThreads, 2) void matvec_kernel(MatvecArgs a) {
   const bool y_wide = a.y_type == ST_SCORE_F32;
   char* const y = static_cast<char*>(a.y) + first_query * a.rows * (y_wide ? 4 : 2);
   auto put_y = [&](char* at, float v) {
-    if (y_wide)
+    if (y_wide && STREAMED)
+      __builtin_nontemporal_store(v, reinterpret_cast<float*>(at));
+    else if (y_wide)
       *reinterpret_cast<float*>(at) = v;
     else
       *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(
           a.y_type == ST_SCORE_F16 ? score_bits<ST_SCORE_F16>(v) : score_bits<ST_SCORE_BF16>(v));
   };
   auto store = [&](int64_t base) {
-    if constexpr (T == 4 && C == 1 && SPREAD == 4) {
-      // one vector: every lane group has its sums, and stores one tile of the
-      // four, so that a wave stores 64 adjacent results
-      if (columns == 1) {
-        float v = 0.0f;
-#pragma unroll
-        for (int t = 0; t < T; ++t) v = quarter == t ? static_cast<float>(acc[t][0][0]) : v;
-        if (base + lane < a.rows) put_y(y + (base + lane) * (y_wide ? 4 : 2), v * unscale[0][0]);
-        return;
-      }
-    }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
       for (int e = 0; e < 4; e += SPREAD) {
-        const int column = c * 16 + (quarter * 4 + e) / SPREAD;
-        const int q = a.parts == 2 ? column >> 1 : column;
-        const bool mine_ = (a.parts == 1 || (column & 1) == 0) && q < queries;
-        char* at = y + (q * a.rows + base + row16) * (y_wide ? 4 : 2);
+        float v[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-          float v = acc[t][c][e];
+          v[t] = acc[t][c][e];
           if constexpr (SPREAD == 1)
-            if (a.parts == 2) v = fmaf(acc[t][c][(e + 1) % 4], 1.0f / 2048.0f, v);
-          if (mine_ && base + t * 16 + row16 < a.rows) put_y(at + t * 16 * (y_wide ? 4 : 2), v * unscale[c][e]);
+            if (a.parts == 2) v[t] = fmaf(acc[t][c][(e + 1) % 4], 1.0f / 2048.0f, v[t]);
+          v[t] *= unscale[c][e];
+        }
+        if constexpr (T == 4) {
+          // Lane groups and tiles exchanged, a wave stores 64 adjacent results
+          // of one vector.
+          const u32x4 w = transpose4(u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                                           __float_as_uint(v[3])});
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int column = c * 16 + (i * 4 + e) / SPREAD;
+            const int q = a.parts == 2 ? column >> 1 : column;
+            if ((a.parts == 2 && (column & 1)) || q >= queries) continue;
+            if (base + lane < a.rows) put_y(y + (q * a.rows + base + lane) * (y_wide ? 4 : 2), __uint_as_float(w[i]));
+          }
+        } else {
+          const int column = c * 16 + (quarter * 4 + e) / SPREAD;
+          const int q = a.parts == 2 ? column >> 1 : column;
+          const bool mine_ = (a.parts == 1 || (column & 1) == 0) && q < queries;
+          char* at = y + (q * a.rows + base + row16) * (y_wide ? 4 : 2);
+#pragma unroll
+          for (int t = 0; t < T; ++t)
+            if (mine_ && base + t * 16 + row16 < a.rows) put_y(at + t * 16 * (y_wide ? 4 : 2), v[t]);
         }
       }
     }
@@ -564,14 +574,14 @@ void check_launch(const char* what) {
   if (e != hipSuccess) throw Error(ST_ERR_HIP, cat(what, " launch failed: ", hipGetErrorString(e)));
 }
 
-template <bool COARSE, bool WIDE, bool ZEROS, int T, int J, int C, int SPREAD>
+template <bool COARSE, bool WIDE, bool ZEROS, int T, int J, int C, int SPREAD, bool STREAMED = false>
 void launch_shape(const MatvecArgs& a, int columns, hipStream_t s) {
   const int64_t rows_at_once = static_cast<int64_t>(kWaves / a.split) * T * 16;
   const int64_t passes = (a.queries + a.queries_at_once - 1) / a.queries_at_once;
   const int lds_blocks = std::min(a.phase_blocks, (a.blocks + 3) / 4 * 4);
   size_t lds = static_cast<size_t>(lds_blocks) * 64 * columns;
   if (a.split > 1) lds += sizeof(float) * kWaves * 64 * T * C * 4;
-  const auto kernel = matvec_kernel<COARSE, WIDE, ZEROS, T, J, C, SPREAD>;
+  const auto kernel = matvec_kernel<COARSE, WIDE, ZEROS, T, J, C, SPREAD, STREAMED>;
   if (lds > 48 * 1024) {
     static std::once_flag once;
     std::call_once(once, [&] {
@@ -594,7 +604,15 @@ void launch_shape(const MatvecArgs& a, int columns, hipStream_t s) {
 
 template <bool COARSE, bool WIDE, bool ZEROS, int T, int J>
 void launch_columns(const MatvecArgs& a, int columns, hipStream_t s) {
-  if (columns <= 4 && a.parts == 1)
+  // One vector against a table that the last-level cache (256 MB) cannot hold
+  // for the next call is read, and the results are stored, past the caches:
+  // 20M x 128 243 us, 266 us through them.  A smaller table is found there again
+  // (1M x 256: 44 us; past the caches 50 us), and several vectors' results, rows
+  // of any length apart, need them to put lines together (2.5M x 128, 16
+  // vectors: 87 us; past them 103 us).
+  if (a.queries == 1 && a.parts == 1 && a.rows * a.row_bytes > (256ll << 20))
+    launch_shape<COARSE, WIDE, ZEROS, T, J, 1, 4, true>(a, columns, s);
+  else if (columns <= 4 && a.parts == 1)
     launch_shape<COARSE, WIDE, ZEROS, T, J, 1, 4>(a, columns, s);
   else if (columns <= 16)
     launch_shape<COARSE, WIDE, ZEROS, T, J, 1, 1>(a, columns, s);
