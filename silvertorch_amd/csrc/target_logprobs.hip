@@ -255,14 +255,13 @@ __device__ __forceinline__ void make_room(SelectLds& l, int k) {
   if (n <= kCandidates - kRoundUnits * kUnit) return;
   rank_keys<T>(l, n, k);
   const int tid = threadIdx.x;
-  if (tid < k) {
-    l.keys[tid] = l.top[tid];
+  if (tid < k) {  // more than k keys were there
+    const uint64_t key = l.top[tid];
+    l.keys[tid] = key;
     l.top[tid] = 0;
+    if (tid == k - 1) l.threshold = key;
   }
-  if (tid == 0) {
-    l.count = k;  // more than k keys were there
-    l.threshold = l.keys[k - 1];
-  }
+  if (tid == 0) l.count = k;
   __syncthreads();
 }
 

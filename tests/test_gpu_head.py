@@ -177,6 +177,17 @@ def test_logprobs_orders(order, rows, columns):
     _check_logprobs(z.repeat(rows, 1), torch.full((rows,), 17), 100, None, 1.0, grads=rows == 1)
 
 
+@pytest.mark.parametrize("rows,columns,threads", [(1, 65_536, 1024), (2100, 20_001, 256)])
+def test_logprobs_high_scores_in_few_threads(rows, columns, threads):
+    """Every score of 40 threads' columns above all others, and more alternatives wanted than that: the candidates
+    outgrow their list."""
+    H.note(f"[logprobs] few threads {rows} x {columns}")
+    at = torch.arange(columns)
+    noise = torch.randperm(columns, generator=torch.Generator().manual_seed(5)).float() / columns
+    z = torch.where(at // 8 % threads < 40, 10 + noise, noise)
+    _check_logprobs(z.repeat(rows, 1), torch.full((rows,), 17), 100, None, 1.0, grads=rows == 1)
+
+
 def test_logprobs_excluded_places():
     """Rows that nothing passes, infinities and NaN behind the filter, the type's lowest value, -inf among what
     passes, targets that are masked, -inf, out of range and absent."""
@@ -393,6 +404,17 @@ def test_route_equal_scores(clusters, probes):
     H.note(f"[route] ties {clusters} probes {probes}")
     _check_route(torch.zeros((5, clusters)), probes)
     _check_route(torch.randint(0, 2, (5, clusters), generator=torch.Generator().manual_seed(3)).to(torch.bfloat16), probes)
+
+
+@pytest.mark.parametrize("clusters,probes,lanes,period", [(1024, 8, 5, 16), (2048, 30, 20, 64), (5000, 24, 80, 256),
+                                                          (30_000, 40, 300, 1024)])
+def test_route_high_scores_in_few_lanes(clusters, probes, lanes, period):
+    """Every score of a few lanes' clusters above all others, so that far more than the probes reach the bound."""
+    H.note(f"[route] few lanes {clusters} probes {probes}")
+    at = torch.arange(clusters)
+    g = torch.Generator().manual_seed(7)
+    noise = torch.stack([torch.randperm(clusters, generator=g) for _ in range(9)]).float() / clusters
+    _check_route(torch.where(at // 8 % period < lanes, 3 + noise, noise), probes, torch.arange(9) != 4)
 
 
 @pytest.mark.parametrize("clusters", [40, 600, 5000])
@@ -700,3 +722,23 @@ def test_module():
     for i in (0, 1, 2, 4):
         _near(out[i], want[i], 64 * U * 100)
     assert torch.equal(other(q)[0].cpu(), torch.zeros(4))
+
+
+def test_example():
+    """Training lowers the loss; answers pass the filter and give the clicked document more than the uniform share."""
+    H.note("[head] example")
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "retrieval_head.py"
+    spec = importlib.util.spec_from_file_location("retrieval_head_example", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    out = module.main(["--docs", "3000", "--pairs", "256", "--steps", "40"])
+    assert out["last"] < out["first"] - 1
+    topics, clicked, ids = out["topics"].cpu(), out["clicked"].cpu(), out["top_ids"].cpu()
+    passes = O.bits(out["mask"].cpu(), 3000)
+    assert passes.gather(1, ids).all() and passes.gather(1, clicked.unsqueeze(1)).all()
+    same = topics.unsqueeze(0) == topics[clicked].unsqueeze(1)
+    assert (passes | ~same).all()  # a bloom filter passes every document of the topic
+    assert (out["logprobs"].cpu() > -torch.log(passes.sum(1).float())).float().mean() > 0.8
