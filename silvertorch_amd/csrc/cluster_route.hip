@@ -267,6 +267,14 @@ __device__ __forceinline__ double loss_scale(int clusters, int probes, double ro
 // keys above it.  Exponentials are 2^(z c - ref), ref the rounded m c, one
 // multiply-add each; p = e / sum e does not depend on ref, and lse takes it
 // back as it is.  The next row's scores are loaded before a row is worked on.
+//
+// What bounds it: vector instructions.  A row of 1,024 scores in one wave takes
+// some 400 of them (a third for the exponentials and sums, the rest for the
+// selection), more than its 2 KB take to arrive; a row of several waves waits at
+// three barriers besides.  Measured with the second kernel: 65,536 x 1,024
+// bfloat16, 8 probes 72 us (46 us without a selection, 37 us for the reads
+// alone); 16,001 x 5,000 float32, 24 probes 134 us; 65,536 x 64 bfloat16, 2
+// probes 17 us; 8 x 2,500 float32, 16 probes 14.5 us in one workgroup.
 template <int DT, int LPR, int U>
 __global__ __launch_bounds__(kThreads<LPR>, 4) void route_kernel(RouteArgs a) {
   constexpr int T = kThreads<LPR>;
@@ -627,7 +635,8 @@ struct FinishArgs {
 };
 
 // Adds up the workgroups' parts: 16 clusters per workgroup, 64 slices of the
-// parts each; the last workgroup to end adds up the loss.
+// parts each; the last workgroup to end adds up the loss.  Latency bounds it: 9
+// us for 512 parts of 1,024 clusters (4 MB).
 __global__ __launch_bounds__(kFinishThreads) void route_finish_kernel(FinishArgs a) {
   constexpr int kSlices = kFinishThreads / kFinishColumns;
   __shared__ double sums[kSlices][kFinishColumns];
@@ -699,7 +708,8 @@ struct RouteBackwardArgs {
 // dz = p (g_loss slope - dot + g_l), then the chosen clusters again with their
 // own g_w; dot = sum of g_loss slope p over the row and of g_w p over the
 // chosen.  A row's scores and what belongs to it are loaded while the one
-// before is worked on.
+// before is worked on; HBM bounds it: 65,536 x 1,024 bfloat16 59 us (4.6 TB/s),
+// 16,001 x 5,000 float32 121 us (5.3 TB/s).
 template <int DT, int LPR, int U>
 __global__ __launch_bounds__(kThreads<LPR>) void route_backward_kernel(RouteBackwardArgs a) {
   constexpr int kRows = kThreads<LPR> / LPR;

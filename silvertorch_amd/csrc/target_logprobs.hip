@@ -415,7 +415,18 @@ struct WorkgroupStats {
   }
 };
 
-// One workgroup per row, or per part of a row.
+// One workgroup per row, or per part of a row (row_chunks, row_threads).
+//
+// What bounds it: the one read of the scores.  Statistics take a multiply-add,
+// an exponential and two sums a score, in registers, rescaled when a thread's
+// maximum rises (settled, take_unit); joins go over lanes and LDS once a row.
+// The alternatives cost a second read of about k threads' units (select_top).
+//
+// Measured: 4,096 x 100,000 bfloat16 147 us (5.6 TB/s); 512 x 100,000 bfloat16,
+// 20 alternatives 27 us (3.7 TB/s: two workgroups a CU end together, and the
+// selection's latency shows); 16 x 2.5M float32 filtered, 100 alternatives 56 us
+// with the join (42 us without alternatives); 1 x 100,000 float32 filtered, 10
+// alternatives 13 us (two launches; 7.5 us without alternatives).
 template <int DT, bool MASKED, int T>
 __global__ __launch_bounds__(T, T == 256 ? 4 : 8) void logprobs_kernel(LogprobsArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
@@ -485,7 +496,8 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 8) void logprobs_kernel(LogprobsA
 // so their j-th entries bound the k-th best key from below: with j = ceil(2k /
 // parts), ceil(k / j) lists have at least k keys at or above the
 // ceil(k / j)-th largest of them.  Everything is read at the start, the first
-// kRoundUnits * kUnit entries into registers.
+// kRoundUnits * kUnit entries into registers: the kernel is one latency after
+// another (4-10 us), of which the launch is the largest.
 template <int DT>
 __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobsArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
@@ -570,7 +582,10 @@ __device__ __forceinline__ bool passes(const BackwardArgs& a, int64_t row, int64
 }
 
 // With e = e^((z-m)/T), p = e/s and log p + H = (z-m)/T + (H - log s):
-// dL/dz = e (k0 + k1 (z-m)) outside the target and the alternatives.
+// dL/dz = e (k0 + k1 (z-m)) outside the target and the alternatives.  Scores are
+// read once and gradients written once; parts of 8,192 columns a workgroup keep
+// the row's factors in registers.  HBM bounds it: 4,096 x 100,000 bfloat16 280
+// us (5.9 TB/s), 1,000 x 33,333 float32 filtered 48 us (5.6 TB/s).
 template <int DT, bool MASKED>
 __global__ __launch_bounds__(kBackwardThreads, 8) void logprobs_backward_kernel(BackwardArgs a, const float* entropy) {
   constexpr int kColumns = kBackwardThreads * kBackwardUnits * kUnit;

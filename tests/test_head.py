@@ -76,6 +76,7 @@ def test_c_entry_points_refuse():
     refused("scales", L.st_int4_matvec(n, n, 5, n, n, 0, 1, 1, 64, 32, n, 0, n))
     refused("null device pointer", L.st_int4_matvec(n, n, 0, n, n, 0, 1, 1, 64, 32, n, 0, n))
     refused("16-byte aligned", L.st_int4_matvec(8, 16, 0, n, 16, 0, 1, 1, 64, 32, 16, 0, n))
+    refused("between 0 and 65536", L.st_int4_matvec(16, 16, 0, n, 16, 0, 65_537, 1, 64, 32, 16, 0, n))
     refused("at least one column", L.st_int4_quantize(n, 0, 1, 0, 32, 1, n, n, n, n))
     refused("topk", L.st_target_logprobs(n, 0, 1, 5, 5, n, n, 0, 0, 200, 1.0, *[n] * 8))
     refused("temperature", L.st_target_logprobs(n, 0, 1, 5, 5, n, n, 0, 0, 2, 0.0, *[n] * 8))
