@@ -561,7 +561,7 @@ int st_target_logprobs_backward(const void* logits, int score_type, int64_t rows
  * counterpart in the reference; the ids are what st_fused_kmean_ann takes.
  *
  * logits [rows, clusters] (ST_SCORE_F32, _F16 or _BF16; row r starts at element
- * r * row_stride; 1 <= clusters <= 32768); valid uint8 [rows] or null.  Per
+ * r * row_stride; 1 <= clusters <= 32768; rows below 2^31); valid uint8 [rows] or null.  Per
  * valid row: lse = log sum e^z, cluster_ids [rows, probes] the clusters of
  * largest score in order, equal ones by cluster (clusters at -inf or NaN are
  * never chosen; padded with -1), weights = e^(z - lse) at them (padded with 0).

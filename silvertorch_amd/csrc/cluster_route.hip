@@ -923,7 +923,7 @@ void launch_route_backward(const RouteBackwardArgs& a, hipStream_t s) {
 void check_route(int score_type, int64_t rows, int64_t clusters, int64_t row_stride, int64_t probes) {
   ST_CHECK(score_type == ST_SCORE_F32 || score_type == ST_SCORE_F16 || score_type == ST_SCORE_BF16,
            "scores must be float32, float16 or bfloat16");
-  ST_CHECK(rows >= 0 && row_stride >= 0, "negative sizes");
+  ST_CHECK(rows >= 0 && rows < (1ll << 31) && row_stride >= 0, "sizes must not be negative, rows below 2^31; got ", rows);
   ST_CHECK(clusters >= 1 && clusters <= kMaxClusters, "clusters must be in [1, ", kMaxClusters, "], got ", clusters);
   ST_CHECK(probes >= 1 && probes <= kMaxProbes, "probes must be in [1, ", kMaxProbes, "], got ", probes);
 }

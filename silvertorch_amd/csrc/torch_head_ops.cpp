@@ -218,6 +218,26 @@ Tensor gradient(const Tensor& g, at::Device d) {
   return g.defined() ? g.to(d, at::kFloat).contiguous() : g;
 }
 
+// A gradient with a graph over it (backward with create_graph): it depends on
+// the scores and on the outputs' gradients, and refuses to be differentiated
+// where it would otherwise count as a constant.
+struct OnceDifferentiable : torch::autograd::Function<OnceDifferentiable> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& grad, const Tensor& /*logits*/, const OptTensor& /*g0*/,
+                        const OptTensor& /*g1*/, const OptTensor& /*g2*/, const OptTensor& /*g3*/, std::string op) {
+    ctx->saved_data["op"] = std::move(op);
+    return grad;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list /*grads*/) {
+    TORCH_CHECK(false, "the gradient of ", ctx->saved_data["op"].toStringRef(), " cannot be differentiated again");
+  }
+};
+
+Tensor differentiable_once(const Tensor& grad, const Tensor& logits, const variable_list& outer, const char* op) {
+  if (!at::GradMode::is_enabled()) return grad;
+  auto given = [&](size_t i) { return outer[i].defined() ? OptTensor(outer[i]) : OptTensor(); };
+  return OnceDifferentiable::apply(grad, logits, given(0), given(1), given(2), given(4), std::string(op));
+}
+
 struct LogprobsFunction : torch::autograd::Function<LogprobsFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& targets, int64_t topk,
                                const OptTensor& packed_mask, double temperature) {
@@ -233,8 +253,13 @@ struct LogprobsFunction : torch::autograd::Function<LogprobsFunction> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    at::AutoDispatchBelowADInplaceOrView below;
     const variable_list saved = ctx->get_saved_variables();
+    const Tensor grad = logits_gradient(ctx, saved, grads);
+    return {differentiable_once(grad, saved[0], grads, "target_logprobs"), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+
+  static Tensor logits_gradient(AutogradContext* ctx, const variable_list& saved, const variable_list& grads) {
+    at::AutoDispatchBelowADInplaceOrView below;
     const Tensor& logits = saved[0];
     const bool on_gpu = logits.is_cuda();
     const at::Device dev = on_gpu ? logits.device() : gpu_for_cpu_call();
@@ -254,7 +279,7 @@ struct LogprobsFunction : torch::autograd::Function<LogprobsFunction> {
                  data_or_null<float>(gl), data_or_null<float>(ge), data_or_null<float>(gs), data_or_null<float>(gt),
                  bytes_or_null(grad), current_stream(z)),
              "target_logprobs");
-    return {on_gpu ? grad : grad.cpu(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return on_gpu ? grad : grad.cpu();
   }
 };
 
@@ -332,8 +357,12 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    at::AutoDispatchBelowADInplaceOrView below;
     const variable_list saved = ctx->get_saved_variables();
+    return {differentiable_once(logits_gradient(saved, grads), saved[0], grads, "cluster_route"), Tensor(), Tensor()};
+  }
+
+  static Tensor logits_gradient(const variable_list& saved, const variable_list& grads) {
+    at::AutoDispatchBelowADInplaceOrView below;
     const bool on_gpu = saved[0].is_cuda();
     const at::Device dev = on_gpu ? saved[0].device() : gpu_for_cpu_call();
     c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
@@ -348,7 +377,7 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
                                        data_or_null<float>(slopes), data_or_null<float>(gw), data_or_null<float>(gs),
                                        data_or_null<float>(gl), bytes_or_null(grad), current_stream(z)),
              "cluster_route");
-    return {on_gpu ? grad : grad.cpu(), Tensor(), Tensor()};
+    return on_gpu ? grad : grad.cpu();
   }
 };
 

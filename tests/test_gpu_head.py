@@ -489,6 +489,21 @@ def test_route_gradient_against_differences():
     assert abs(slope - (grad.cpu().double() * way.double()).sum().item()) < 25 * (h * h + 64 * U * 15 / h)
 
 
+def test_second_derivatives_refused():
+    """A graph over the gradients is allowed; going back through it says that it cannot be."""
+    H.note("[head] second derivatives")
+    for device in ("cuda", "cpu"):
+        x = torch.randn((3, 50), generator=torch.Generator().manual_seed(1)).to(device).requires_grad_()
+        targets = torch.arange(3, device=device)
+        for name, output in (("target_logprobs", lambda: torch.ops.st.target_logprobs(x, targets)[0]),
+                             ("cluster_route", lambda: torch.ops.st.cluster_route(x, 4)[2])):
+            plain, = torch.autograd.grad(output().sum(), x)
+            once, = torch.autograd.grad(output().sum(), x, create_graph=True)
+            assert torch.equal(plain, once) and not plain.requires_grad
+            with pytest.raises(RuntimeError, match=f"gradient of {name} cannot be differentiated again"):
+                torch.autograd.grad(once.square().sum(), x)
+
+
 # ------------------------------------------------------------------ 4-bit tables
 
 

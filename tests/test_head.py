@@ -86,6 +86,7 @@ def test_c_entry_points_refuse():
     refused("null device pointer", L.st_target_logprobs_backward(16, 0, 1, 5, 5, 16, n, 0, 0, 2, 1.0, *[n] * 9))
     refused("probes", L.st_cluster_route(n, 0, 1, 5, 5, 0, *[n] * 10))
     refused("clusters", L.st_cluster_route(n, 0, 1, 40_000, 5, 1, *[n] * 10))
+    refused("below 2^31", L.st_cluster_route(n, 0, 1 << 31, 5, 5, 1, *[n] * 10))
     refused("null device pointer", L.st_cluster_route(n, 0, 1, 5, 5, 1, *[n] * 10))
     refused("null device pointer", L.st_cluster_route_backward(n, 0, 1, 5, 5, 1, *[n] * 9))
     assert L.st_target_logprobs(n, 0, 0, 5, 5, n, n, 0, 0, 2, 1.0, *[n] * 8) == 0
