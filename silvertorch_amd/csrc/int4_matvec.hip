@@ -26,6 +26,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTileColumns = 64;         // vectors' parts a pass takes
 constexpr int kVectorLds = 64 * 1024;       // the vectors' share of LDS, in phases
 constexpr int kWholeVectorLds = 128 * 1024;  // or, if they fit at once
+constexpr int kMostLds = 160 * 1024 - 512;   // with room for largest[]
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
@@ -599,7 +600,7 @@ void launch_shape(const MatvecArgs& a, int columns, hipStream_t s) {
     static std::once_flag once;
     std::call_once(once, [&] {
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 512);
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
       if (e != hipSuccess) throw Error(ST_ERR_HIP, cat("hipFuncSetAttribute failed: ", hipGetErrorString(e)));
     });
   }
@@ -642,13 +643,19 @@ void launch_matvec(MatvecArgs& a, hipStream_t s) {
   // block / group_blocks: the reciprocal rounded up is exact while block *
   // group_blocks stays below 2^32 (blocks are at most 2^16); 1 has none
   a.group_magic = a.group_blocks == 1 ? 0 : static_cast<uint32_t>((0x100000000ull + a.group_blocks - 1) / a.group_blocks);
-  const int whole = (a.blocks + 15) / 16 * 16;
-  a.phase_blocks = whole * 64 * columns <= kWholeVectorLds ? whole : std::max(16, kVectorLds / (64 * columns) / 16 * 16);
   const bool coarse = a.group_blocks % 4 == 0;
   const bool is_long = a.blocks > 8;
   a.split = 1;
   if (is_long)
     while (a.split < kWaves && (a.rows + 15) / 16 * a.split < 8 * cu_count()) a.split *= 2;
+  // All of the vectors at once, if there is room for them beside the sums of
+  // the waves that share rows (T = 1; launch_shape).
+  const int tiles = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
+  const int sums = a.split > 1 ? static_cast<int>(sizeof(float)) * kWaves * 64 * tiles * 4 : 0;
+  const int whole = (a.blocks + 15) / 16 * 16;
+  a.phase_blocks = whole * 64 * columns <= std::min(kWholeVectorLds, kMostLds - sums)
+                       ? whole
+                       : std::max(16, kVectorLds / (64 * columns) / 16 * 16);
   auto launch = [&](auto coarse_, auto wide_, auto zeros_) {
     if (is_long)
       launch_columns<coarse_(), wide_(), zeros_(), 1, 4>(a, columns, s);

@@ -545,6 +545,19 @@ def test_matvec(n, dim, group, queries, asymmetric, dtype):
     _check_matvec(packed, scales, zeros, x[0], group)
 
 
+@pytest.mark.parametrize("n,dim,queries,dtype", [
+    (1000, 1024, 64, torch.bfloat16), (1000, 900, 63, torch.float16), (1000, 1000, 32, torch.float32),
+    (33_000, 1024, 64, torch.bfloat16), (500, 1536, 42, torch.bfloat16), (500, 2048, 32, torch.float16),
+    (200, 4096, 16, torch.bfloat16), (200, 4097, 8, torch.float32),
+])
+def test_matvec_vectors_that_fill_lds(n, dim, queries, dtype):
+    """As many vectors as are held at once, beside the sums of the waves that share rows."""
+    H.note(f"[int4] full LDS {n} x {dim} queries {queries} {dtype}")
+    packed, scales, zeros = _table(n, dim, 64, torch.bfloat16, True, n + dim)
+    x = torch.randn((queries, dim), generator=torch.Generator().manual_seed(dim)).to(dtype)
+    _check_matvec(packed, scales, zeros, x, 64, torch.float32)
+
+
 @pytest.mark.parametrize("n", [1, 15, 16, 63, 4096, 70_001, 600_000])
 @pytest.mark.parametrize("dim,queries", [(64, 1), (128, 7), (128, 16)])
 def test_matvec_row_counts(n, dim, queries):
