@@ -639,23 +639,33 @@ void launch_columns(const MatvecArgs& a, int columns, hipStream_t s) {
 void launch_matvec(MatvecArgs& a, hipStream_t s) {
   a.parts = a.x_type == ST_SCORE_F32 ? 2 : 1;
   a.queries_at_once = static_cast<int>(std::min<int64_t>(a.queries, kMaxTileColumns / a.parts));
+  const bool is_long = a.blocks > 8;
+  a.split = 1;
+  if (is_long)
+    while (a.split < kWaves && (a.rows + 15) / 16 * a.split < 8 * cu_count()) a.split *= 2;
+  const int whole = (a.blocks + 15) / 16 * 16;
+  auto phase_of = [&](int columns) { return std::max(16, kVectorLds / (64 * columns) / 16 * 16); };
+  // Where four or eight waves share a row but a phase of many vectors has fewer
+  // steps than that, some would have none: 16 parts a pass then (64 vectors x
+  // 8,192 columns: 500 rows 160 -> 41 us, 8,192 rows 211 -> 145 us).  With two
+  // waves a row, or one, reading the table again costs more (30,000 x 1,300,
+  // 32 float32 vectors 48 against 55 us; 100,000 x 8,192, 64 vectors 760
+  // against 874 us).
+  const int most = a.queries_at_once * a.parts;
+  if (a.split >= 4 && whole * 64 * most > kWholeVectorLds && a.split > phase_of(most) / 16)
+    a.queries_at_once = std::min(a.queries_at_once, 16 / a.parts);
   const int columns = a.queries_at_once * a.parts;
   // block / group_blocks: the reciprocal rounded up is exact while block *
   // group_blocks stays below 2^32 (blocks are at most 2^16); 1 has none
   a.group_magic = a.group_blocks == 1 ? 0 : static_cast<uint32_t>((0x100000000ull + a.group_blocks - 1) / a.group_blocks);
   const bool coarse = a.group_blocks % 4 == 0;
-  const bool is_long = a.blocks > 8;
-  a.split = 1;
-  if (is_long)
-    while (a.split < kWaves && (a.rows + 15) / 16 * a.split < 8 * cu_count()) a.split *= 2;
   // All of the vectors at once, if there is room for them beside the sums of
   // the waves that share rows (T = 1; launch_shape).
   const int tiles = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
   const int sums = a.split > 1 ? static_cast<int>(sizeof(float)) * kWaves * 64 * tiles * 4 : 0;
-  const int whole = (a.blocks + 15) / 16 * 16;
   a.phase_blocks = whole * 64 * columns <= std::min(kWholeVectorLds, kMostLds - sums)
                        ? whole
-                       : std::max(16, kVectorLds / (64 * columns) / 16 * 16);
+                       : phase_of(columns);
   auto launch = [&](auto coarse_, auto wide_, auto zeros_) {
     if (is_long)
       launch_columns<coarse_(), wide_(), zeros_(), 1, 4>(a, columns, s);

@@ -558,6 +558,18 @@ def test_matvec_vectors_that_fill_lds(n, dim, queries, dtype):
     _check_matvec(packed, scales, zeros, x, 64, torch.float32)
 
 
+@pytest.mark.parametrize("n,dim,queries,dtype", [
+    (500, 2100, 64, torch.bfloat16), (3000, 1100, 65, torch.float16), (9000, 2100, 33, torch.bfloat16),
+    (700, 2100, 33, torch.float32), (17_000, 1100, 64, torch.bfloat16),
+])
+def test_matvec_many_long_vectors(n, dim, queries, dtype):
+    """Vectors that LDS cannot hold at once, taken in passes or in phases."""
+    H.note(f"[int4] long vectors {n} x {dim} queries {queries} {dtype}")
+    packed, scales, zeros = _table(n, dim, 64, torch.bfloat16, True, n + dim)
+    x = torch.randn((queries, dim), generator=torch.Generator().manual_seed(dim)).to(dtype)
+    _check_matvec(packed, scales, zeros, x, 64, torch.float32)
+
+
 @pytest.mark.parametrize("n", [1, 15, 16, 63, 4096, 70_001, 600_000])
 @pytest.mark.parametrize("dim,queries", [(64, 1), (128, 7), (128, 16)])
 def test_matvec_row_counts(n, dim, queries):
