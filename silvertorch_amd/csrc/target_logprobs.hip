@@ -43,6 +43,7 @@ struct LogprobsArgs {
   int64_t mask_stride;                // words; 0: one row for all
   int topk;
   float c, inv_t;                     // log2(e) / T, 1 / T
+  float limit;                        // fast_limit(c)
   int chunks;
   int64_t chunk_columns;              // a multiple of kUnit
   SoftStats* part_stats;              // [rows, chunks], with chunks > 1
@@ -83,29 +84,36 @@ __device__ __forceinline__ void load_unit(const void* row, const uint64_t* mask,
 // A thread's running statistics.  In the loop they are kept relative to k =
 // round(m c) instead of m c: then e^((z-m)/T) is 2^(z c - k), one multiply-add
 // and the exponential, and t adds up e (z c - k).  What the rounding of k moved
-// is put back once at the end (rest = m c - k is exact).
+// is put back once at the end (rest = m c - k is exact).  rest is half an ulp
+// of m c at most, and past 2^31 2^rest may not be a finite number: maxima
+// outside (-limit, limit], where rest is 64 at most, are kept relative to m
+// itself.  A rest that large costs no accuracy: the scores' own spacing is more
+// than it, so that only those equal to m count.  (Limits as low as 2^26 took a
+// second look at units with scores of -1e9: 2,000 x 30,000 bfloat16, half of
+// them so, 27.2 against 24.8 us.)
 struct Running {
   SoftStats a;      // a.m: the maximum itself, -inf before any
-  float least, k;   // max(m, -1e29) and its k
+  float least, k;   // max(m, -limit) and its k
 };
 
-constexpr float kFast = -1e29f;  // maxima outside (kFast, -kFast] are kept relative to m c
-constexpr float kFill = -1e30f;  // stands in an excluded column: 2^(kFill c - k) is 0
+float fast_limit(float c) { return 0x1.Fp30f / c; }
 
-__device__ __forceinline__ Running running_none(float c) { return {soft_none(), kFast, kFast * c}; }
+__device__ __forceinline__ bool is_fast(float m, float limit) { return m > -limit && m <= limit; }
+
+__device__ __forceinline__ Running running_none(float c, float limit) { return {soft_none(), -limit, -limit * c}; }
 
 // To the reference m (t in units of z) and back.
-__device__ __forceinline__ SoftStats settled(const Running& r, float c) {
-  if (!(r.a.m > kFast && r.a.m <= -kFast)) return r.a;
+__device__ __forceinline__ SoftStats settled(const Running& r, float c, float limit) {
+  if (!is_fast(r.a.m, limit)) return r.a;
   const float rest = fmaf(r.a.m, c, -r.k);
   const float back = __builtin_amdgcn_exp2f(-rest);
   return {r.a.m, r.a.s * back, (r.a.t - rest * r.a.s) * back / c};
 }
 
-__device__ __forceinline__ Running running_of(const SoftStats& a, float c) {
-  Running r{a, fmaxf(a.m, kFast), 0.0f};
+__device__ __forceinline__ Running running_of(const SoftStats& a, float c, float limit) {
+  Running r{a, fmaxf(a.m, -limit), 0.0f};
   r.k = r.least * c;
-  if (a.m > kFast && a.m <= -kFast) {
+  if (is_fast(a.m, limit)) {
     const float rest = fmaf(a.m, c, -r.k), on = __builtin_amdgcn_exp2f(rest);
     r.a.s = a.s * on;
     r.a.t = (a.t * c + rest * a.s) * on;
@@ -140,38 +148,39 @@ __device__ __forceinline__ float min8(const float v[8]) {
 // Adds a unit's scores, those that `pass` excludes (MASKED) left out, to a
 // thread's statistics; true when they hold a new maximum.
 template <bool MASKED>
-__device__ __forceinline__ bool take_unit(Running& r, float v[8], uint32_t pass, float c) {
+__device__ __forceinline__ bool take_unit(Running& r, float v[8], uint32_t pass, float c, float limit) {
+  const float fill = -2.0f * limit;  // stands in an excluded column: 2^(fill c - k) is 0
   const float low = min8(v);
-  if constexpr (MASKED) exclude8(v, pass, kFill);
+  if constexpr (MASKED) exclude8(v, pass, fill);
   float top = max8(v);
-  if (__any(!(low > kFast) || fmaxf(top, r.least) > -kFast)) {
+  if (__any(!(low > -limit) || fmaxf(top, r.least) > limit)) {
     if constexpr (MASKED) {
       exclude8(v, pass, kMinusInf);
       top = max8(v);
     }
     // Maxima that are not ordinary take the general way; -inf and very low
     // scores beside ordinary ones count as excluded ones do (their e is 0).
-    const bool general = fmaxf(top, r.a.m) > -kFast || (top > kMinusInf && top <= kFast && !(r.a.m > kFast));
+    const bool general = fmaxf(top, r.a.m) > limit || (top > kMinusInf && top <= -limit && !(r.a.m > -limit));
     if (__any(general)) {
       const float before = r.a.m;
-      r = running_of(take_any(settled(r, c), v, top, c), c);
+      r = running_of(take_any(settled(r, c, limit), v, top, c), c, limit);
       return r.a.m > before;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = v[i] < kFill ? kFill : v[i];
+    for (int i = 0; i < 8; ++i) v[i] = v[i] < fill ? fill : v[i];
   }
   const bool higher = top > r.least;
   if (higher) {
-    const float k = top * c;
-    if (r.a.m > kFast) {
+    if (r.a.m > -limit) {
+      const float k = top * c;
       const float d = r.k - k, scale = __builtin_amdgcn_exp2f(d);
       r.a.t = scale == 0.0f ? 0.0f : (r.a.t + r.a.s * d) * scale;
       r.a.s *= scale;
-    } else {
-      r.a = soft_rebase(r.a, top, c);  // nothing yet, or scores too low to count
+      r.a.m = r.least = top;
+      r.k = k;
+    } else {  // nothing yet, or lower maxima, kept relative to themselves
+      r = running_of(soft_rebase(r.a, top, c), c, limit);
     }
-    r.a.m = r.least = top;
-    r.k = k;
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -442,7 +451,7 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 8) void logprobs_kernel(LogprobsA
     const uint64_t* mask = MASKED ? a.mask + r * a.mask_stride : nullptr;
     const uint32_t full = static_cast<uint32_t>(columns / kUnit);
     const int64_t target_id = tid == 0 && a.chunks == 1 ? a.targets[r] : -1;
-    Running run = running_none(a.c);
+    Running run = running_none(a.c, a.limit);
     uint32_t top_unit = 0;
     // units a thread has in flight: 64 bytes, half that beside the filter's registers
     constexpr int kAhead = (DT == ST_SCORE_F32 ? 2 : 4) / (MASKED ? 2 : 1);
@@ -460,7 +469,7 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 8) void logprobs_kernel(LogprobsA
       for (int i = 0; i < kAhead; ++i) {
         float v[8];
         unpack8<DT>(raw[i], v);
-        if (take_unit<MASKED>(run, v, pass[i], a.c)) top_unit = u + i * T;
+        if (take_unit<MASKED>(run, v, pass[i], a.c, a.limit)) top_unit = u + i * T;
       }
     }
     const uint32_t units = static_cast<uint32_t>((columns + kUnit - 1) / kUnit);
@@ -470,9 +479,9 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 8) void logprobs_kernel(LogprobsA
       load_unit<DT, false>(row, mask, col, u < full ? kUnit : static_cast<int>(columns % kUnit), v);
       uint32_t pass = 0xFFu;
       if constexpr (MASKED) pass = pass_byte(mask, col / kUnit);
-      if (take_unit<MASKED>(run, v, pass, a.c)) top_unit = u;
+      if (take_unit<MASKED>(run, v, pass, a.c, a.limit)) top_unit = u;
     }
-    SoftStats st = settled(run, a.c);
+    SoftStats st = settled(run, a.c, a.limit);
     const Target target = find_target<DT>(a, r, target_id);  // one thread's
     if (a.topk > 0) {
       select_top<DT, MASKED, T>(l, row, mask, first, columns, st.m, top_unit, a.topk, [&] { joined.put(st, a.c); });
@@ -795,6 +804,7 @@ extern "C" int st_target_logprobs(const void* logits, int score_type, int64_t ro
     a.topk = static_cast<int>(topk);
     a.c = static_cast<float>(1.4426950408889634 / temperature);
     a.inv_t = static_cast<float>(1.0 / temperature);
+    a.limit = fast_limit(a.c);
     a.chunks = row_chunks(rows, columns);
     a.chunk_columns = ((columns + a.chunks - 1) / a.chunks + kUnit - 1) / kUnit * kUnit;
     if (a.chunks > 1) {

@@ -1,0 +1,131 @@
+"""The retrieval head's operators at scores that are large against the temperature, or share a large offset, against
+plain 64-bit forms (tests/head_oracle.py).
+
+Probabilities and their gradients depend on the scores' distances alone, so none of the tolerances here grows with an
+offset (u = 2^-24, the rounding of 32 bits; L = log columns):
+- an exponential's argument d = (z - max) / T, in units of log 2, has a few roundings of relative u, which moves the
+  exponential by a few u |d|; a sum of them is dominated by terms of |d| below a few L, and its additions stay below
+  32 u (a few hundred terms a thread, then a tree).  A log-probability is such a sum's logarithm and one distance of its own
+  size: 64 u (1 + L + |value|); the entropy is a difference of two values of size L: 64 u (1 + 2 L); lse has the offset
+  itself: 64 u (1 + L + |value|).
+- a probability has the relative error 64 u (1 + L + |log p|), and a gradient's element twice that of the sum of the
+  absolute values of its terms, then one rounding to its type.
+"""
+
+import math
+
+import pytest
+import torch
+
+from tests import gpu_helpers as H
+from tests import head_oracle as O
+from tests.test_gpu_head import HALF, TINY, TYPES, U, _near
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU tests need a HIP device")
+    import silvertorch_amd.ops._load_ops  # noqa: F401
+
+
+# ------------------------------------------------------------------ log-probabilities
+
+
+def _check_logprobs(logits, targets, topk, mask, temperature):
+    """Every output, and the gradient of all four."""
+    rows, columns = logits.shape
+    wide = math.log(max(2, columns))
+    x = logits.cuda().requires_grad_()
+    out = torch.ops.st.target_logprobs(x, targets.cuda(), topk, mask.cuda() if mask is not None else None, temperature)
+    # At 1e15 and more 64 bits cannot hold a sum's logarithm beside the offset: the form takes the distances from each
+    # row's largest score, and lse the offset afterwards.
+    raw, allowed = logits.double(), torch.ones(logits.shape, dtype=torch.bool)
+    if mask is not None:
+        allowed = O.bits(mask.expand(rows, -1), columns)
+    top = torch.where(allowed, raw, -math.inf).amax(1)
+    leaf = torch.where(allowed, raw - top.unsqueeze(1), 0.0).requires_grad_()
+    want = list(O.target_logprobs(leaf, targets, topk, mask, temperature))
+    assert torch.equal(out[3].cpu(), want[3]), "top_ids"
+    want_lse = want[2].detach() + top / temperature
+    _near(out[2], want_lse, 64 * U * (1 + wide + want_lse.abs()), "lse")
+    for i, what in ((0, "logprobs"), (4, "top_logprobs")):
+        size = torch.where(torch.isfinite(want[i]), want[i].detach(), 0.0).abs()
+        _near(out[i], want[i], 64 * U * (1 + wide + size), what)
+    _near(out[1], want[1], 64 * U * (1 + 2 * wide), "entropy")
+
+    g = torch.Generator().manual_seed(rows * 31 + columns)
+    cot = [torch.randn(o.shape, generator=g) for o in (out[0], out[1], out[2], out[4])]
+    got, = torch.autograd.grad([out[0], out[1], out[2], out[4]], [x], [c.cuda() for c in cot])
+    total = sum((torch.where(torch.isfinite(w), w, 0.0) * c).sum() for w, c in zip((want[0], want[1], want[2], want[4]), cot))
+    grad, = torch.autograd.grad(total, leaf)
+    with torch.no_grad():
+        z = torch.where(allowed, leaf / temperature, -math.inf)
+        lse = want[2].unsqueeze(1)
+        p = torch.where(allowed, (z - lse).exp(), 0.0)
+        logp = torch.where(p > 0, z - lse, 0.0)
+        whole = cot[0].abs() + cot[2].abs() + cot[3].abs().sum(1)
+        terms = p * (whole.unsqueeze(1) + cot[1].abs().unsqueeze(1) * (logp.abs() + want[1].unsqueeze(1)))
+        terms.scatter_add_(1, targets.clamp(0, columns - 1).unsqueeze(1), cot[0].abs().double().unsqueeze(1))
+        terms.scatter_add_(1, want[3].clamp(min=0), cot[3].abs().double())
+        atol = terms / temperature * (128 * U * (1 + wide + logp.abs()) + HALF[logits.dtype] * 1.01) + TINY[logits.dtype]
+    _near(got, grad, atol, "grad_logits")
+    assert not got.cpu()[~allowed].any()
+
+
+# z / T of a row's scores: where the product with log2 e has an ulp of a hundredth, of more than one, and of more than
+# the exponents of 32 bits
+CENTRES = [1e3, 1e5, 3e6, 4.65e7, 1e8, 1.4e9, 1.44e9, 1.49e9, 2e9, 1e10, 1e15, 1e25]
+
+
+@pytest.mark.parametrize("columns", [300, 70_001])
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 1.0, 1e3])
+@pytest.mark.parametrize("centre", [s * c for c in CENTRES for s in (1, -1)])
+def test_logprobs_far_from_zero(centre, temperature, columns):
+    """Rows around a large score, an ordinary one beside them, rows of both, with either sign, filtered and whole."""
+    H.note(f"[logprobs] scores / T around {centre} T {temperature} columns {columns}")
+    g = torch.Generator().manual_seed(columns)
+    noise = torch.randn((6, columns), generator=g).double() * 2
+    at = torch.arange(columns)
+    z = noise.clone()
+    z[0] += centre
+    z[1] += torch.where(at % 2 == 0, centre, 0.0)
+    z[2] += torch.where(at < columns // 2, centre, -centre)
+    z[3] += torch.where(at // 8 % 5 == 0, -centre, centre)
+    z[5] += centre * (1 + (at % 7) * 2.0 ** -22)
+    logits = (z * temperature).float()
+    targets = torch.randint(0, columns, (6,), generator=g)
+    passes = torch.rand((6, columns), generator=g) < 0.4
+    passes[torch.arange(6), targets] = True
+    for mask in (None, O.pack(passes)):
+        _check_logprobs(logits, targets, 7, mask, temperature)
+
+
+@pytest.mark.parametrize("columns", [300, 70_001])
+@pytest.mark.parametrize("dtype,temperature,scale", [
+    (torch.float16, 1e-5, 20_000.0), (torch.float16, 1e-6, 500.0), (torch.bfloat16, 1.0, 1e12), (torch.bfloat16, 1e-3, 1e6),
+    (torch.bfloat16, 1.0, 1e32), (torch.float32, 1.0, 1e9), (torch.float32, 1e-6, 1e4), (torch.float32, 1e6, 1e15)])
+def test_logprobs_wide_scores(dtype, temperature, scale, columns):
+    """Scores that spread over many multiples of the temperature."""
+    H.note(f"[logprobs] wide scores {dtype} T {temperature} scale {scale} columns {columns}")
+    g = torch.Generator().manual_seed(3)
+    largest = torch.finfo(dtype).max
+    logits = (torch.randn((3, columns), generator=g) * scale).clamp(-largest, largest).to(dtype)
+    targets = torch.randint(0, columns, (3,), generator=g)
+    targets[0] = logits[0].float().argmax()
+    _check_logprobs(logits, targets, 4, None, temperature)
+
+
+@pytest.mark.parametrize("temperature", [1e-6, 1.0])
+@pytest.mark.parametrize("columns", [20_000, 70_001])
+def test_logprobs_rise_through_large_scores(columns, temperature):
+    """Scores that rise, or fall, through the large ones of either sign, a little a column: every thread meets them in
+    order."""
+    H.note(f"[logprobs] rising scores T {temperature} columns {columns}")
+    at = torch.arange(columns).double()
+    up = [c + at * (64.0 / columns) * step for c in (-4.65e7, 4.65e7, -3.3e7, 9.3e7) for step in (1, 16)]
+    up += [c + at * (1e9 / columns) for c in (1e9, -2e9, -1.5e9)]
+    z = torch.stack(up + [r.flip(0) for r in up])
+    _check_logprobs((z * temperature).float(), torch.arange(len(z)) * 11, 3, None, temperature)
