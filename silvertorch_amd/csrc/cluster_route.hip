@@ -416,10 +416,12 @@ __global__ __launch_bounds__(kThreads<LPR>, 4) void route_kernel(RouteArgs a) {
       }
     }
 
-    // exponentials and their sum; scores past 1e30 either way are taken relative
-    // to the maximum, whose product with c may not be finite
+    // Exponentials and their sum.  The rounding of ref is half an ulp of m c at
+    // most, 1/16 below the bound here (from 2^31 on it could pass the exponents
+    // of 32 bits); rows with larger maxima, either way, are taken relative to m
+    // itself.
     const float m = top == kMinusInf ? 0.0f : top;
-    const bool wide = !(fabsf(m) < 1e30f);
+    const bool wide = !(fabsf(m) < 0x1p20f);
     const float ref = wide ? 0.0f : m * kLog2e;
     auto exponential = [&](float z) {
       return __builtin_amdgcn_exp2f(wide ? (z - m) * kLog2e : fmaf(z, kLog2e, -ref));
@@ -501,7 +503,7 @@ __global__ __launch_bounds__(kThreads<LPR>, 4) void route_kernel(RouteArgs a) {
       wave_fence();
     }
     const bool some = !(top == kMinusInf && sum == 0.0f);
-    const float inv = some ? __builtin_amdgcn_rcpf(sum) : 0.0f;  // sum is 1 or more
+    const float inv = some ? __builtin_amdgcn_rcpf(sum) : 0.0f;  // sum is 2^(-1/16) or more
 #pragma unroll
     for (int i = 0; i < U * 8; ++i) acc[i] = fmaf(LPR > 8 ? v[i] : exponential(v[i]), inv, acc[i]);
     if (mine && in_row == 0) {

@@ -129,3 +129,50 @@ def test_logprobs_rise_through_large_scores(columns, temperature):
     up += [c + at * (1e9 / columns) for c in (1e9, -2e9, -1.5e9)]
     z = torch.stack(up + [r.flip(0) for r in up])
     _check_logprobs((z * temperature).float(), torch.arange(len(z)) * 11, 3, None, temperature)
+
+
+# ------------------------------------------------------------------ routing
+
+
+def _route_rows(clusters, centre, dtype):
+    """Rows around a large score, ordinary ones, rows of both, with either sign."""
+    g = torch.Generator().manual_seed(clusters)
+    z = torch.randn((9, clusters), generator=g).double() * 2
+    at = torch.arange(clusters)
+    z[0] += centre
+    z[2] += torch.where(at % 2 == 0, centre, 0.0)
+    z[4] += torch.where(at < clusters // 2, centre, -centre)
+    z[5] += centre * (1 + (at % 7) * 2.0 ** -22)
+    z[8] -= centre
+    return z.to(dtype)
+
+
+def _route_oracle(logits, probes):
+    """The form of the distances from each row's largest score (what lies at the offset 64 bits cannot hold beside a
+    sum's logarithm), lse with the offset; and log p."""
+    top = logits.double().amax(1)
+    leaf = (logits.double() - top.unsqueeze(1)).requires_grad_()
+    want = list(O.cluster_route(leaf, probes))
+    log_p = (leaf - want[2].unsqueeze(1)).detach()
+    return leaf, want, want[2].detach() + top, log_p
+
+
+ROUTE_CENTRES = [1e3, 1e5, 1e6, 1.04e6, 1.05e6, 3e6, 1e8, 1.45e9, 3e9, 1e10, 1e15, 1e25, 9e29, 2e30]
+
+
+@pytest.mark.parametrize("clusters,probes", [(60, 5), (200, 16), (700, 8), (1800, 30), (3000, 12), (10_000, 20)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("centre", [s * c for c in ROUTE_CENTRES for s in (1, -1)])
+def test_route_far_from_zero(centre, dtype, clusters, probes):
+    """The outputs of rows around a large score, and the loss over them and ordinary ones."""
+    H.note(f"[route] scores around {centre} {dtype} clusters {clusters}")
+    logits = _route_rows(clusters, centre, dtype)
+    out = torch.ops.st.cluster_route(logits.cuda(), probes)
+    _, want, lse, log_p = _route_oracle(logits, probes)
+    wide = math.log(clusters)
+    assert torch.equal(out[0].cpu(), want[0]) and torch.equal(out[3].cpu(), want[3])
+    size = log_p.gather(1, want[0]).abs()
+    _near(out[1], want[1], 64 * U * (1 + wide + size) * want[1].detach() + 1e-37, "weights")
+    _near(out[2], lse, 64 * U * (1 + wide + lse.abs()), "lse")
+    # a sum over the rows, one more rounding for each
+    _near(out[4], want[4], U * (64 * (1 + 2 * wide) + len(logits)) * want[4].detach(), "loss")
