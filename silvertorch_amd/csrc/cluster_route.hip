@@ -49,7 +49,7 @@ struct RouteArgs {
   int clusters, probes;
   const uint8_t* valid;   // null: all
   int64_t* ids;
-  float *weights, *lse, *stats;  // stats [rows, 2]: max and sum of exponentials
+  float *weights, *lse, *stats;  // stats [rows, 2]: max and sum of exponentials (reference)
   float* part_sums;       // [groups, clusters]
   uint32_t* part_counts;  // [groups, clusters]
   uint32_t* part_rows;    // [groups]
@@ -58,6 +58,12 @@ struct RouteArgs {
   int64_t* counts;
   float *slopes, *loss;
 };
+
+// A row's exponentials are 2^(z c - ref), c = log2 e and ref = m c rounded, or,
+// of rows whose maximum m is wide, 2^((z - m) c).  The rounding is half an ulp
+// of m c at most, 1/16 for those that are not; from 2^31 on it could pass the
+// exponents of 32 bits.
+__device__ __forceinline__ bool is_wide(float m) { return !(fabsf(m) < 0x1p20f); }
 
 template <int LPR>
 __device__ __forceinline__ float row_sum(float x, float* red) {
@@ -416,12 +422,9 @@ __global__ __launch_bounds__(kThreads<LPR>, 4) void route_kernel(RouteArgs a) {
       }
     }
 
-    // Exponentials and their sum.  The rounding of ref is half an ulp of m c at
-    // most, 1/16 below the bound here (from 2^31 on it could pass the exponents
-    // of 32 bits); rows with larger maxima, either way, are taken relative to m
-    // itself.
+    // exponentials and their sum
     const float m = top == kMinusInf ? 0.0f : top;
-    const bool wide = !(fabsf(m) < 0x1p20f);
+    const bool wide = is_wide(m);
     const float ref = wide ? 0.0f : m * kLog2e;
     auto exponential = [&](float z) {
       return __builtin_amdgcn_exp2f(wide ? (z - m) * kLog2e : fmaf(z, kLog2e, -ref));
@@ -799,7 +802,11 @@ __global__ __launch_bounds__(kThreads<LPR>) void route_backward_kernel(RouteBack
     load(r + stride, next);
     const bool some = !(top == kMinusInf && sum == 0.0f);
     const float m = top == kMinusInf ? 0.0f : top;
-    const float inv = some ? 1.0f / sum : 0.0f;
+    // Exponentials are relative to m here, the sum is to the rounded m c: 2^rest
+    // between them.  (Put back where the sum is stored, the forward kernel took
+    // 129 us instead of 111 for 65,536 x 200 with 32 probes.)
+    const float rest = is_wide(m) ? 0.0f : fmaf(m, kLog2e, -(m * kLog2e));
+    const float inv = some ? __builtin_amdgcn_exp2f(rest) / sum : 0.0f;
     float dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < U * 8; ++i) {

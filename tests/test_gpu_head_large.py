@@ -176,3 +176,52 @@ def test_route_far_from_zero(centre, dtype, clusters, probes):
     _near(out[2], lse, 64 * U * (1 + wide + lse.abs()), "lse")
     # a sum over the rows, one more rounding for each
     _near(out[4], want[4], U * (64 * (1 + 2 * wide) + len(logits)) * want[4].detach(), "loss")
+
+
+@pytest.mark.parametrize("clusters,probes", [(60, 5), (200, 16), (700, 8), (1800, 30), (3000, 12), (10_000, 20)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("centre", [s * c for c in ROUTE_CENTRES for s in (1, -1)])
+def test_route_gradient_far_from_zero(centre, dtype, clusters, probes):
+    """The gradient of rows around a large score."""
+    H.note(f"[route] gradient around {centre} {dtype} clusters {clusters}")
+    logits = _route_rows(clusters, centre, dtype)
+    rows, wide = len(logits), math.log(clusters)
+    x = logits.cuda().requires_grad_()
+    out = torch.ops.st.cluster_route(x, probes)
+    leaf, want, _, log_p = _route_oracle(logits, probes)
+    g = torch.Generator().manual_seed(rows)
+    cot = [torch.randn(out[1].shape, generator=g), torch.randn(out[2].shape, generator=g), torch.tensor(1.7)]
+    got, = torch.autograd.grad([out[1], out[2], out[4]], [x], [c.cuda() for c in cot])
+    grad, = torch.autograd.grad(sum((w * c).sum() for w, c in zip((want[1], want[2], want[4]), cot)), leaf)
+    p = log_p.exp()
+    a = (1.7 * clusters * want[3].double() / (probes * rows * rows)).expand_as(p).clone()
+    a.scatter_add_(1, want[0], cot[0].abs().double())
+    terms = p * (a + (p * a).sum(1, keepdim=True) + cot[1].abs().unsqueeze(1))
+    log_p = torch.where(p > 0, log_p, 0.0)
+    _near(got, grad, terms * (128 * U * (1 + wide + log_p.abs()) + HALF[dtype] * 1.01) + TINY[dtype], "grad_logits")
+
+
+@pytest.mark.parametrize("clusters", [60, 700, 5000])
+@pytest.mark.parametrize("offset", [2.0 ** 10, 2.0 ** 16, 2.0 ** 19, 2.0 ** 20, 2.0 ** 22])
+def test_gradients_without_the_offset(offset, clusters):
+    """Scores of multiples of a half have gradients, of both operators, that an offset does not change: each side is
+    within 128 u (1 + L + |log p|) of the terms' sizes, which are at most 2 max |cotangent| p here."""
+    H.note(f"[head] offset {offset} clusters {clusters}")
+    g = torch.Generator().manual_seed(5)
+    z = torch.randint(-12, 12, (7, clusters), generator=g).float() / 2
+    weights = torch.randn((7, 6), generator=g).cuda()
+    targets = torch.randint(0, clusters, (7,), generator=g).cuda()
+
+    def gradients(scores):
+        x = scores.cuda().requires_grad_()
+        route = torch.autograd.grad((torch.ops.st.cluster_route(x, 6)[1] * weights).sum(), x)[0]
+        o = torch.ops.st.target_logprobs(x, targets)
+        return route.cpu().double(), torch.autograd.grad(o[0].sum() + o[1].sum(), x)[0].cpu().double()
+
+    p = torch.softmax(z.double(), 1)
+    size = 128 * U * (1 + math.log(clusters) + p.log().abs())
+    at = torch.zeros_like(p).scatter_(1, targets.cpu().unsqueeze(1), 1.0)
+    entropy = -(p * p.log()).sum(1, keepdim=True)
+    for (a, b), terms in zip(zip(gradients(z), gradients(z + offset)),
+                             (2 * p * weights.abs().max().item(), at + p * (1 + p.log().abs() + entropy))):
+        _near(b.float(), a, 2 * size * terms + 1e-37)
