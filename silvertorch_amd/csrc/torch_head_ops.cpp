@@ -3,7 +3,8 @@
 //
 // As in torch_ops.cpp, GPU tensors run on their device's current stream and
 // CPU tensors are copied to the current GPU and the results back.  The two
-// operators a model is trained through carry their gradients (Autograd key).
+// operators a model is trained through carry their gradients (Autograd key);
+// the 4-bit ones refuse to be differentiated.
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
@@ -128,6 +129,64 @@ Tensor int4_matvec_cpu(const Tensor& packed, const Tensor& scales, const Tensor&
   check_matvec(packed, scales, x, group_size, zeros, out_dtype.value_or(x.scalar_type()));
   const at::Device gpu = gpu_for_cpu_call();
   return int4_matvec_gpu(packed.to(gpu), scales.to(gpu), x.to(gpu), group_size, moved(zeros, gpu), out_dtype).cpu();
+}
+
+// The 4-bit operators have no gradients.  Their results say so when one is
+// asked for, where they would otherwise count as constants.
+template <typename Op>
+auto find_op(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Op>();
+}
+
+using QuantizeOp = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, int64_t, bool);
+using MatvecOp = Tensor(const Tensor&, const Tensor&, const Tensor&, int64_t, const OptTensor&,
+                        std::optional<at::ScalarType>);
+
+std::tuple<Tensor, Tensor, Tensor> quantize_below(const Tensor& weight, int64_t group_size, bool symmetric) {
+  static const auto op = find_op<QuantizeOp>("st::int4_quantize");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(weight, group_size, symmetric);
+}
+
+Tensor matvec_below(const Tensor& packed, const Tensor& scales, const Tensor& x, int64_t group_size,
+                    const OptTensor& zeros, std::optional<at::ScalarType> out_dtype) {
+  static const auto op = find_op<MatvecOp>("st::int4_matvec");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(packed, scales, x, group_size, zeros, out_dtype);
+}
+
+struct QuantizeFunction : torch::autograd::Function<QuantizeFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& weight, int64_t group_size, bool symmetric) {
+    auto [packed, scales, zeros] = quantize_below(weight, group_size, symmetric);
+    ctx->mark_non_differentiable({packed, zeros});
+    return {packed, scales, zeros};
+  }
+  static variable_list backward(AutogradContext* /*ctx*/, variable_list /*grads*/) {
+    TORCH_CHECK(false, "int4_quantize has no gradient");
+  }
+};
+
+struct MatvecFunction : torch::autograd::Function<MatvecFunction> {
+  static Tensor forward(AutogradContext* /*ctx*/, const Tensor& packed, const Tensor& scales, const Tensor& x,
+                        int64_t group_size, const OptTensor& zeros, std::optional<at::ScalarType> out_dtype) {
+    return matvec_below(packed, scales, x, group_size, zeros, out_dtype);
+  }
+  static variable_list backward(AutogradContext* /*ctx*/, variable_list /*grads*/) {
+    TORCH_CHECK(false, "int4_matvec has no gradient");
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> int4_quantize_autograd(const Tensor& weight, int64_t group_size, bool symmetric) {
+  if (!at::GradMode::is_enabled() || !weight.requires_grad()) return quantize_below(weight, group_size, symmetric);
+  const variable_list o = QuantizeFunction::apply(weight, group_size, symmetric);
+  return {o[0], o[1], o[2]};
+}
+
+Tensor int4_matvec_autograd(const Tensor& packed, const Tensor& scales, const Tensor& x, int64_t group_size,
+                            const OptTensor& zeros, std::optional<at::ScalarType> out_dtype) {
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || scales.requires_grad()))
+    return matvec_below(packed, scales, x, group_size, zeros, out_dtype);
+  return MatvecFunction::apply(packed, scales, x, group_size, zeros, out_dtype);
 }
 
 // A score row is readable with any row stride; columns have to be adjacent.
@@ -429,6 +488,8 @@ TORCH_LIBRARY_IMPL(st, CPU, m) {
 }
 
 TORCH_LIBRARY_IMPL(st, Autograd, m) {
+  m.impl("int4_quantize", TORCH_FN(int4_quantize_autograd));
+  m.impl("int4_matvec", TORCH_FN(int4_matvec_autograd));
   m.impl("target_logprobs", TORCH_FN(target_logprobs_autograd));
   m.impl("cluster_route", TORCH_FN(cluster_route_autograd));
 }
