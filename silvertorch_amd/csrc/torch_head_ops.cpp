@@ -41,6 +41,13 @@ T* data_or_null(const Tensor& t) {
 
 void* bytes_or_null(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
 
+// None of these operators has a forward-mode derivative: an input that carries
+// a tangent is refused, where the result would otherwise come without one.
+void refuse_tangents(std::initializer_list<const Tensor*> inputs, const char* op) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), op, " has no forward-mode derivative");
+}
+
 Tensor moved(const OptTensor& t, at::Device d) { return t.has_value() && t->defined() ? t->to(d) : Tensor(); }
 
 // ------------------------------------------ 4-bit tables
@@ -177,6 +184,7 @@ struct MatvecFunction : torch::autograd::Function<MatvecFunction> {
 };
 
 std::tuple<Tensor, Tensor, Tensor> int4_quantize_autograd(const Tensor& weight, int64_t group_size, bool symmetric) {
+  refuse_tangents({&weight}, "int4_quantize");
   if (!at::GradMode::is_enabled() || !weight.requires_grad()) return quantize_below(weight, group_size, symmetric);
   const variable_list o = QuantizeFunction::apply(weight, group_size, symmetric);
   return {o[0], o[1], o[2]};
@@ -184,6 +192,7 @@ std::tuple<Tensor, Tensor, Tensor> int4_quantize_autograd(const Tensor& weight, 
 
 Tensor int4_matvec_autograd(const Tensor& packed, const Tensor& scales, const Tensor& x, int64_t group_size,
                             const OptTensor& zeros, std::optional<at::ScalarType> out_dtype) {
+  refuse_tangents({&scales, &x}, "int4_matvec");
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || scales.requires_grad()))
     return matvec_below(packed, scales, x, group_size, zeros, out_dtype);
   return MatvecFunction::apply(packed, scales, x, group_size, zeros, out_dtype);
@@ -352,6 +361,7 @@ Logprobs target_logprobs(const Tensor& logits, const Tensor& targets, int64_t to
 
 Logprobs target_logprobs_autograd(const Tensor& logits, const Tensor& targets, int64_t topk, const OptTensor& mask,
                                   double temperature) {
+  refuse_tangents({&logits}, "target_logprobs");
   if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
     at::AutoDispatchBelowADInplaceOrView below;
     return target_logprobs(logits, targets, topk, mask, temperature);
@@ -448,6 +458,7 @@ Route cluster_route(const Tensor& logits, int64_t probes, const OptTensor& valid
 }
 
 Route cluster_route_autograd(const Tensor& logits, int64_t probes, const OptTensor& valid) {
+  refuse_tangents({&logits}, "cluster_route");
   if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
     at::AutoDispatchBelowADInplaceOrView below;
     return cluster_route(logits, probes, valid);

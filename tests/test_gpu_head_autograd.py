@@ -69,3 +69,27 @@ def test_module_refuses_to_train_through_its_table():
     assert torch.equal(logprobs.detach(), again[0]) and torch.equal(ids, again[3])
     _refuses("int4_matvec has no gradient", lambda: (-logprobs.mean()).backward())
     assert all(p.grad is None for p in tower.parameters())
+
+
+def test_tangents_are_refused():
+    """An input with a forward-mode tangent is refused; beside one, and with forward mode off, calls are as ever."""
+    H.note("[head] tangents")
+    import torch.autograd.forward_ad as fwAD
+
+    z = torch.randn((3, 300), generator=torch.Generator().manual_seed(1)).cuda()
+    targets = torch.arange(3, device="cuda")
+    packed, scales, zeros = torch.ops.st.int4_quantize(z, 32)
+    calls = {
+        "target_logprobs": lambda t: torch.ops.st.target_logprobs(t, targets, 4),
+        "cluster_route": lambda t: torch.ops.st.cluster_route(t, 4),
+        "int4_matvec": lambda t: (torch.ops.st.int4_matvec(packed, scales, t, 32, zeros),),
+        "int4_quantize": lambda t: torch.ops.st.int4_quantize(t, 32),
+    }
+    for name, call in calls.items():
+        want = call(z)
+        with fwAD.dual_level():
+            dual = fwAD.make_dual(z, torch.ones_like(z))
+            _refuses(f"{name} has no forward-mode derivative", lambda: call(dual))
+            with fwAD._set_fwd_grad_enabled(False):
+                assert all(torch.equal(a, b) for a, b in zip(call(dual), want))
+            assert all(torch.equal(a, b) for a, b in zip(call(fwAD.unpack_dual(dual).primal), want))
