@@ -678,6 +678,9 @@ void launch_matvec(MatvecArgs& a, hipStream_t s) {
   });
 }
 
+// Any group size of check_table is in range: one past the columns makes one group.
+int64_t groups_of(int64_t dim, int64_t group_size) { return (dim - 1) / group_size + 1; }
+
 void check_type(int type, const char* what) {
   ST_CHECK(type == ST_SCORE_F32 || type == ST_SCORE_F16 || type == ST_SCORE_BF16, what,
            " must be float32, float16 or bfloat16");
@@ -700,7 +703,7 @@ extern "C" int st_int4_quantize(const void* weight, int weight_type, int64_t row
     check_table(rows, dim, group_size);
     if (rows == 0) return;
     ST_CHECK(weight && packed && scales && zeros, "null device pointer");
-    QuantizeArgs a{weight, packed, scales, zeros, rows, dim, group_size, (dim + group_size - 1) / group_size,
+    QuantizeArgs a{weight, packed, scales, zeros, rows, dim, group_size, groups_of(dim, group_size),
                    (dim + kBlock - 1) / kBlock * (kBlock / 2), symmetric};
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>((rows * a.groups + 3) / 4, 64ll * cu_count()));
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -736,7 +739,7 @@ extern "C" int st_int4_matvec(const uint8_t* packed, const void* scales, int sca
     a.rows = rows;
     a.queries = queries;
     a.dim = static_cast<int>(dim);
-    a.groups = static_cast<int>((dim + group_size - 1) / group_size);
+    a.groups = static_cast<int>(groups_of(dim, group_size));
     a.blocks = static_cast<int>((dim + kBlock - 1) / kBlock);
     a.row_bytes = a.blocks * (kBlock / 2);
     a.group_blocks = static_cast<int>(std::min<int64_t>(group_size / kBlock, a.blocks));

@@ -69,7 +69,7 @@ std::tuple<Tensor, Tensor, Tensor> int4_quantize_gpu(const Tensor& weight_in, in
   check_quantize(weight_in, group_size);
   c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(weight_in.device());
   const Tensor weight = weight_in.contiguous();
-  const int64_t n = weight.size(0), dim = weight.size(1), groups = (dim + group_size - 1) / group_size;
+  const int64_t n = weight.size(0), dim = weight.size(1), groups = (dim - 1) / group_size + 1;
   const auto bytes = weight.options().dtype(at::kByte);
   Tensor packed = at::empty({n, (dim + kInt4Block - 1) / kInt4Block * (kInt4Block / 2)}, bytes);
   Tensor scales = at::empty({n, groups}, weight.options());
@@ -97,7 +97,7 @@ void check_matvec(const Tensor& packed, const Tensor& scales, const Tensor& x, i
   score_type(out_type, "out_dtype");
   const int64_t n = packed.size(0), dim = x.size(-1);
   TORCH_CHECK(dim >= 1, "x must have at least one column");
-  const int64_t groups = (dim + group_size - 1) / group_size;
+  const int64_t groups = (dim - 1) / group_size + 1;
   const int64_t row_bytes = (dim + kInt4Block - 1) / kInt4Block * (kInt4Block / 2);
   TORCH_CHECK(packed.size(1) == row_bytes, "packed has ", packed.size(1), " bytes a row, ", dim, " columns take ",
               row_bytes);

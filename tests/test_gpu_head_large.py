@@ -225,3 +225,22 @@ def test_gradients_without_the_offset(offset, clusters):
     for (a, b), terms in zip(zip(gradients(z), gradients(z + offset)),
                              (2 * p * weights.abs().max().item(), at + p * (1 + p.log().abs() + entropy))):
         _near(b.float(), a, 2 * size * terms + 1e-37)
+
+
+# ------------------------------------------------------------------ 4-bit tables
+
+
+@pytest.mark.parametrize("group_size", [1 << 21, 1 << 40, (1 << 63) - 32])
+def test_group_sizes_past_the_columns(group_size):
+    """One group, as of the first multiple of 32 that holds the columns."""
+    H.note(f"[int4] group size {group_size}")
+    g = torch.Generator().manual_seed(2)
+    for dim in (1, 31, 32, 40, 300):
+        w, x = torch.randn((70, dim), generator=g).cuda(), torch.randn((3, dim), generator=g).cuda()
+        least = -(-dim // 32) * 32
+        for symmetric in (True, False):
+            want = torch.ops.st.int4_quantize(w, least, symmetric)
+            got = torch.ops.st.int4_quantize(w, group_size, symmetric)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            assert torch.equal(torch.ops.st.int4_matvec(*got[:2], x, group_size, got[2]),
+                               torch.ops.st.int4_matvec(*want[:2], x, least, want[2]))
