@@ -497,7 +497,8 @@ int st_fused_kmean_ann_noalloc(const int64_t* cluster_offsets, int64_t num_offse
  * st_int4_quantize: weight [rows, dim] to packed, scales (of the weight's type)
  * and zeros, in 32-bit arithmetic with IEEE division.  Symmetric: scale =
  * max |w| / 7, zero 8, code = round(w / scale) + 8; else scale = (max(w, 0) -
- * min(w, 0)) / 15, zero = round(-min(w, 0) / scale), code = round(w / scale)
+ * min(w, 0)) / 15 (of each by itself, where the difference is past float32's
+ * range), zero = round(-min(w, 0) / scale), code = round(w / scale)
  * + zero; the scale is rounded to its type first, ties go to even, codes and
  * zeros are kept in [0, 15].  A group of zeros has scale 0, one with a value
  * that is not finite scale NaN.

@@ -532,8 +532,9 @@ struct QuantizeArgs {
 // weights' type, code = w / scale to the nearest even, kept in [-8, 7], plus 8.
 // Else lo = min(w, 0), hi = max(w, 0): scale = (hi - lo) / 15, zero = -lo /
 // scale, code = w / scale + zero, each to the nearest even and kept in
-// [0, 15].  A group of zeros has scale 0; one with a value that is not finite
-// has scale NaN, so that its products say so.
+// [0, 15]; a difference past float32's range is taken as hi / 15 - lo / 15.  A
+// group of zeros has scale 0; one with a value that is not finite has scale NaN,
+// so that its products say so.
 template <int DT>
 __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs a) {
   const int lane = threadIdx.x % 64;
@@ -557,7 +558,13 @@ __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs a) {
       hi = fmaxf(hi, __shfl_xor(hi, o));
     }
     finite = __all(finite);
-    float scale = a.symmetric ? __fdiv_rn(fmaxf(-lo, hi), 7.0f) : __fdiv_rn(hi - lo, 15.0f);
+    float scale;
+    if (a.symmetric) {
+      scale = __fdiv_rn(fmaxf(-lo, hi), 7.0f);
+    } else {
+      scale = __fdiv_rn(hi - lo, 15.0f);
+      if (scale == __builtin_inff()) scale = __fdiv_rn(hi, 15.0f) - __fdiv_rn(lo, 15.0f);
+    }
     if (!finite) scale = __builtin_nanf("");
     scale = score_of_bits<DT>(score_bits<DT>(scale));
     const bool any = scale > 0.0f;

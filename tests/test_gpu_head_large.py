@@ -244,3 +244,24 @@ def test_group_sizes_past_the_columns(group_size):
             assert all(torch.equal(a, b) for a, b in zip(got, want))
             assert torch.equal(torch.ops.st.int4_matvec(*got[:2], x, group_size, got[2]),
                                torch.ops.st.int4_matvec(*want[:2], x, least, want[2]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_differences_past_the_type(dtype):
+    """A group from -3e38 to 3e38 has a finite scale, (hi - lo) / 15 to its type's rounding (a rounding of each of two
+    quotients and of their difference before that), and codes within half a step of the weights (the zero point is
+    rounded to a whole code, and so are the weights: one step at most)."""
+    H.note(f"[int4] wide groups {dtype}")
+    w = (torch.randn((6, 96), generator=torch.Generator().manual_seed(4)) * 1e38).clamp(-3.3e38, 3.3e38)
+    w[0, :2] = torch.tensor([3.3e38, -3.3e38])
+    w[1, 40:42] = torch.tensor([-2.9e38, 1.2e38])
+    w[2] = 3.3e38
+    w[3, ::3] = -3.3e38
+    w = w.to(dtype)
+    packed, scales, zeros = (t.cpu() for t in torch.ops.st.int4_quantize(w.cuda(), 32, False))
+    groups = w.double().view(6, 3, 32)
+    lo, hi = groups.amin(2).clamp(max=0), groups.amax(2).clamp(min=0)
+    want = (hi - lo) / 15
+    _near(scales, want, want * (4 * U + HALF[dtype] * 1.01), "scales")
+    back = O.dequantize(packed, scales, zeros, 96, 32)
+    assert ((back - w.double()).abs() <= scales.double().repeat_interleave(32, 1) * 1.01 + want.repeat_interleave(32, 1) * 15 * HALF[dtype]).all()
