@@ -265,3 +265,38 @@ def test_quantize_differences_past_the_type(dtype):
     _near(scales, want, want * (4 * U + HALF[dtype] * 1.01), "scales")
     back = O.dequantize(packed, scales, zeros, 96, 32)
     assert ((back - w.double()).abs() <= scales.double().repeat_interleave(32, 1) * 1.01 + want.repeat_interleave(32, 1) * 15 * HALF[dtype]).all()
+
+
+def test_matvec_bits_of_each_element():
+    """What a product keeps of its vector's elements.  Rows of one code of 1 and scale 1 give the elements back: of
+    float32 vectors each to 2^-23 of itself, at and beside elements 2^27 times as large, and below that to 2^-50 of the
+    largest; of bfloat16 ones exactly down to 2^-31 of the largest, to 2^-39 of it below; float16 ones exactly."""
+    H.note("[int4] bits of each element")
+    dim = 256
+    codes = torch.full((dim, dim), 8, dtype=torch.uint8)
+    codes.fill_diagonal_(9)
+    packed = (codes[:, ::2] | (codes[:, 1::2] << 4)).cuda()
+    scales = torch.ones((dim, dim // 32)).cuda()
+    g = torch.Generator().manual_seed(8)
+
+    def kept(x):
+        return torch.ops.st.int4_matvec(packed, scales, x.cuda(), 32, None, torch.float32).cpu().double()
+
+    for size in (1.0, 2.0 ** 100, 2.0 ** -100):
+        for low in (0, -10, -27, -40, -60):
+            x = (1 + torch.rand((40, dim), generator=g)) * torch.where(torch.rand((40, dim), generator=g) < 0.5, 1.0, -1.0)
+            x *= torch.exp2(torch.randint(low, 1, (40, dim), generator=g).float()) * size
+            x[:, 0] = 1.9999 * size
+            largest = x.double().abs().amax(1, keepdim=True)
+            _near(kept(x).float(), x, torch.maximum(x.double().abs() * 2.0 ** -23, largest * 2.0 ** -50), low)
+            b = x.bfloat16()
+            largest = b.double().abs().amax(1, keepdim=True)
+            near = b.double().abs() >= largest * 2.0 ** -31
+            _near(kept(b).float(), b.double(), torch.where(near, 0.0, largest * 2.0 ** -39), low)
+            # the whole of a float32 vector, as two vectors
+            if low >= -10:
+                top = x.bfloat16().float()
+                assert torch.equal(kept(top) + kept(x - top), x.double())
+    h = torch.randint(-32768, 32768, (40, dim), generator=g, dtype=torch.int16).view(torch.float16)
+    h = torch.where(torch.isfinite(h), h, torch.ones_like(h))
+    assert torch.equal(kept(h), h.double())
