@@ -504,8 +504,11 @@ int st_fused_kmean_ann_noalloc(const int64_t* cluster_offsets, int64_t num_offse
  * that is not finite scale NaN.
  *
  * st_int4_matvec: y [queries, rows] (y_type) = x [queries, dim] (x_type) times
- * the table transposed, summed in 32 bits and rounded once.  float32 vectors
- * keep 22 bits of each element; sums stay finite while scales are below 2^90.
+ * the table transposed, summed in 32 bits and rounded once.  float16 elements
+ * are taken as they are, bfloat16 ones down to 2^-31 of their vector's largest
+ * (to 2^-39 of it below), float32 ones to 2^-23 of themselves down to 2^-27 of
+ * the largest (to 2^-50 of it below).  Sums stay finite while scales are below
+ * 2^90.
  * dim <= 2^21, queries <= 65536.
  * ------------------------------------------------------------------------- */
 int st_int4_quantize(const void* weight, int weight_type, int64_t rows, int64_t dim,

@@ -136,13 +136,18 @@ struct Step {
 
 // Products on the matrix cores: a wave takes 16 table rows as the columns of a
 // 16x16x32 product and up to 16 vectors' parts (C tiles of them) as its rows.
-// Vectors are held in LDS as float16: scaled by a power of two (undone at the
-// end) so that bfloat16 values stay exact down to 2^-28 of the largest, and
-// float32 ones split in two parts, which leaves 2^-22 of each out; they lie in
-// the order that the codes come in.  Codes less zero points are exact in
-// float16; each block of 32 columns (COARSE: each group, of whole 128 columns)
-// is summed by the matrix core in 32 bits and added to the row's sum times its
-// scale in 32 bits.
+// Vectors are held in LDS as float16, scaled by a power of two that brings the
+// largest element to 2^14 or more (undone at the end).  float16's 11 bits and
+// its spacing of 2^-24 near zero hold bfloat16 elements exactly down to 2^-31 of
+// the largest, to 2^-39 of it below.  float32 ones go in two parts, the second
+// 2^11 times as large: what the first leaves out has up to 13 bits with its
+// sign, of which float16 holds all but the last of some, so that an element
+// keeps 2^-23 of itself (down to 2^-27 of the largest, 2^-50 of it below); the
+// rounding of a product in 32 bits is 2^-24.  A third part would hold the last
+// bit, for 4 vectors a tile instead of 8.  The parts lie in the order that the
+// codes come in.  Codes less zero points are exact in float16; each block of 32
+// columns (COARSE: each group, of whole 128 columns) is summed by the matrix
+// core in 32 bits and added to the row's sum times its scale in 32 bits.
 //
 // What bounds it: HBM.  A CU gets some 11 bytes a cycle, 22 codes; unpacking
 // takes 9 vector instructions for 8 codes and one matrix instruction 512, so
@@ -160,7 +165,7 @@ struct Step {
 // moves 5.1); 2.5M x 128, groups of 32 with zero points, 16 vectors to float32
 // 86 us (350 MB, nearly half of it results: 4.05 TB/s); 8,192 x 8,192, one
 // vector 14 us (34.6 MB: a launch, the vector's way to LDS and two steps of each
-// wave); 100,000 x 64 5.4 us.
+// wave); 100,000 x 64 6.4 us.
 template <bool COARSE, bool WIDE, bool ZEROS, int T, int J, int C, int SPREAD, bool STREAMED>
 __global__ __launch_bounds__(kThreads, 2) void matvec_kernel(MatvecArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
@@ -528,8 +533,14 @@ struct QuantizeArgs {
   int symmetric;
 };
 
-// A wave per row and group: run once over a table, bound by its reads.  Symmetric: scale = max |w| / 7 rounded to the
-// weights' type, code = w / scale to the nearest even, kept in [-8, 7], plus 8.
+// A wave per row and group, run once over a table.  Instructions per group bound
+// it, not bytes: bfloat16 and float32 take the same time, 2.5M x 128 2.9 ms in
+// groups of 32 and 0.9 ms in groups of 128 (a copy's rate would take 0.16 ms for
+// the former's bytes in bfloat16); half of the lanes read a group of 32, a
+// quarter of them pack it.
+//
+// Symmetric: scale = max |w| / 7 rounded to the weights' type, code = w / scale
+// to the nearest even, kept in [-8, 7], plus 8.
 // Else lo = min(w, 0), hi = max(w, 0): scale = (hi - lo) / 15, zero = -lo /
 // scale, code = w / scale + zero, each to the nearest even and kept in
 // [0, 15]; a difference past float32's range is taken as hi / 15 - lo / 15.  A
@@ -654,10 +665,14 @@ void launch_matvec(MatvecArgs& a, hipStream_t s) {
   auto phase_of = [&](int columns) { return std::max(16, kVectorLds / (64 * columns) / 16 * 16); };
   // Where four or eight waves share a row but a phase of many vectors has fewer
   // steps than that, some would have none: 16 parts a pass then (64 vectors x
-  // 8,192 columns: 500 rows 160 -> 41 us, 8,192 rows 211 -> 145 us).  With two
-  // waves a row, or one, reading the table again costs more (30,000 x 1,300,
-  // 32 float32 vectors 48 against 55 us; 100,000 x 8,192, 64 vectors 760
-  // against 874 us).
+  // 8,192 columns: 500 rows 160 -> 41 us, 8,192 rows 211 -> 145 us; 64 x 1,100,
+  // 3,000 rows 30 -> 21 us).  With two waves a row, or one, the whole pass and
+  // 16 parts a pass measured both ways, and neither the rows nor the columns
+  // tell them apart: 760 and 874 us (64 vectors, 100,000 x 8,192), 78 and 96 us
+  // (64, 60,000 x 1,500), 48 and 55 us (32 float32, 30,000 x 1,300), 56 and 59
+  // us (20, 20,000 x 4,000), but 179 and 128 us (64, 20,000 x 4,000), 312 and
+  // 242 us (64, 200,000 x 2,000), 247 and 207 us (40, 200,000 x 2,000).  They
+  // read the table once.
   const int most = a.queries_at_once * a.parts;
   if (a.split >= 4 && whole * 64 * most > kWholeVectorLds && a.split > phase_of(most) / 16)
     a.queries_at_once = std::min(a.queries_at_once, 16 / a.parts);

@@ -505,8 +505,9 @@ __global__ __launch_bounds__(T, T == 256 ? 4 : 8) void logprobs_kernel(LogprobsA
 // so their j-th entries bound the k-th best key from below: with j = ceil(2k /
 // parts), ceil(k / j) lists have at least k keys at or above the
 // ceil(k / j)-th largest of them.  Everything is read at the start, the first
-// kRoundUnits * kUnit entries into registers: the kernel is one latency after
-// another (4-10 us), of which the launch is the largest.
+// kRoundUnits * kUnit entries into registers.  Up to a few thousand entries the
+// kernel is one latency after another (4-12 us), of which the launch is the
+// largest; 25,600 (one row of 4M, 100 alternatives) take 26 us.
 template <int DT>
 __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobsArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
