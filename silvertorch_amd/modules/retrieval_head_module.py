@@ -13,7 +13,8 @@ class RetrievalHeadModule(nn.Module):
     """Holds a table of document embeddings in 4 bits as buffers (they follow
     ``.to(device)`` and ``state_dict``; a saved table loads into a new module),
     scores query vectors against it and gives the scores' log-probabilities
-    among the documents that a filter lets pass.
+    among the documents that a filter lets pass.  The table's scores have no
+    gradient: a backward pass through them is an error.
 
     Args:
         group_size: columns that share a scale (a multiple of 32).
