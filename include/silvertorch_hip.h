@@ -594,6 +594,91 @@ int st_cluster_route_backward(const void* logits, int score_type, int64_t rows,
                               const float* grad_weights, const float* grad_lse,
                               const float* grad_loss, void* grad_logits, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Dropout without a stored mask.  No counterpart in the reference.
+ *
+ * y[e] = x[e] * 2^16 / (2^16 - t) where element e stays, else 0, with t = p in
+ * units of 2^-16, rounded.  Which stay comes from Philox4x32-10 (Salmon et al.,
+ * 2011) with key state[0] and counter (e / 8, state[1]): element e has half word
+ * e % 8 of the four words, low halves first, and stays if that is at least t.
+ * state: two int64 on the device, read when the kernel runs.  used (or null): two
+ * int64 that receive them.  The gradient is the same call on the result's
+ * gradient with the state that was used.  0 <= p <= 1; type ST_SCORE_F32, _F16 or
+ * _BF16; contiguous.
+ * ------------------------------------------------------------------------- */
+int st_dropout(const void* x, int type, int64_t elements, double p, const int64_t* state,
+               void* y, int64_t* used, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Layer norm, alone or of a residual plus dropout, and its gradients.  No
+ * counterpart in the reference.
+ *
+ * st_layer_norm: y = n * weight + bias with n = (h - mean h) / sqrt(var h + eps)
+ * for each row h of dim columns (1 to 32768).  h is x's row (x_type; row r starts
+ * at element r * x_stride), or, with a residual (of x's type or ST_SCORE_F32;
+ * rows residual_stride apart), residual + dropout(x) rounded to the residual's
+ * type, which is written to sum as well.  Dropout is st_dropout's, element e =
+ * r * dim + column; p is 0 without a residual.  weight and bias (weight_type; null
+ * for 1 and 0).  y (x's type) and sum are contiguous.  stats (or null) [rows,
+ * ST_NORM_STATS]: what the backward call needs.  Statistics are 32-bit: squares
+ * of what a row is apart from its mean have to sum up below 2^128.
+ *
+ * st_layer_norm_backward: from grad_y (y_type, x's) and grad_sum (h_type, or
+ * null) the gradients of x (y_type), of the residual (h_type), weight and bias
+ * (weight_type), each null where it is not wanted; grad_x is grad_residual's value
+ * through dropout with the state that was used.  h: x or sum.  workspace: device
+ * memory of st_layer_norm_workspace_bytes(rows, dim) bytes, for the last two.  The
+ * same inputs give the same bits.
+ *
+ * st_layer_norm_int8: the norm's rows in 8 bits, from their 32-bit values, as
+ * st_int8_quantize would hold them.
+ * ------------------------------------------------------------------------- */
+#define ST_NORM_STATS 3
+int st_layer_norm(const void* x, int x_type, int64_t rows, int64_t dim, int64_t x_stride,
+                  const void* residual, int residual_type, int64_t residual_stride,
+                  const void* weight, const void* bias, int weight_type, double eps, double p,
+                  const int64_t* state, void* y, void* sum, float* stats, int64_t* used,
+                  void* stream);
+int64_t st_layer_norm_workspace_bytes(int64_t rows, int64_t dim);
+int st_layer_norm_backward(const void* grad_y, int y_type, const void* grad_sum, const void* h,
+                           int h_type, int64_t rows, int64_t dim, int64_t h_stride,
+                           const void* weight, int weight_type, const float* stats, double p,
+                           const int64_t* state, void* workspace, void* grad_x,
+                           void* grad_residual, void* grad_weight, void* grad_bias,
+                           void* stream);
+int st_layer_norm_int8(const void* x, int x_type, int64_t rows, int64_t dim, int64_t x_stride,
+                       const void* weight, const void* bias, int weight_type, double eps,
+                       int8_t* codes, float* scales, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Rows held in 8 bits and their products.  No counterpart in the reference.
+ *
+ * st_int8_quantize: x [rows, dim] (x_type; rows x_stride apart) to codes int8
+ * [rows, st_int8_columns(dim)] (whole blocks of 16 columns, zeros past dim;
+ * 16-byte aligned) and scales [rows]: scale = max |x| / 127, code = x * (127 /
+ * max |x|) to the nearest even, both quotients rounded to 32 bits.  A row whose
+ * largest magnitude is below 2^-119 has scale 0; one with a value that is not
+ * finite has codes 0 and scale NaN.
+ *
+ * st_int8_matmul: y [tokens, rows] (y_type) = x_scales[m] * scales[n] * sum_k
+ * x[m, k] codes[n, k] + bias[n] (bias: float32 or null).  The sum is exact, the
+ * rest in 32 bits, rounded once.  x [tokens, dim] of floats (rows x_stride apart)
+ * is held as st_int8_quantize would hold it, with x_scales null; codes
+ * (ST_CODE_I8, dim = columns = x_stride) come with x_scales [tokens].  columns, a
+ * multiple of 16, is at most 2^17 - 16, whatever the codes (-128 among them).
+ * workspace: device memory of st_int8_matmul_workspace_bytes(x_type, tokens,
+ * columns) bytes (may be 0), 16-byte aligned.
+ * ------------------------------------------------------------------------- */
+#define ST_CODE_I8 6
+int64_t st_int8_columns(int64_t dim);
+int st_int8_quantize(const void* x, int x_type, int64_t rows, int64_t dim, int64_t x_stride,
+                     int8_t* codes, float* scales, void* stream);
+int64_t st_int8_matmul_workspace_bytes(int x_type, int64_t tokens, int64_t columns);
+int st_int8_matmul(const int8_t* codes, const float* scales, int64_t rows, int64_t columns,
+                   const void* x, int x_type, const float* x_scales, int64_t tokens,
+                   int64_t dim, int64_t x_stride, const float* bias, void* y, int y_type,
+                   void* workspace, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

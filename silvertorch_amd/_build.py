@@ -42,11 +42,12 @@ HIP_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 
-# (source, ST_SEARCH_K) pairs: the search kernel is compiled once per K.
+# (source, definition) pairs: the search kernel is compiled once per K, the
+# layer norm's once per type.
 LIB_SOURCES = [
     "st_runtime.hip",
     "bloom_search.hip",
-    *[("bloom_search_k.hip", k) for k in range(1, 11)],
+    *[("bloom_search_k.hip", f"ST_SEARCH_K={k}") for k in range(1, 11)],
     "bloom_build.hip",
     "bloom_compact.hip",
     "bloom_partial.hip",
@@ -57,13 +58,17 @@ LIB_SOURCES = [
     "int4_matvec.hip",
     "target_logprobs.hip",
     "cluster_route.hip",
+    "dropout.hip",
+    "layer_norm.hip",
+    *[("layer_norm_t.hip", f"ST_NORM_TYPE={t}") for t in range(3)],
+    "int8_matmul.hip",
     "search_plan.cpp",
     "host_pool.cpp",
     "expression_parser.cpp",
 ]
 
 # torch.ops.st.* registration
-EXT_SOURCES = ["torch_ops.cpp", "torch_head_ops.cpp"]
+EXT_SOURCES = ["torch_ops.cpp", "torch_head_ops.cpp", "torch_tower_ops.cpp"]
 
 
 def _run(cmd: list[str]) -> None:
@@ -89,8 +94,8 @@ INCREMENTAL = False  # set by `python -m silvertorch_amd._build --incremental`
 
 
 def _compile_lib_object(spec) -> Path:
-    src, k = spec if isinstance(spec, tuple) else (spec, None)
-    obj = OBJ / (src + ("" if k is None else f".k{k}") + ".o")
+    src, definition = spec if isinstance(spec, tuple) else (spec, None)
+    obj = OBJ / (src + ("" if definition is None else "." + definition.replace("=", "")) + ".o")
     path = CSRC / src
     if INCREMENTAL and not _stale(obj, path):
         return obj
@@ -98,8 +103,8 @@ def _compile_lib_object(spec) -> Path:
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-c"]
     else:
         cmd = [HIPCC, *HIP_FLAGS, "-c"]
-    if k is not None:
-        cmd.append(f"-DST_SEARCH_K={k}")
+    if definition is not None:
+        cmd.append(f"-D{definition}")
     cmd += [str(path), "-o", str(obj)]
     _run(cmd)
     return obj

@@ -65,6 +65,19 @@ SIGNATURES = {
                                           ctypes.c_double, *[_vp] * 8]),
     "st_target_logprobs_backward": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
                                                    ctypes.c_double, *[_vp] * 9]),
+    "st_dropout": (ctypes.c_int, [_vp, ctypes.c_int, _i64, ctypes.c_double, _vp, _vp, _vp, _vp]),
+    "st_layer_norm": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, _vp, ctypes.c_int, _i64, _vp, _vp, ctypes.c_int,
+                                     ctypes.c_double, ctypes.c_double, *[_vp] * 6]),
+    "st_layer_norm_workspace_bytes": (_i64, [_i64, _i64]),
+    "st_layer_norm_backward": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, ctypes.c_int, _i64, _i64, _i64, _vp,
+                                              ctypes.c_int, _vp, ctypes.c_double, *[_vp] * 7]),
+    "st_layer_norm_int8": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, _vp, _vp, ctypes.c_int, ctypes.c_double,
+                                          _vp, _vp, _vp]),
+    "st_int8_columns": (_i64, [_i64]),
+    "st_int8_quantize": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "st_int8_matmul_workspace_bytes": (_i64, [ctypes.c_int, _i64, _i64]),
+    "st_int8_matmul": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp, ctypes.c_int, _vp, _i64, _i64, _i64, _vp, _vp,
+                                      ctypes.c_int, _vp, _vp]),
     "st_cluster_route_workspace_bytes": (_i64, [_i64, _i64]),
     "st_cluster_route": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, _i64, *[_vp] * 10]),
     "st_cluster_route_backward": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, _i64, *[_vp] * 9]),

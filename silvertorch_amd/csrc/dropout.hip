@@ -1,0 +1,75 @@
+// Dropout, forward and backward: y = x times 2^16 / (2^16 - dropped) where the
+// element stays, 0 elsewhere (dropout_bits.hpp says which stay).  The backward
+// pass is the same kernel on the result's gradient: it draws the numbers again,
+// and no mask is stored.  No reference operator.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "dropout_bits.hpp"
+#include "score_ops.hpp"
+#include "st_errors.hpp"
+
+namespace st {
+
+DropoutArgs dropout_args(double p, const int64_t* state, int64_t* used) {
+  ST_CHECK(p >= 0.0 && p <= 1.0, "p must be in [0, 1], got ", p);
+  DropoutArgs d{};
+  d.dropped = static_cast<int>(__builtin_rint(p * kDropoutOne));
+  d.times = d.dropped < kDropoutOne ? static_cast<float>(static_cast<double>(kDropoutOne) / (kDropoutOne - d.dropped)) : 0.0f;
+  d.state = state;
+  d.used = used;
+  return d;
+}
+
+namespace {
+
+// A thread takes a block of eight elements at a time.
+template <int DT>
+__global__ __launch_bounds__(256) void dropout_kernel(const void* x, void* y, int64_t elements, DropoutArgs d) {
+  const DropoutKey key = dropout_key(d.state);
+  if (d.used && blockIdx.x == 0 && threadIdx.x < 2) d.used[threadIdx.x] = d.state[threadIdx.x];
+  const int64_t whole = elements / 8, blocks = (elements + 7) / 8;
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < blocks;
+       at += static_cast<int64_t>(gridDim.x) * 256) {
+    if (at < whole) {
+      const Raw8<DT> raw = load_raw8<DT>(x, at * 8);
+      const uint32_t keeps = dropout_keeps(key, static_cast<uint64_t>(at) * 8, d.dropped);
+      float v[8];
+      unpack8<DT>(raw, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (keeps >> i) & 1 ? v[i] * d.times : 0.0f;
+      store8<DT>(y, at * 8, v);
+    } else {
+      const uint32_t keeps = dropout_keeps(key, static_cast<uint64_t>(at) * 8, d.dropped);
+      for (int64_t e = at * 8; e < elements; ++e)
+        store_score<DT>(y, e, (keeps >> (e & 7)) & 1 ? load_score<DT>(x, e) * d.times : 0.0f);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace st
+
+extern "C" int st_dropout(const void* x, int type, int64_t elements, double p, const int64_t* state, void* y,
+                          int64_t* used, void* stream) {
+  using namespace st;
+  return guarded([&] {
+    ST_CHECK(type == ST_SCORE_F32 || type == ST_SCORE_F16 || type == ST_SCORE_BF16,
+             "x must be float32, float16 or bfloat16");
+    ST_CHECK(elements >= 0, "negative number of elements");
+    const DropoutArgs d = dropout_args(p, state, used);
+    if (elements == 0) return;
+    ST_CHECK(x && y && state, "null device pointer");
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((elements + 2047) / 2048, 1 << 22));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (type == ST_SCORE_F32)
+      hipLaunchKernelGGL((dropout_kernel<ST_SCORE_F32>), dim3(grid), dim3(256), 0, s, x, y, elements, d);
+    else if (type == ST_SCORE_F16)
+      hipLaunchKernelGGL((dropout_kernel<ST_SCORE_F16>), dim3(grid), dim3(256), 0, s, x, y, elements, d);
+    else
+      hipLaunchKernelGGL((dropout_kernel<ST_SCORE_BF16>), dim3(grid), dim3(256), 0, s, x, y, elements, d);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) throw Error(ST_ERR_HIP, cat("dropout_kernel launch failed: ", hipGetErrorString(e)));
+  });
+}

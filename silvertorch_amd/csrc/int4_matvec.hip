@@ -65,16 +65,6 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, float v, int type)
     store_score<ST_SCORE_BF16>(p, i, v);
 }
 
-// Lane groups of 16 and registers transposed: register i of lane group g
-// becomes register g of lane group i.
-__device__ __forceinline__ u32x4 transpose4(u32x4 d) {
-  auto s02 = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false);
-  auto s13 = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
-  auto s01 = __builtin_amdgcn_permlane16_swap(s02[0], s13[0], false, false);
-  auto s23 = __builtin_amdgcn_permlane16_swap(s02[1], s13[1], false, false);
-  return u32x4{s01[0], s01[1], s23[0], s23[1]};
-}
-
 // Register i: the value of lane group i, in all four groups.
 __device__ __forceinline__ u32x4 broadcast4(uint32_t v) {
   auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);

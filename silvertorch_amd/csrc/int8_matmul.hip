@@ -1,0 +1,403 @@
+// Products of a table held in 8 bits with vectors held in 8 bits, and both's
+// making.  No reference operator.
+//
+//   y[m, n] = x_scale[m] scale[n] sum_k x[m, k] code[n, k] + bias[n]
+// The sum is exact (32-bit integers); each row of the table (a document, an
+// output channel) and each vector (a query, a token) has one scale.  Rows are
+// whole blocks of 16 columns; vectors that come as floats are taken to 8 bits
+// on the way (code_ops.hpp), zeros past their last column.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "code_ops.hpp"
+#include "layer_norm_kernel.hpp"
+#include "score_ops.hpp"
+#include "st_errors.hpp"
+
+namespace st {
+int cu_count();
+void launch_codes(const void* x, int x_type, int64_t rows, int64_t dim, int64_t x_stride, int8_t* codes, int64_t columns,
+                  float* scales, hipStream_t s);
+
+namespace {
+
+constexpr int64_t kMaxColumns = (1 << 17) - 16;  // 2^14 a product: sums stay below 2^31
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kFusedBytes = 32 * 1024;  // of LDS for vectors that the product itself takes to 8 bits
+
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
+struct MatmulArgs {
+  const int8_t* codes;
+  const float* scales;
+  const float* bias;  // or null
+  const void* x;      // codes [tokens, columns], or what they are made of
+  const float* x_scales;
+  void* y;
+  int64_t rows, tokens, x_stride;
+  int dim, columns;
+  int x_type, y_type;
+};
+
+__device__ __forceinline__ void store_typed(void* y, int64_t at, float v, int type) {
+  if (type == ST_SCORE_F32)
+    store_score<ST_SCORE_F32>(y, at, v);
+  else if (type == ST_SCORE_F16)
+    store_score<ST_SCORE_F16>(y, at, v);
+  else
+    store_score<ST_SCORE_BF16>(y, at, v);
+}
+
+template <int DT>
+__device__ __forceinline__ void load_eight(const void* row, int col, int dim, float v[8]) {
+  if (col + 8 <= dim) {
+    unpack8<DT>(load_raw8<DT>(row, col), v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < dim ? load_score<DT>(row, col + i) : 0.0f;
+  }
+}
+
+// One vector to 8 bits by one wave: codes to LDS in the order of the matrix
+// instruction's operand (1 KB for 64 columns of 16 vectors: 256 bytes for each
+// 16 columns), zeros up to `padded`; returns the scale.
+template <int DT>
+__device__ __forceinline__ float codes_to_lds(const void* row, int dim, int padded, uint8_t* to, int step_bytes) {
+  const int lane = threadIdx.x % 64;
+  float most = 0.0f, odd = 0.0f, v[8];
+  for (int col = lane * 8; col < dim; col += 512) {
+    load_eight<DT>(row, col, dim, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      most = fmaxf(most, fabsf(v[i]));
+      odd = fmaf(v[i], 0.0f, odd);
+    }
+  }
+  const CodeScale c = code_scale(wave_max(odd != odd ? __builtin_inff() : most));
+  for (int col = lane * 8; col < padded; col += 512) {
+    load_eight<DT>(row, col, dim, v);
+    *reinterpret_cast<uint64_t*>(to + (col >> 6) * step_bytes + ((col >> 4) & 3) * 256 + (col & 15)) = codes8(v, c);
+  }
+  return c.scale;
+}
+
+// Few vectors: HBM bounds it, the table's bytes or the results'.  The table goes
+// from memory to registers, 16 rows x 64 columns an instruction, vectors (16 T at
+// a time) beside it.  R blocks of 16 rows a wave, J steps of 64 columns at a
+// time; SPLIT waves share a row's columns.
+template <int T, int R, int J, bool SPLIT, bool FUSED>
+__global__ __launch_bounds__(kThreads) void few_kernel(MatmulArgs a) {
+  extern __shared__ uint8_t lds[];
+  __shared__ float fused_scales[FUSED ? 16 * T : 1];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, q = lane / 16, c = lane % 16;
+  const int64_t token0 = static_cast<int64_t>(blockIdx.y) * (16 * T);
+  const int tokens = static_cast<int>(min(a.tokens - token0, static_cast<int64_t>(16 * T)));
+  const int steps = (a.columns + 64 * J - 1) / (64 * J);  // of J times 64 columns
+  constexpr int kStepBytes = T * 1024;                    // of LDS, for 64 columns
+
+  if constexpr (FUSED) {
+    for (int m = wave; m < tokens; m += kWaves) {
+      uint8_t* to = lds + (m / 16) * 1024 + (m % 16) * 16;
+      const int64_t row = (token0 + m) * a.x_stride;
+      float scale;
+      if (a.x_type == ST_SCORE_F32)
+        scale = codes_to_lds<ST_SCORE_F32>(static_cast<const float*>(a.x) + row, a.dim, steps * J * 64, to, kStepBytes);
+      else if (a.x_type == ST_SCORE_F16)
+        scale = codes_to_lds<ST_SCORE_F16>(static_cast<const uint16_t*>(a.x) + row, a.dim, steps * J * 64, to, kStepBytes);
+      else
+        scale = codes_to_lds<ST_SCORE_BF16>(static_cast<const uint16_t*>(a.x) + row, a.dim, steps * J * 64, to, kStepBytes);
+      if (lane == 0) fused_scales[m] = scale;
+    }
+    __syncthreads();
+  }
+
+  struct Step {
+    i32x4 w[R][J], x[FUSED ? 1 : T][FUSED ? 1 : J];
+  };
+  const int64_t tiles = (a.rows + 16 * R - 1) / (16 * R);
+  const int64_t tile_step = static_cast<int64_t>(gridDim.x) * (SPLIT ? 1 : kWaves);
+  int64_t tile = SPLIT ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kWaves + wave;
+  const int first_step = SPLIT ? wave : 0;
+  constexpr int kStepStep = SPLIT ? kWaves : 1;
+
+  auto load = [&](int64_t at, int step, Step& s) {
+    const int64_t row0 = at * (16 * R);
+    const int8_t* table = a.codes + row0 * a.columns;
+    const int last = static_cast<int>(min(a.rows - row0, static_cast<int64_t>(16 * R))) - 1;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int k = (step * J + j) * 64 + q * 16;
+      const bool in = k < a.columns;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        // rows past the last and columns past theirs read others; the former's
+        // results are not stored, the latter meet zeros of x
+        const int64_t offset = static_cast<int64_t>(min(16 * r + c, last)) * a.columns + (in ? k : 0);
+        s.w[r][j] = *reinterpret_cast<const i32x4*>(table + offset);
+      }
+      if constexpr (!FUSED) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          const int64_t m = token0 + min(16 * t + c, tokens - 1);
+          i32x4 v = *reinterpret_cast<const i32x4*>(static_cast<const int8_t*>(a.x) + m * a.columns + (in ? k : 0));
+          if (!in) v = i32x4{0, 0, 0, 0};
+          s.x[t][j] = v;
+        }
+      }
+    }
+  };
+
+  i32x4 acc[T][R];
+  auto clear = [&] {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int r = 0; r < R; ++r) acc[t][r] = i32x4{0, 0, 0, 0};
+  };
+  auto compute = [&](int step, const Step& s) {
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        i32x4 x;
+        if constexpr (FUSED)
+          x = *reinterpret_cast<const i32x4*>(lds + (step * J + j) * kStepBytes + t * 1024 + lane * 16);
+        else
+          x = s.x[t][j];
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[t][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, s.w[r][j], acc[t][r], 0, 0, 0);
+      }
+  };
+  auto x_scale = [&](int m) { return FUSED ? fused_scales[m] : a.x_scales[token0 + m]; };
+  auto put = [&](int m, int64_t n, int sum, float scale, float bias) {
+    store_typed(a.y, (token0 + m) * a.rows + n, fmaf(static_cast<float>(sum) * x_scale(m), scale, bias), a.y_type);
+  };
+
+  if (tile >= tiles) return;
+  Step next;
+  load(tile, min(first_step, steps - 1), next);
+  for (; tile < tiles; tile += tile_step) {
+    clear();
+    for (int step = first_step; step < steps; step += kStepStep) {
+      const Step now = next;
+      const bool more = step + kStepStep < steps;
+      // past the end: this step again, not used
+      const int64_t to = more || tile + tile_step >= tiles ? tile : tile + tile_step;
+      load(to, more ? step + kStepStep : min(first_step, steps - 1), next);
+      compute(step, now);
+    }
+    const int64_t row0 = tile * (16 * R);
+    if constexpr (SPLIT) {
+      static_assert(R == 1 && kWaves == 4, "");
+      i32x4* sums = reinterpret_cast<i32x4*>(lds + (FUSED ? steps * J * kStepBytes : 0));
+#pragma unroll
+      for (int t = 0; t < T; ++t) sums[(wave * T + t) * 64 + lane] = acc[t][0];
+      __syncthreads();
+      // element i of each lane by wave i
+      const int64_t n = row0 + c;
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) sum += reinterpret_cast<const int*>(sums)[((w * T + t) * 64 + lane) * 4 + wave];
+        const int m = 16 * t + 4 * q + wave;
+        if (m < tokens && n < a.rows) put(m, n, sum, a.scales[n], a.bias ? a.bias[n] : 0.0f);
+      }
+      __syncthreads();
+    } else {
+      static_assert(R == 4, "");
+      const int64_t n = row0 + lane;
+      const bool live = n < a.rows;
+      const float scale = live ? a.scales[n] : 0.0f, bias = live && a.bias ? a.bias[n] : 0.0f;
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (16 * t + i >= tokens) continue;
+          // one vector's results of 64 rows side by side
+          const u32x4 v = transpose4(u32x4{static_cast<uint32_t>(acc[t][0][i]), static_cast<uint32_t>(acc[t][1][i]),
+                                           static_cast<uint32_t>(acc[t][2][i]), static_cast<uint32_t>(acc[t][3][i])});
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int m = 16 * t + 4 * j + i;
+            if (m < tokens && live) put(m, n, static_cast<int>(v[j]), scale, bias);
+          }
+        }
+    }
+  }
+}
+
+template <int T, bool FUSED>
+void launch_few(const MatmulArgs& a, hipStream_t s) {
+  const int64_t passes = (a.tokens + 16 * T - 1) / (16 * T);
+  const bool split = a.columns >= 1024 && (a.rows + 63) / 64 < 8 * cu_count();
+  const int64_t groups = split ? (a.rows + 15) / 16 : (a.rows + 64 * kWaves - 1) / (64 * kWaves);
+  const int64_t grid = std::min<int64_t>(groups, 4 * cu_count());
+  const int padded = split ? (a.columns + 255) / 256 * 256 : (a.columns + 63) / 64 * 64;
+  const size_t fused = FUSED ? static_cast<size_t>(padded) * 16 * T : 0;
+  for (int64_t at = 0; at < passes; at += 32768) {
+    MatmulArgs part = a;
+    const int64_t first = at * 16 * T;
+    part.tokens = std::min<int64_t>(a.tokens - first, static_cast<int64_t>(32768) * 16 * T);
+    const int x_bytes = a.x_type == ST_CODE_I8 ? 1 : a.x_type == ST_SCORE_F32 ? 4 : 2;
+    const int y_bytes = a.y_type == ST_SCORE_F32 ? 4 : 2;
+    part.x = static_cast<const char*>(a.x) + first * a.x_stride * x_bytes;
+    if (a.x_scales) part.x_scales = a.x_scales + first;
+    part.y = static_cast<char*>(a.y) + first * a.rows * y_bytes;
+    const dim3 blocks(static_cast<unsigned>(grid), static_cast<unsigned>((part.tokens + 16 * T - 1) / (16 * T)));
+    if (split)
+      hipLaunchKernelGGL((few_kernel<T, 1, 4, true, FUSED>), blocks, dim3(kThreads), fused + T * kThreads * 16, s, part);
+    else
+      hipLaunchKernelGGL((few_kernel<T, 4, 1, false, FUSED>), blocks, dim3(kThreads), fused, s, part);
+  }
+}
+
+// Whether the product takes the vectors to 8 bits itself: each workgroup does it
+// again, so they have to be few; a launch of its own (about 4 us) does it
+// otherwise.
+bool is_fused(int x_type, int64_t tokens, int64_t columns) {
+  return x_type != ST_CODE_I8 && tokens <= 16 && (columns + 255) / 256 * 256 * 16 <= kFusedBytes;
+}
+
+void check_codes(int64_t rows, int64_t columns) {
+  ST_CHECK(rows >= 0, "negative number of rows");
+  ST_CHECK(columns >= 16 && columns % 16 == 0 && columns <= kMaxColumns,
+           "rows of codes are whole blocks of 16 columns, at most ", kMaxColumns, ", got ", columns);
+}
+
+void check_type(int type, const char* what) {
+  ST_CHECK(type == ST_SCORE_F32 || type == ST_SCORE_F16 || type == ST_SCORE_BF16, what,
+           " must be float32, float16 or bfloat16");
+}
+
+void check_launch(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) throw Error(ST_ERR_HIP, cat(what, " launch failed: ", hipGetErrorString(e)));
+}
+
+// Vectors of more columns than the norm's kernels hold: a workgroup each, which
+// reads them twice.
+template <int DT>
+__global__ __launch_bounds__(1024) void long_codes_kernel(const void* x, int64_t x_stride, int dim, int columns, int8_t* codes,
+                                                          float* scales) {
+  __shared__ float room[16];
+  const char* row = static_cast<const char*>(x) + blockIdx.x * x_stride * kScoreBytes<DT>;
+  float most = 0.0f, odd = 0.0f, v[8];
+  for (int col = threadIdx.x * 8; col < dim; col += 8192) {
+    load_eight<DT>(row, col, dim, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      most = fmaxf(most, fabsf(v[i]));
+      odd = fmaf(v[i], 0.0f, odd);
+    }
+  }
+  most = wave_max(odd != odd ? __builtin_inff() : most);
+  if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 16; ++w) most = fmaxf(most, room[w]);
+  const CodeScale c = code_scale(most);
+  if (threadIdx.x == 0) scales[blockIdx.x] = c.scale;
+  for (int col = threadIdx.x * 8; col < columns; col += 8192) {
+    load_eight<DT>(row, col, dim, v);
+    *reinterpret_cast<uint64_t*>(codes + static_cast<int64_t>(blockIdx.x) * columns + col) = codes8(v, c);
+  }
+}
+
+void quantize(const void* x, int x_type, int64_t rows, int64_t dim, int64_t x_stride, int8_t* codes, float* scales,
+              hipStream_t s) {
+  const int64_t columns = (dim + 15) / 16 * 16;
+  if (dim <= kMaxNormColumns) {
+    launch_codes(x, x_type, rows, dim, x_stride, codes, columns, scales, s);
+    return;
+  }
+  const int64_t most = 1 << 21;  // rows a launch: 2^31 threads
+  for (int64_t at = 0; at < rows; at += most) {
+    const dim3 grid(static_cast<unsigned>(std::min(most, rows - at)));
+    const char* from = static_cast<const char*>(x) + at * x_stride * (x_type == ST_SCORE_F32 ? 4 : 2);
+    int8_t* to = codes + at * columns;
+    const int d = static_cast<int>(dim), c = static_cast<int>(columns);
+    if (x_type == ST_SCORE_F32)
+      hipLaunchKernelGGL((long_codes_kernel<ST_SCORE_F32>), grid, dim3(1024), 0, s, from, x_stride, d, c, to, scales + at);
+    else if (x_type == ST_SCORE_F16)
+      hipLaunchKernelGGL((long_codes_kernel<ST_SCORE_F16>), grid, dim3(1024), 0, s, from, x_stride, d, c, to, scales + at);
+    else
+      hipLaunchKernelGGL((long_codes_kernel<ST_SCORE_BF16>), grid, dim3(1024), 0, s, from, x_stride, d, c, to, scales + at);
+    check_launch("long_codes_kernel");
+  }
+}
+
+int64_t codes_bytes(int64_t tokens, int64_t columns) { return (tokens * columns + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace st
+
+extern "C" int64_t st_int8_columns(int64_t dim) { return (dim + 15) / 16 * 16; }
+
+extern "C" int st_int8_quantize(const void* x, int x_type, int64_t rows, int64_t dim, int64_t x_stride, int8_t* codes,
+                                float* scales, void* stream) {
+  using namespace st;
+  return guarded([&] {
+    check_type(x_type, "x");
+    ST_CHECK(dim >= 1, "a row has at least one column, got ", dim);
+    check_codes(rows, st_int8_columns(dim));
+    if (rows == 0) return;
+    ST_CHECK(x && codes && scales, "null device pointer");
+    ST_CHECK(reinterpret_cast<uintptr_t>(codes) % 16 == 0, "codes must be 16-byte aligned");
+    quantize(x, x_type, rows, dim, x_stride, codes, scales, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int64_t st_int8_matmul_workspace_bytes(int x_type, int64_t tokens, int64_t columns) {
+  using namespace st;
+  if (x_type == ST_CODE_I8 || tokens <= 0 || columns <= 0 || is_fused(x_type, tokens, columns)) return 0;
+  return codes_bytes(tokens, columns) + tokens * static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int st_int8_matmul(const int8_t* codes, const float* scales, int64_t rows, int64_t columns, const void* x,
+                              int x_type, const float* x_scales, int64_t tokens, int64_t dim, int64_t x_stride,
+                              const float* bias, void* y, int y_type, void* workspace, void* stream) {
+  using namespace st;
+  return guarded([&] {
+    if (x_type != ST_CODE_I8) check_type(x_type, "x");
+    check_type(y_type, "the result");
+    check_codes(rows, columns);
+    ST_CHECK(tokens >= 0, "negative number of vectors");
+    ST_CHECK(dim >= 1 && st_int8_columns(dim) == columns, "the table's rows have ", columns, " columns, vectors of ", dim,
+             " take ", st_int8_columns(dim));
+    ST_CHECK(x_type != ST_CODE_I8 || (dim == columns && x_stride == columns), "vectors of codes are whole rows side by side");
+    if (rows == 0 || tokens == 0) return;
+    ST_CHECK(codes && scales && x && y, "null device pointer");
+    ST_CHECK(reinterpret_cast<uintptr_t>(codes) % 16 == 0, "the table must be 16-byte aligned");
+    ST_CHECK(x_type != ST_CODE_I8 || (x_scales && reinterpret_cast<uintptr_t>(x) % 16 == 0),
+             "vectors of codes come with scales and must be 16-byte aligned");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    MatmulArgs a{codes, scales, bias, x, x_scales, y, rows, tokens, x_stride, static_cast<int>(dim), static_cast<int>(columns),
+                 x_type, y_type};
+    if (is_fused(x_type, tokens, columns)) {
+      launch_few<1, true>(a, s);
+      check_launch("few_kernel");
+      return;
+    }
+    if (x_type != ST_CODE_I8) {
+      ST_CHECK(workspace, "null device pointer");
+      int8_t* made = static_cast<int8_t*>(workspace);
+      float* made_scales = reinterpret_cast<float*>(made + codes_bytes(tokens, columns));
+      quantize(x, x_type, tokens, dim, x_stride, made, made_scales, s);
+      a.x = made;
+      a.x_scales = made_scales;
+      a.x_type = ST_CODE_I8;
+      a.x_stride = columns;
+      a.dim = static_cast<int>(columns);
+    }
+    if (tokens <= 16)
+      launch_few<1, false>(a, s);
+    else if (tokens <= 32)
+      launch_few<2, false>(a, s);
+    else
+      launch_few<4, false>(a, s);
+    check_launch("few_kernel");
+  });
+}

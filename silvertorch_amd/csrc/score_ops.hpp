@@ -194,6 +194,16 @@ __device__ __forceinline__ float wave_sum(float x) {
   return (r0 + r1) + (r2 + r3);
 }
 
+// Lane groups of 16 and registers transposed: register i of lane group g
+// becomes register g of lane group i.
+__device__ __forceinline__ u32x4 transpose4(u32x4 d) {
+  auto s02 = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false);
+  auto s13 = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
+  auto s01 = __builtin_amdgcn_permlane16_swap(s02[0], s13[0], false, false);
+  auto s23 = __builtin_amdgcn_permlane16_swap(s02[1], s13[1], false, false);
+  return u32x4{s01[0], s01[1], s23[0], s23[1]};
+}
+
 // The statistics of all lanes' scores, in every lane.
 __device__ __forceinline__ SoftStats soft_wave_join(SoftStats a, float c) {
   a = soft_rebase(a, wave_max(a.m), c);

@@ -5,50 +5,29 @@
 // CPU tensors are copied to the current GPU and the results back.  The two
 // operators a model is trained through carry their gradients (Autograd key);
 // the 4-bit ones refuse to be differentiated.
-#include <ATen/core/dispatch/Dispatcher.h>
-#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
-#include "torch_common.hpp"
+#include "torch_autograd.hpp"
 
 namespace {
 
 using at::Tensor;
+using st_torch::bytes_or_null;
 using st_torch::check_st;
 using st_torch::current_stream;
+using st_torch::data_or_null;
+using st_torch::find_op;
 using st_torch::gpu_for_cpu_call;
+using st_torch::gradient;
+using st_torch::if_defined;
+using st_torch::moved;
+using st_torch::OnceDifferentiable;
+using st_torch::OptTensor;
+using st_torch::refuse_tangents;
+using st_torch::score_type;
+using st_torch::with_adjacent_columns;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-using OptTensor = std::optional<Tensor>;
-
-int score_type(at::ScalarType t, const char* what) {
-  switch (t) {
-    case at::kFloat:
-      return ST_SCORE_F32;
-    case at::kHalf:
-      return ST_SCORE_F16;
-    case at::kBFloat16:
-      return ST_SCORE_BF16;
-    default:
-      TORCH_CHECK(false, what, " must be float32, float16 or bfloat16, got ", t);
-  }
-}
-
-template <typename T>
-T* data_or_null(const Tensor& t) {
-  return t.defined() && t.numel() ? t.data_ptr<T>() : nullptr;
-}
-
-void* bytes_or_null(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
-
-// None of these operators has a forward-mode derivative: an input that carries
-// a tangent is refused, where the result would otherwise come without one.
-void refuse_tangents(std::initializer_list<const Tensor*> inputs, const char* op) {
-  for (const Tensor* t : inputs)
-    TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), op, " has no forward-mode derivative");
-}
-
-Tensor moved(const OptTensor& t, at::Device d) { return t.has_value() && t->defined() ? t->to(d) : Tensor(); }
 
 // ------------------------------------------ 4-bit tables
 
@@ -140,11 +119,6 @@ Tensor int4_matvec_cpu(const Tensor& packed, const Tensor& scales, const Tensor&
 
 // The 4-bit operators have no gradients.  Their results say so when one is
 // asked for, where they would otherwise count as constants.
-template <typename Op>
-auto find_op(const char* name) {
-  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Op>();
-}
-
 using QuantizeOp = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, int64_t, bool);
 using MatvecOp = Tensor(const Tensor&, const Tensor&, const Tensor&, int64_t, const OptTensor&,
                         std::optional<at::ScalarType>);
@@ -197,9 +171,6 @@ Tensor int4_matvec_autograd(const Tensor& packed, const Tensor& scales, const Te
     return matvec_below(packed, scales, x, group_size, zeros, out_dtype);
   return MatvecFunction::apply(packed, scales, x, group_size, zeros, out_dtype);
 }
-
-// A score row is readable with any row stride; columns have to be adjacent.
-Tensor with_adjacent_columns(const Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
 
 // ------------------------------------------ log-probabilities of given documents
 
@@ -281,29 +252,10 @@ LogprobsOut logprobs_any(const Tensor& logits, const Tensor& targets, int64_t to
   return o;
 }
 
-// A gradient as the kernels take it: float32, contiguous, on the device.
-Tensor gradient(const Tensor& g, at::Device d) {
-  return g.defined() ? g.to(d, at::kFloat).contiguous() : g;
-}
-
-// A gradient with a graph over it (backward with create_graph): it depends on
-// the scores and on the outputs' gradients, and refuses to be differentiated
-// where it would otherwise count as a constant.
-struct OnceDifferentiable : torch::autograd::Function<OnceDifferentiable> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& grad, const Tensor& /*logits*/, const OptTensor& /*g0*/,
-                        const OptTensor& /*g1*/, const OptTensor& /*g2*/, const OptTensor& /*g3*/, std::string op) {
-    ctx->saved_data["op"] = std::move(op);
-    return grad;
-  }
-  static variable_list backward(AutogradContext* ctx, variable_list /*grads*/) {
-    TORCH_CHECK(false, "the gradient of ", ctx->saved_data["op"].toStringRef(), " cannot be differentiated again");
-  }
-};
-
 Tensor differentiable_once(const Tensor& grad, const Tensor& logits, const variable_list& outer, const char* op) {
   if (!at::GradMode::is_enabled()) return grad;
-  auto given = [&](size_t i) { return outer[i].defined() ? OptTensor(outer[i]) : OptTensor(); };
-  return OnceDifferentiable::apply(grad, logits, given(0), given(1), given(2), given(4), std::string(op));
+  return OnceDifferentiable::apply(grad, logits, if_defined(outer[0]), if_defined(outer[1]), if_defined(outer[2]),
+                                   if_defined(outer[4]), std::string(op));
 }
 
 struct LogprobsFunction : torch::autograd::Function<LogprobsFunction> {
