@@ -29,7 +29,6 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kFusedBytes = 32 * 1024;  // of LDS for vectors that the product itself takes to 8 bits
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
-typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
 struct MatmulArgs {
   const int8_t* codes;
@@ -256,233 +255,271 @@ void launch_few(const MatmulArgs& a, hipStream_t s) {
   }
 }
 
-// `count` numbers from p[n] on, 0 for the others of eight.
-__device__ __forceinline__ void load_some(const float* p, int64_t n, int count, float v[8]) {
-  if (count == 8) {
-    unpack8<ST_SCORE_F32>(load_raw8<ST_SCORE_F32>(p, n), v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < count ? p[n + i] : 0.0f;
-  }
-}
-
-// Many vectors: the matrix units bound it.  A workgroup of four waves takes a
-// tile of 2 WT vectors x 2 WR rows, each wave a quarter of it, in 32x32x32 blocks
-// whose sums stay in registers: for WT = WR = 128 all 512 of a lane's registers,
-// 256 of them sums, so that a byte from LDS takes part in 128 products.
+// Many vectors: the matrix units bound it, and the power they may draw: 16x16x64
+// blocks run at 4,840 TOP/s on zeros and 4,070 on random codes (registers alone),
+// 32x32x32 ones at 3,290 and 2,600.  A workgroup of NT x NR waves takes tiles of
+// NT WT vectors x NR WR rows, each wave its part of them, with the sums in registers.
 //
-// Steps of 64 columns; a tile of 128 columns (whole cache lines) is two.  While a
-// step's products run, the operands of the next step go from LDS to registers,
-// half of the next tile from registers to LDS (vectors one step ahead of rows,
-// so that every step moves as much), and half of the tile after it from memory to
-// registers.  Two buffers in LDS and a barrier a step.
+// Columns go in parts of 128 (whole cache lines), two steps of 64 each, a step in
+// groups of one block of vectors by all of rows.  While a group's products run, the
+// vectors of the group `kAhead` on, or the rows of the next step, go from LDS to
+// registers.  Two buffers in LDS; one barrier a part, where its last vectors are in
+// registers: from there on the next part is read, and the one after it goes from
+// memory straight to LDS.  The stream of parts does not end with a tile: the next
+// tile's first two are under way while a tile's results are stored.
 //
-// In LDS a row is 8 chunks of 16 bytes, chunk c at place c ^ f(row): eight lanes
-// that read or write at once meet all banks.  Rows of the table enter the matrix
-// instruction so that a lane's 16 sums of a block are neighbours in a result's
-// row.
-template <int YT, int WT, int WR>
-__global__ __launch_bounds__(kThreads, WT* WR > 64 * 64 ? 1 : 2) void many_kernel(MatmulArgs a) {
-  constexpr int BT = WT / 32, BR = WR / 32;           // blocks of a wave
-  constexpr int kTokens = 2 * WT, kRows = 2 * WR;     // of the workgroup
-  constexpr int LT = kTokens / 32, LR = kRows / 32;   // loads of 16 bytes a lane and tile
+// In LDS a row is 8 chunks of 16 bytes, chunk c at place c ^ f(row): the 16 lanes
+// that read or write at once (two rows, whose addresses differ by half of the 64
+// banks, or one chunk of 16 rows) meet all banks.
+template <int YT, int WT, int WR, int NT, int NR>
+__global__ __launch_bounds__(64 * NT * NR, WT* WR < 64 * 128 ? 2 : 1) void many_kernel(MatmulArgs a) {
+  constexpr int BT = WT / 16, BR = WR / 16;                           // blocks of a wave
+  constexpr int kAhead = BT >= 8 ? 3 : 2;                             // groups between a block's read and its use
+  constexpr int kTokens = NT * WT, kRows = NR * WR;                   // of the workgroup
+  constexpr int kAtOnce = 8 * NT * NR;                                // rows that its waves bring with one load each
+  constexpr int LT = kTokens / kAtOnce, LR = kRows / kAtOnce, kMoves = LT + LR;
   constexpr int kX = kTokens * 128, kW = kRows * 128;  // bytes of a buffer
+  constexpr int kGroups = 2 * BT, kTurn = kGroups - kAhead;  // the group ahead of which the barrier is
+  static_assert(kAtOnce % 16 == 0 && BT % 4 == 0, "");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int half = lane / 32, in_block = lane % 32;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int q = lane / 16, in_block = lane % 16;
+  const int parts = (a.columns + 127) / 128;
 
   // Tiles in an order that shares the last-level caches: an eighth of them to
   // each of the 8 dies (workgroups go round them), there 8 tiles of vectors by
   // one of rows after another.
   const int64_t tiles_t = (a.tokens + kTokens - 1) / kTokens, tiles_r = (a.rows + kRows - 1) / kRows;
-  int64_t id = blockIdx.x;
   const int64_t all = tiles_t * tiles_r;
-  {
+  struct Tile {
+    int64_t token0, row0;
+  };
+  auto tile_of = [&](int64_t id) {
     const int64_t each = all / 8, more = all % 8, die = id % 8;
     id = die * each + min(die, more) + id / 8;
-  }
-  const int64_t in_group = 8 * tiles_r, group = id / in_group;
-  const int64_t height = min(static_cast<int64_t>(8), tiles_t - group * 8);
-  const int64_t within = id - group * in_group;
-  const int64_t token0 = (group * 8 + within % height) * kTokens, row0 = within / height * kRows;
-
-  const int8_t* x = static_cast<const int8_t*>(a.x) + token0 * a.columns;
-  const int8_t* w = a.codes + row0 * a.columns;
-  const int tiles = (a.columns + 127) / 128;
-
-  // This lane's chunk of the rows that it brings, by number: row 32 i + 8 wave +
-  // lane / 8.  Rows past the last read it again; their sums are not stored.
-  const int chunk = lane % 8, first_row = wave * 8 + lane / 8;
-  uint32_t x_from[LT], w_from[LR];
-  const int last_token = static_cast<int>(min(a.tokens - token0, static_cast<int64_t>(kTokens))) - 1;
-  const int last_row = static_cast<int>(min(a.rows - row0, static_cast<int64_t>(kRows))) - 1;
-#pragma unroll
-  for (int i = 0; i < LT; ++i) x_from[i] = static_cast<uint32_t>(min(32 * i + first_row, last_token)) * a.columns + chunk * 16;
-#pragma unroll
-  for (int i = 0; i < LR; ++i) w_from[i] = static_cast<uint32_t>(min(32 * i + first_row, last_row)) * a.columns + chunk * 16;
-  const auto place_x = [](int row) { return row & 7; };
-  const auto place_w = [](int row) { return (row & 3) | ((row >> 2) & 4); };
-  const uint32_t x_to = first_row * 128 + ((chunk ^ place_x(first_row)) * 16);
-  // f of rows 32 apart is the same
-  const uint32_t w_to = 2 * kX + first_row * 128 + ((chunk ^ place_w(first_row)) * 16);
-
-  // Columns past the last: vectors are 0 there, the table's row is read at the
-  // tile's start.
-  auto past = [&](int tile) { return tile * 128 + chunk * 16 >= a.columns; };
-  i32x4 gx[LT], gw[LR];
-  auto load_x = [&](int tile, int i) {
-    tile = min(tile, tiles - 1);
-    const i32x4 v = *reinterpret_cast<const i32x4*>(x + static_cast<int64_t>(tile) * 128 + (x_from[i] - (past(tile) ? chunk * 16 : 0)));
-    gx[i] = v;
-  };
-  auto load_w = [&](int tile, int i) {
-    tile = min(tile, tiles - 1);
-    gw[i] = *reinterpret_cast<const i32x4*>(w + static_cast<int64_t>(tile) * 128 + (w_from[i] - (past(tile) ? chunk * 16 : 0)));
-  };
-  auto write_x = [&](int tile, int i) {
-    const i32x4 v = past(tile) ? i32x4{0, 0, 0, 0} : gx[i];
-    *reinterpret_cast<i32x4*>(lds + (tile & 1) * kX + x_to + i * 4096) = v;
-  };
-  auto write_w = [&](int tile, int i) { *reinterpret_cast<i32x4*>(lds + (tile & 1) * kW + w_to + i * 4096) = gw[i]; };
-
-  // Operands: x of a step and sub-step, block b; the table's rows in the order
-  // that leaves 16 neighbours to a lane: row 8 a + 4 h + b of a block is its row 16 h
-  // + 4 a + b.
-  const int x_row = (wave / 2) * WT + in_block;
-  const int w_in = ((in_block >> 2) & 1) * 16 + (in_block >> 3) * 4 + (in_block & 3);
-  const int w_row = (wave % 2) * WR + w_in;
-  i32x4 fx[2][BT][2], fw[2][BR][2];
-  auto read_x = [&](int set, int tile, int step, int b, int j) {
-    const int c = step * 4 + j * 2 + half;
-    fx[set][b][j] = *reinterpret_cast<const i32x4*>(lds + (tile & 1) * kX + x_row * 128 + ((c ^ place_x(x_row)) * 16) + b * 4096);
-  };
-  auto read_w = [&](int set, int tile, int step, int b, int j) {
-    const int c = step * 4 + j * 2 + half;
-    fw[set][b][j] = *reinterpret_cast<const i32x4*>(lds + 2 * kX + (tile & 1) * kW + w_row * 128 + ((c ^ place_w(w_row)) * 16) + b * 4096);
+    const int64_t in_group = 8 * tiles_r, group = id / in_group, within = id - group * in_group;
+    const int64_t height = min(static_cast<int64_t>(8), tiles_t - group * 8);
+    return Tile{(group * 8 + within % height) * kTokens, within / height * kRows};
   };
 
-  i32x16 acc[BT][BR];
+  // What a wave brings: 8 rows a load, lane l the chunk that belongs at place l % 8
+  // of row kAtOnce i + 8 wave + l / 8 (f of rows 16 apart is the same).  Rows past the
+  // last read it again; their sums are not stored.
+  const auto place = [](int row) { return (row >> 1) & 7; };
+  const int first_row = wave * 8 + lane / 8, chunk = (lane % 8) ^ place(first_row);
+  // Columns past the last are read at the part's start, and of the vectors zeros put
+  // in their places once they are there (`settle`).
+  const int past = (parts - 1) * 128 + chunk * 16 >= a.columns ? chunk * 16 : 0;
+  int64_t bring_id = blockIdx.x;  // the tile and the part that are brought next, and its buffer
+  int bring_part = 0, bring_buffer = 0;
+  const int8_t *x, *w;
+  uint32_t from[kMoves];
+  auto aim = [&] {
+    const Tile tile = tile_of(bring_id);
+    x = static_cast<const int8_t*>(a.x) + tile.token0 * a.columns;
+    w = a.codes + tile.row0 * a.columns;
+    const int last_token = static_cast<int>(min(a.tokens - tile.token0, static_cast<int64_t>(kTokens))) - 1;
+    const int last_row = static_cast<int>(min(a.rows - tile.row0, static_cast<int64_t>(kRows))) - 1;
 #pragma unroll
-  for (int t = 0; t < BT; ++t)
+    for (int i = 0; i < kMoves; ++i) {
+      const int row = i < LT ? min(kAtOnce * i + first_row, last_token) : min(kAtOnce * (i - LT) + first_row, last_row);
+      from[i] = static_cast<uint32_t>(row) * a.columns + chunk * 16;
+    }
+  };
+  auto place_of = [&](int buffer, int i) {
+    return lds + (i < LT ? buffer * kX + i * kAtOnce * 128 : 2 * kX + buffer * kW + (i - LT) * kAtOnce * 128) + wave * 1024;
+  };
+  auto bring = [&](int i) {
+    const int8_t* base = (i < LT ? x : w) + static_cast<int64_t>(bring_part) * 128;
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void*)(base + (from[i] - (bring_part == parts - 1 ? past : 0))),
+        (__attribute__((address_space(3))) void*)place_of(bring_buffer, i), 16, 0, 0);
+  };
+  auto brought = [&] {
+    bring_buffer ^= 1;
+    if (++bring_part < parts) return;
+    bring_part = 0;
+    bring_id += gridDim.x;
+    if (bring_id < all) aim();
+  };
+  // Waits for what this wave brought, and for its reads of LDS.
+  auto settle = [&](int part, int buffer) {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+    if (part == parts - 1 && past != 0) {
 #pragma unroll
-    for (int r = 0; r < BR; ++r)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[t][r][i] = 0;
-
+      for (int i = 0; i < LT; ++i) *reinterpret_cast<i32x4*>(place_of(buffer, i) + lane * 16) = i32x4{0, 0, 0, 0};
+    }
+  };
   auto barrier = [] {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   };
 
-#pragma unroll
-  for (int i = 0; i < LT; ++i) load_x(0, i);
-#pragma unroll
-  for (int i = 0; i < LR; ++i) load_w(0, i);
-#pragma unroll
-  for (int i = 0; i < LT; ++i) write_x(0, i);
-#pragma unroll
-  for (int i = 0; i < LR; ++i) write_w(0, i);
-#pragma unroll
-  for (int i = 0; i < LT; ++i) load_x(1, i);
-#pragma unroll
-  for (int i = 0; i < LR; ++i) load_w(1, i);
-#pragma unroll
-  for (int i = 0; i < LT; ++i) write_x(1, i);
-#pragma unroll
-  for (int i = 0; i < LT; ++i) load_x(2, i);
-  barrier();
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-#pragma unroll
-    for (int b = 0; b < BR; ++b) read_w(0, 0, 0, b, j);
-#pragma unroll
-    for (int b = 0; b < BT; ++b) read_x(0, 0, 0, b, j);
-  }
-
-  // One step: products of set `set`; meanwhile operands of (tile, step) into the
-  // other set, what `move(i)` brings to LDS and from memory.
-  auto run = [&](int set, int tile, int step, auto move, int moves) {
-    constexpr int kProducts = 2 * BT * BR, kReads = 2 * (BT + BR);
-#pragma unroll
-    for (int p = 0; p < kProducts; ++p) {
-      const int j = p / (BT * BR), t = p % (BT * BR) / BR, r = p % BR;
-      acc[t][r] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[set][r][j], fx[set][t][j], acc[t][r], 0, 0, 0);
-#pragma unroll
-      for (int k = p * kReads / kProducts; k < (p + 1) * kReads / kProducts; ++k) {
-        const int jj = k / (BT + BR), b = k % (BT + BR);
-        if (b < BR)
-          read_w(set ^ 1, tile, step, b, jj);
-        else
-          read_x(set ^ 1, tile, step, b - BR, jj);
-      }
-#pragma unroll
-      for (int k = p * moves / kProducts; k < (p + 1) * moves / kProducts; ++k) move(k);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+  // Operands: block t of the vectors, into a ring of four; block r of the rows, into
+  // the step's set.
+  const int x_row = (wave / NR) * WT + in_block, w_row = (wave % NR) * WR + in_block;
+  i32x4 fx[4], fw[2][BR];
+  auto read_x = [&](int buffer, int step, int t) {
+    fx[t & 3] = *reinterpret_cast<const i32x4*>(lds + buffer * kX + x_row * 128 + (((step * 4 + q) ^ place(x_row)) * 16) + t * 2048);
   };
-#pragma unroll 1
-  for (int tile = 0; tile < tiles; ++tile) {
-    run(0, tile, 1, [&](int i) { write_w(tile + 1, i); load_w(tile + 2, i); }, LR);
-    barrier();
-    run(1, tile + 1, 0, [&](int i) { write_x(tile + 2, i); load_x(tile + 3, i); }, LT);
-    barrier();
-  }
+  auto read_w = [&](int buffer, int step, int r) {
+    fw[step][r] = *reinterpret_cast<const i32x4*>(lds + 2 * kX + buffer * kW + w_row * 128 + (((step * 4 + q) ^ place(w_row)) * 16) + r * 2048);
+  };
 
-  // a lane's sums: of vector in_block of each block, 16 rows side by side
-  const int64_t n0 = row0 + (wave % 2) * WR + half * 16, m0 = token0 + (wave / 2) * WT + in_block;
+  i32x4 acc[BT][BR];
+  auto clear = [&] {
 #pragma unroll
-  for (int r = 0; r < BR; ++r) {
+    for (int t = 0; t < BT; ++t)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int64_t n = n0 + r * 32 + e * 8;
-      const int count = static_cast<int>(max(static_cast<int64_t>(0), min(a.rows - n, static_cast<int64_t>(8))));
-      float scale[8], bias[8];
-      load_some(a.scales, n, count, scale);
-      load_some(a.bias, n, a.bias ? count : 0, bias);
+      for (int r = 0; r < BR; ++r) acc[t][r] = i32x4{0, 0, 0, 0};
+  };
+
+  // Results by way of LDS, each wave in a part of its own: 16 vectors x WR rows of
+  // sums, chunk c of 4 at place c ^ vector, so that a store writes whole lines of a
+  // result's row (16 bytes here and there, straight from the sums: 620 us for 16,384 x
+  // 4,096 x 8,192 where this took 509).
+  constexpr int kEach = YT == ST_SCORE_F32 ? 4 : 8;  // results a lane stores at once, 16 bytes
+  constexpr int kLanes = WR / kEach;                 // of a vector's
+  i32x4* sums = reinterpret_cast<i32x4*>(lds + 2 * (kX + kW)) + wave * 4 * WR;
+  auto store = [&](const Tile& tile) {
+    const int64_t n = tile.row0 + (wave % NR) * WR + lane % kLanes * kEach;
+    const int count = static_cast<int>(max(static_cast<int64_t>(0), min(a.rows - n, static_cast<int64_t>(kEach))));
+    float scale[kEach], bias[kEach];
 #pragma unroll
-      for (int t = 0; t < BT; ++t) {
-        const int64_t m = m0 + t * 32;
-        if (m < a.tokens) {
-          const float x_scale = a.x_scales[m];
-          float v[8];
+    for (int i = 0; i < kEach; ++i) {
+      scale[i] = i < count ? a.scales[n + i] : 0.0f;
+      bias[i] = a.bias && i < count ? a.bias[n + i] : 0.0f;
+    }
+    constexpr int kStores = 16 * kLanes / 64;  // of a block of vectors
+    float x_scales[BT][kStores];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = fmaf(static_cast<float>(acc[t][r][8 * e + i]) * x_scale, scale[i], bias[i]);
-          if (count == 8) {
-            store8<YT>(a.y, m * a.rows + n, v);
+    for (int t = 0; t < BT; ++t)
+#pragma unroll
+      for (int g = 0; g < kStores; ++g)
+        x_scales[t][g] = a.x_scales[min(tile.token0 + (wave / NR) * WT + t * 16 + g * (64 / kLanes) + lane / kLanes, a.tokens - 1)];
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): no load is left for the loop to wait for
+#pragma unroll
+    for (int t = 0; t < BT; ++t) {
+#pragma unroll
+      for (int r = 0; r < BR; ++r) sums[in_block * (WR / 4) + ((r * 4 + q) ^ in_block)] = acc[t][r];
+      // LDS serves a wave in order; only the compiler must keep it
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+#pragma unroll
+      for (int g = 0; g < kStores; ++g) {
+        const int in = g * (64 / kLanes) + lane / kLanes;
+        const int64_t m = tile.token0 + (wave / NR) * WT + t * 16 + in;
+        if (m >= a.tokens || count == 0) continue;
+        const float x_scale = x_scales[t][g];
+        float v[8];
+#pragma unroll
+        for (int c = 0; c < kEach / 4; ++c) {
+          const i32x4 sum = sums[in * (WR / 4) + ((lane % kLanes * (kEach / 4) + c) ^ in)];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[4 * c + i] = fmaf(static_cast<float>(sum[i]) * x_scale, scale[4 * c + i], bias[4 * c + i]);
+        }
+        const int64_t at = m * a.rows + n;
+        if (count == kEach) {
+          if constexpr (YT == ST_SCORE_F32) {
+            *reinterpret_cast<u32x4_by4*>(static_cast<float*>(a.y) + at) =
+                u32x4_by4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
           } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (i < count) store_score<YT>(a.y, m * a.rows + n + i, v[i]);
+            store8<YT>(a.y, at, v);
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kEach; ++i)
+            if (i < count) store_score<YT>(a.y, at + i, v[i]);
         }
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
     }
+  };
+
+  aim();
+#pragma unroll
+  for (int i = 0; i < kMoves; ++i) bring(i);
+  brought();
+  settle(0, 0);
+  barrier();
+  if (bring_id < all) {
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) bring(i);
+    brought();
+  }
+#pragma unroll
+  for (int r = 0; r < BR; ++r) read_w(0, 0, r);
+#pragma unroll
+  for (int t = 0; t < kAhead; ++t) read_x(0, 0, t);
+  clear();
+  int64_t id = blockIdx.x;
+  int part = 0, buffer = 0;
+#pragma unroll 1
+  while (true) {
+    const int next_part = part + 1 < parts ? part + 1 : 0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int step = g / BT, t = g % BT;
+      if (g == kTurn) {
+        settle(next_part, buffer ^ 1);
+        barrier();
+      }
+      // reads: the block kAhead groups on; the next step's rows
+      if (g < kTurn)
+        read_x(buffer, (g + kAhead) / BT, (g + kAhead) % BT);
+      else
+        read_x(buffer ^ 1, 0, g - kTurn);
+      if (step == 0) {
+#pragma unroll
+        for (int r = t * BR / BT; r < (t + 1) * BR / BT; ++r) read_w(buffer, 1, r);
+      } else if (g == kTurn) {
+#pragma unroll
+        for (int r = 0; r < BR; ++r) read_w(buffer ^ 1, 0, r);
+      }
+#pragma unroll
+      for (int r = 0; r < BR; ++r)
+        acc[t][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[step][r], fx[t & 3], acc[t][r], 0, 0, 0);
+      // the part after the next, into this one's buffer
+      if (g >= kTurn && bring_id < all) {
+#pragma unroll
+        for (int i = (g - kTurn) * kMoves / kAhead; i < (g - kTurn + 1) * kMoves / kAhead; ++i) bring(i);
+        if (g == kGroups - 1) brought();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    buffer ^= 1;
+    part = next_part;
+    if (part != 0) continue;
+    store(tile_of(id));
+    id += gridDim.x;
+    if (id >= all) break;
+    clear();
   }
 }
 
-template <int YT, int WT, int WR>
+template <int YT, int WT, int WR, int NT, int NR>
 void launch_many_as(const MatmulArgs& a, hipStream_t s) {
-  constexpr int kLds = 4 * (WT + WR) * 128;
-  const auto kernel = many_kernel<YT, WT, WR>;
+  constexpr int kLds = 2 * (NT * WT + NR * WR) * 128 + NT * NR * 64 * WR;
+  const auto kernel = many_kernel<YT, WT, WR, NT, NR>;
   static std::once_flag once;
   std::call_once(once, [&] {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (e != hipSuccess) throw Error(ST_ERR_HIP, cat("hipFuncSetAttribute failed: ", hipGetErrorString(e)));
   });
-  const int64_t tiles = ((a.tokens + 2 * WT - 1) / (2 * WT)) * ((a.rows + 2 * WR - 1) / (2 * WR));
-  ST_CHECK(tiles < (1ll << 24), "the product has too many tiles");
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(kThreads), kLds, s, a);
+  const int64_t tiles = ((a.tokens + NT * WT - 1) / (NT * WT)) * ((a.rows + NR * WR - 1) / (NR * WR));
+  const int64_t grid = std::min<int64_t>(tiles, cu_count() * (160 * 1024 / kLds));
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * NT * NR), kLds, s, a);
 }
 
-template <int WT, int WR>
+template <int WT, int WR, int NT, int NR>
 void launch_many(const MatmulArgs& a, hipStream_t s) {
   if (a.y_type == ST_SCORE_F32)
-    launch_many_as<ST_SCORE_F32, WT, WR>(a, s);
+    launch_many_as<ST_SCORE_F32, WT, WR, NT, NR>(a, s);
   else if (a.y_type == ST_SCORE_F16)
-    launch_many_as<ST_SCORE_F16, WT, WR>(a, s);
+    launch_many_as<ST_SCORE_F16, WT, WR, NT, NR>(a, s);
   else
-    launch_many_as<ST_SCORE_BF16, WT, WR>(a, s);
+    launch_many_as<ST_SCORE_BF16, WT, WR, NT, NR>(a, s);
 }
 
 // Whether the product takes the vectors to 8 bits itself: each workgroup does it
@@ -625,9 +662,9 @@ extern "C" int st_int8_matmul(const int8_t* codes, const float* scales, int64_t 
     }
     if (tokens > 64 && columns >= 256) {
       if (((tokens + 255) / 256) * ((rows + 255) / 256) >= cu_count() / 2)
-        launch_many<128, 128>(a, s);
+        launch_many<128, 64, 2, 4>(a, s);
       else
-        launch_many<64, 64>(a, s);
+        launch_many<64, 64, 2, 2>(a, s);
       check_launch("many_kernel");
       return;
     }
