@@ -667,13 +667,14 @@ int st_layer_norm_int8(const void* x, int x_type, int64_t rows, int64_t dim, int
  * (ST_CODE_I8, dim = columns = x_stride) come with x_scales [tokens].  columns, a
  * multiple of 16, is at most 2^17 - 16, whatever the codes (-128 among them).
  * workspace: device memory of st_int8_matmul_workspace_bytes(x_type, tokens,
- * columns) bytes (may be 0), 16-byte aligned.
+ * rows, columns) bytes (may be 0), 16-byte aligned.
  * ------------------------------------------------------------------------- */
 #define ST_CODE_I8 6
 int64_t st_int8_columns(int64_t dim);
 int st_int8_quantize(const void* x, int x_type, int64_t rows, int64_t dim, int64_t x_stride,
                      int8_t* codes, float* scales, void* stream);
-int64_t st_int8_matmul_workspace_bytes(int x_type, int64_t tokens, int64_t columns);
+int64_t st_int8_matmul_workspace_bytes(int x_type, int64_t tokens, int64_t rows,
+                                       int64_t columns);
 int st_int8_matmul(const int8_t* codes, const float* scales, int64_t rows, int64_t columns,
                    const void* x, int x_type, const float* x_scales, int64_t tokens,
                    int64_t dim, int64_t x_stride, const float* bias, void* y, int y_type,

@@ -75,7 +75,7 @@ SIGNATURES = {
                                           _vp, _vp, _vp]),
     "st_int8_columns": (_i64, [_i64]),
     "st_int8_quantize": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, _i64, _vp, _vp, _vp]),
-    "st_int8_matmul_workspace_bytes": (_i64, [ctypes.c_int, _i64, _i64]),
+    "st_int8_matmul_workspace_bytes": (_i64, [ctypes.c_int, _i64, _i64, _i64]),
     "st_int8_matmul": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp, ctypes.c_int, _vp, _i64, _i64, _i64, _vp, _vp,
                                       ctypes.c_int, _vp, _vp]),
     "st_cluster_route_workspace_bytes": (_i64, [_i64, _i64]),

@@ -26,9 +26,11 @@ namespace {
 constexpr int64_t kMaxColumns = (1 << 17) - 16;  // 2^14 a product: sums stay below 2^31
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kFusedBytes = 32 * 1024;  // of LDS for vectors that the product itself takes to 8 bits
+constexpr int kFewTokens = 4, kFewColumns = 2048;  // of few_kernel
+constexpr int64_t kFewBytes = 32 << 20;              // of its table
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct MatmulArgs {
   const int8_t* codes;
@@ -65,7 +67,7 @@ __device__ __forceinline__ void load_eight(const void* row, int col, int dim, fl
 // instruction's operand (1 KB for 64 columns of 16 vectors: 256 bytes for each
 // 16 columns), zeros up to `padded`; returns the scale.
 template <int DT>
-__device__ __forceinline__ float codes_to_lds(const void* row, int dim, int padded, uint8_t* to, int step_bytes) {
+__device__ __forceinline__ float codes_to_lds(const void* row, int dim, int padded, uint8_t* to) {
   const int lane = threadIdx.x % 64;
   float most = 0.0f, odd = 0.0f, v[8];
   for (int col = lane * 8; col < dim; col += 512) {
@@ -79,180 +81,124 @@ __device__ __forceinline__ float codes_to_lds(const void* row, int dim, int padd
   const CodeScale c = code_scale(wave_max(odd != odd ? __builtin_inff() : most));
   for (int col = lane * 8; col < padded; col += 512) {
     load_eight<DT>(row, col, dim, v);
-    *reinterpret_cast<uint64_t*>(to + (col >> 6) * step_bytes + ((col >> 4) & 3) * 256 + (col & 15)) = codes8(v, c);
+    *reinterpret_cast<uint64_t*>(to + (col >> 6) * 1024 + ((col >> 4) & 3) * 256 + (col & 15)) = codes8(v, c);
   }
   return c.scale;
 }
 
-// Few vectors: HBM bounds it, the table's bytes or the results'.  The table goes
-// from memory to registers, 16 rows x 64 columns an instruction, vectors (16 T at
-// a time) beside it.  R blocks of 16 rows a wave, J steps of 64 columns at a
-// time; SPLIT waves share a row's columns.
-template <int T, int R, int J, bool SPLIT, bool FUSED>
+// One to four vectors of floats against a table of a few megabytes, where a launch
+// counts: every workgroup takes the vectors to 8 bits itself, into LDS, while its
+// first rows are on their way.  R blocks of 16 rows a wave, J steps of 64 columns at a
+// time, straight from memory to registers; with SPLIT four waves share a row's
+// columns.
+template <int R, int J, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void few_kernel(MatmulArgs a) {
-  extern __shared__ uint8_t lds[];
-  __shared__ float fused_scales[FUSED ? 16 * T : 1];
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ float x_scales[kFewTokens];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, q = lane / 16, c = lane % 16;
-  const int64_t token0 = static_cast<int64_t>(blockIdx.y) * (16 * T);
-  const int tokens = static_cast<int>(min(a.tokens - token0, static_cast<int64_t>(16 * T)));
+  const int tokens = static_cast<int>(a.tokens);
   const int steps = (a.columns + 64 * J - 1) / (64 * J);  // of J times 64 columns
-  constexpr int kStepBytes = T * 1024;                    // of LDS, for 64 columns
 
-  if constexpr (FUSED) {
-    for (int m = wave; m < tokens; m += kWaves) {
-      uint8_t* to = lds + (m / 16) * 1024 + (m % 16) * 16;
-      const int64_t row = (token0 + m) * a.x_stride;
-      float scale;
-      if (a.x_type == ST_SCORE_F32)
-        scale = codes_to_lds<ST_SCORE_F32>(static_cast<const float*>(a.x) + row, a.dim, steps * J * 64, to, kStepBytes);
-      else if (a.x_type == ST_SCORE_F16)
-        scale = codes_to_lds<ST_SCORE_F16>(static_cast<const uint16_t*>(a.x) + row, a.dim, steps * J * 64, to, kStepBytes);
-      else
-        scale = codes_to_lds<ST_SCORE_BF16>(static_cast<const uint16_t*>(a.x) + row, a.dim, steps * J * 64, to, kStepBytes);
-      if (lane == 0) fused_scales[m] = scale;
-    }
-    __syncthreads();
-  }
-
-  struct Step {
-    i32x4 w[R][J], x[FUSED ? 1 : T][FUSED ? 1 : J];
-  };
   const int64_t tiles = (a.rows + 16 * R - 1) / (16 * R);
   const int64_t tile_step = static_cast<int64_t>(gridDim.x) * (SPLIT ? 1 : kWaves);
   int64_t tile = SPLIT ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kWaves + wave;
   const int first_step = SPLIT ? wave : 0;
   constexpr int kStepStep = SPLIT ? kWaves : 1;
-
+  struct Step {
+    i32x4 w[R][J];
+  };
   auto load = [&](int64_t at, int step, Step& s) {
+    at = min(at, tiles - 1);
     const int64_t row0 = at * (16 * R);
     const int8_t* table = a.codes + row0 * a.columns;
     const int last = static_cast<int>(min(a.rows - row0, static_cast<int64_t>(16 * R))) - 1;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int k = (step * J + j) * 64 + q * 16;
-      const bool in = k < a.columns;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
+      for (int r = 0; r < R; ++r)
         // rows past the last and columns past theirs read others; the former's
         // results are not stored, the latter meet zeros of x
-        const int64_t offset = static_cast<int64_t>(min(16 * r + c, last)) * a.columns + (in ? k : 0);
-        s.w[r][j] = *reinterpret_cast<const i32x4*>(table + offset);
-      }
-      if constexpr (!FUSED) {
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-          const int64_t m = token0 + min(16 * t + c, tokens - 1);
-          i32x4 v = *reinterpret_cast<const i32x4*>(static_cast<const int8_t*>(a.x) + m * a.columns + (in ? k : 0));
-          if (!in) v = i32x4{0, 0, 0, 0};
-          s.x[t][j] = v;
-        }
-      }
+        s.w[r][j] = *reinterpret_cast<const i32x4*>(table + static_cast<int64_t>(min(16 * r + c, last)) * a.columns + (k < a.columns ? k : 0));
     }
   };
-
-  i32x4 acc[T][R];
-  auto clear = [&] {
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-      for (int r = 0; r < R; ++r) acc[t][r] = i32x4{0, 0, 0, 0};
-  };
-  auto compute = [&](int step, const Step& s) {
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        i32x4 x;
-        if constexpr (FUSED)
-          x = *reinterpret_cast<const i32x4*>(lds + (step * J + j) * kStepBytes + t * 1024 + lane * 16);
-        else
-          x = s.x[t][j];
-#pragma unroll
-        for (int r = 0; r < R; ++r) acc[t][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, s.w[r][j], acc[t][r], 0, 0, 0);
-      }
-  };
-  auto x_scale = [&](int m) { return FUSED ? fused_scales[m] : a.x_scales[token0 + m]; };
-  auto put = [&](int m, int64_t n, int sum, float scale, float bias) {
-    store_typed(a.y, (token0 + m) * a.rows + n, fmaf(static_cast<float>(sum) * x_scale(m), scale, bias), a.y_type);
-  };
-
-  if (tile >= tiles) return;
   Step next;
   load(tile, min(first_step, steps - 1), next);
+
+  if (wave < tokens) {
+    const int64_t row = wave * a.x_stride;
+    float scale;
+    if (a.x_type == ST_SCORE_F32)
+      scale = codes_to_lds<ST_SCORE_F32>(static_cast<const float*>(a.x) + row, a.dim, steps * J * 64, lds + wave * 16);
+    else if (a.x_type == ST_SCORE_F16)
+      scale = codes_to_lds<ST_SCORE_F16>(static_cast<const uint16_t*>(a.x) + row, a.dim, steps * J * 64, lds + wave * 16);
+    else
+      scale = codes_to_lds<ST_SCORE_BF16>(static_cast<const uint16_t*>(a.x) + row, a.dim, steps * J * 64, lds + wave * 16);
+    if (lane == 0) x_scales[wave] = scale;
+  }
+  __syncthreads();
+
+  auto put = [&](int m, int64_t n, int sum) {
+    store_typed(a.y, m * a.rows + n, fmaf(static_cast<float>(sum) * x_scales[m], a.scales[n], a.bias ? a.bias[n] : 0.0f), a.y_type);
+  };
   for (; tile < tiles; tile += tile_step) {
-    clear();
+    i32x4 acc[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = i32x4{0, 0, 0, 0};
     for (int step = first_step; step < steps; step += kStepStep) {
       const Step now = next;
       const bool more = step + kStepStep < steps;
-      // past the end: this step again, not used
-      const int64_t to = more || tile + tile_step >= tiles ? tile : tile + tile_step;
-      load(to, more ? step + kStepStep : min(first_step, steps - 1), next);
-      compute(step, now);
+      load(more ? tile : tile + tile_step, more ? step + kStepStep : min(first_step, steps - 1), next);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        // vectors past the last hold whatever LDS does; their sums are not stored
+        const i32x4 x = *reinterpret_cast<const i32x4*>(lds + (step * J + j) * 1024 + lane * 16);
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, now.w[r][j], acc[r], 0, 0, 0);
+      }
     }
+    // vector m's sums lie in element m of the first 16 lanes
     const int64_t row0 = tile * (16 * R);
     if constexpr (SPLIT) {
-      static_assert(R == 1 && kWaves == 4, "");
-      i32x4* sums = reinterpret_cast<i32x4*>(lds + (FUSED ? steps * J * kStepBytes : 0));
-#pragma unroll
-      for (int t = 0; t < T; ++t) sums[(wave * T + t) * 64 + lane] = acc[t][0];
+      static_assert(R == 1 && kWaves == kFewTokens, "");
+      int* sums = reinterpret_cast<int*>(lds + steps * J * 1024);
+      if (q == 0) *reinterpret_cast<i32x4*>(sums + (wave * 16 + c) * 4) = acc[0];
       __syncthreads();
-      // element i of each lane by wave i
-      const int64_t n = row0 + c;
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
+      // vector `wave` by wave `wave`
+      if (q == 0 && wave < tokens && row0 + c < a.rows) {
         int sum = 0;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) sum += reinterpret_cast<const int*>(sums)[((w * T + t) * 64 + lane) * 4 + wave];
-        const int m = 16 * t + 4 * q + wave;
-        if (m < tokens && n < a.rows) put(m, n, sum, a.scales[n], a.bias ? a.bias[n] : 0.0f);
+        for (int w = 0; w < kWaves; ++w) sum += sums[(w * 16 + c) * 4 + wave];
+        put(wave, row0 + c, sum);
       }
       __syncthreads();
     } else {
       static_assert(R == 4, "");
       const int64_t n = row0 + lane;
-      const bool live = n < a.rows;
-      const float scale = live ? a.scales[n] : 0.0f, bias = live && a.bias ? a.bias[n] : 0.0f;
 #pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (16 * t + i >= tokens) continue;
-          // one vector's results of 64 rows side by side
-          const u32x4 v = transpose4(u32x4{static_cast<uint32_t>(acc[t][0][i]), static_cast<uint32_t>(acc[t][1][i]),
-                                           static_cast<uint32_t>(acc[t][2][i]), static_cast<uint32_t>(acc[t][3][i])});
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int m = 16 * t + 4 * j + i;
-            if (m < tokens && live) put(m, n, static_cast<int>(v[j]), scale, bias);
-          }
-        }
+      for (int i = 0; i < kFewTokens; ++i) {
+        if (i >= tokens) break;
+        // 64 rows side by side
+        const u32x4 v = transpose4(u32x4{static_cast<uint32_t>(acc[0][i]), static_cast<uint32_t>(acc[1][i]),
+                                         static_cast<uint32_t>(acc[2][i]), static_cast<uint32_t>(acc[3][i])});
+        if (n < a.rows) put(i, n, static_cast<int>(v[0]));
+      }
     }
   }
 }
 
-template <int T, bool FUSED>
+// Too few rows for as many waves as hide a load's latency: four share a row.
+bool few_split(const MatmulArgs& a) { return a.columns >= 1024 && (a.rows + 63) / 64 < 8 * cu_count(); }
+
 void launch_few(const MatmulArgs& a, hipStream_t s) {
-  const int64_t passes = (a.tokens + 16 * T - 1) / (16 * T);
-  const bool split = a.columns >= 1024 && (a.rows + 63) / 64 < 8 * cu_count();
+  const bool split = few_split(a);
   const int64_t groups = split ? (a.rows + 15) / 16 : (a.rows + 64 * kWaves - 1) / (64 * kWaves);
-  const int64_t grid = std::min<int64_t>(groups, 4 * cu_count());
-  const int padded = split ? (a.columns + 255) / 256 * 256 : (a.columns + 63) / 64 * 64;
-  const size_t fused = FUSED ? static_cast<size_t>(padded) * 16 * T : 0;
-  for (int64_t at = 0; at < passes; at += 32768) {
-    MatmulArgs part = a;
-    const int64_t first = at * 16 * T;
-    part.tokens = std::min<int64_t>(a.tokens - first, static_cast<int64_t>(32768) * 16 * T);
-    const int x_bytes = a.x_type == ST_CODE_I8 ? 1 : a.x_type == ST_SCORE_F32 ? 4 : 2;
-    const int y_bytes = a.y_type == ST_SCORE_F32 ? 4 : 2;
-    part.x = static_cast<const char*>(a.x) + first * a.x_stride * x_bytes;
-    if (a.x_scales) part.x_scales = a.x_scales + first;
-    part.y = static_cast<char*>(a.y) + first * a.rows * y_bytes;
-    const dim3 blocks(static_cast<unsigned>(grid), static_cast<unsigned>((part.tokens + 16 * T - 1) / (16 * T)));
-    if (split)
-      hipLaunchKernelGGL((few_kernel<T, 1, 4, true, FUSED>), blocks, dim3(kThreads), fused + T * kThreads * 16, s, part);
-    else
-      hipLaunchKernelGGL((few_kernel<T, 4, 1, false, FUSED>), blocks, dim3(kThreads), fused, s, part);
-  }
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(groups, 4 * cu_count())));
+  const size_t padded = split ? (a.columns + 255) / 256 * 256 : (a.columns + 63) / 64 * 64;
+  if (split)
+    hipLaunchKernelGGL((few_kernel<1, 4, true>), grid, dim3(kThreads), padded * 16 + kWaves * 256, s, a);
+  else
+    hipLaunchKernelGGL((few_kernel<4, 1, false>), grid, dim3(kThreads), padded * 16, s, a);
 }
 
 // Many vectors: the matrix units bound it, and the power they may draw: 16x16x64
@@ -280,7 +226,7 @@ __global__ __launch_bounds__(64 * NT * NR, WT* WR < 64 * 128 ? 2 : 1) void many_
   constexpr int LT = kTokens / kAtOnce, LR = kRows / kAtOnce, kMoves = LT + LR;
   constexpr int kX = kTokens * 128, kW = kRows * 128;  // bytes of a buffer
   constexpr int kGroups = 2 * BT, kTurn = kGroups - kAhead;  // the group ahead of which the barrier is
-  static_assert(kAtOnce % 16 == 0 && BT % 4 == 0, "");
+  static_assert(kAtOnce % 16 == 0 && kGroups % 4 == 0 && kGroups > kAhead, "");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int q = lane / 16, in_block = lane % 16;
@@ -289,17 +235,17 @@ __global__ __launch_bounds__(64 * NT * NR, WT* WR < 64 * 128 ? 2 : 1) void many_
   // Tiles in an order that shares the last-level caches: an eighth of them to
   // each of the 8 dies (workgroups go round them), there 8 tiles of vectors by
   // one of rows after another.
-  const int64_t tiles_t = (a.tokens + kTokens - 1) / kTokens, tiles_r = (a.rows + kRows - 1) / kRows;
-  const int64_t all = tiles_t * tiles_r;
+  const uint32_t tiles_t = static_cast<uint32_t>((a.tokens + kTokens - 1) / kTokens);
+  const uint32_t tiles_r = static_cast<uint32_t>((a.rows + kRows - 1) / kRows), all = tiles_t * tiles_r;
   struct Tile {
     int64_t token0, row0;
   };
-  auto tile_of = [&](int64_t id) {
-    const int64_t each = all / 8, more = all % 8, die = id % 8;
-    id = die * each + min(die, more) + id / 8;
-    const int64_t in_group = 8 * tiles_r, group = id / in_group, within = id - group * in_group;
-    const int64_t height = min(static_cast<int64_t>(8), tiles_t - group * 8);
-    return Tile{(group * 8 + within % height) * kTokens, within / height * kRows};
+  auto tile_of = [&](uint32_t id) {
+    const uint32_t die = id % 8;
+    id = die * (all / 8) + min(die, all % 8) + id / 8;
+    const uint32_t group = id / (8 * tiles_r), within = id - group * (8 * tiles_r);
+    const uint32_t height = min(8u, tiles_t - group * 8), column = within / height;
+    return Tile{static_cast<int64_t>(group * 8 + (within - column * height)) * kTokens, static_cast<int64_t>(column) * kRows};
   };
 
   // What a wave brings: 8 rows a load, lane l the chunk that belongs at place l % 8
@@ -310,7 +256,7 @@ __global__ __launch_bounds__(64 * NT * NR, WT* WR < 64 * 128 ? 2 : 1) void many_
   // Columns past the last are read at the part's start, and of the vectors zeros put
   // in their places once they are there (`settle`).
   const int past = (parts - 1) * 128 + chunk * 16 >= a.columns ? chunk * 16 : 0;
-  int64_t bring_id = blockIdx.x;  // the tile and the part that are brought next, and its buffer
+  uint32_t bring_id = blockIdx.x;  // the tile and the part that are brought next, and its buffer
   int bring_part = 0, bring_buffer = 0;
   const int8_t *x, *w;
   uint32_t from[kMoves];
@@ -342,9 +288,16 @@ __global__ __launch_bounds__(64 * NT * NR, WT* WR < 64 * 128 ? 2 : 1) void many_
     bring_id += gridDim.x;
     if (bring_id < all) aim();
   };
-  // Waits for what this wave brought, and for its reads of LDS.
-  auto settle = [&](int part, int buffer) {
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+  // Waits for what this wave brought, and for its reads of LDS; not for `stored`
+  // stores that it issued since.
+  auto settle = [&](int part, int buffer, int stored) {
+    constexpr int kFull = BT * (16 * (WR / (YT == ST_SCORE_F32 ? 4 : 8)) / 64);
+    if (stored == 0)
+      __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+    else if (stored == 1)
+      __builtin_amdgcn_s_waitcnt(0x0071);
+    else
+      __builtin_amdgcn_s_waitcnt(0x0070 | (kFull & 15) | ((kFull & 0x30) << 10));
     if (part == parts - 1 && past != 0) {
 #pragma unroll
       for (int i = 0; i < LT; ++i) *reinterpret_cast<i32x4*>(place_of(buffer, i) + lane * 16) = i32x4{0, 0, 0, 0};
@@ -361,7 +314,7 @@ __global__ __launch_bounds__(64 * NT * NR, WT* WR < 64 * 128 ? 2 : 1) void many_
   const int x_row = (wave / NR) * WT + in_block, w_row = (wave % NR) * WR + in_block;
   i32x4 fx[4], fw[2][BR];
   auto read_x = [&](int buffer, int step, int t) {
-    fx[t & 3] = *reinterpret_cast<const i32x4*>(lds + buffer * kX + x_row * 128 + (((step * 4 + q) ^ place(x_row)) * 16) + t * 2048);
+    fx[(step * BT + t) & 3] = *reinterpret_cast<const i32x4*>(lds + buffer * kX + x_row * 128 + (((step * 4 + q) ^ place(x_row)) * 16) + t * 2048);
   };
   auto read_w = [&](int buffer, int step, int r) {
     fw[step][r] = *reinterpret_cast<const i32x4*>(lds + 2 * kX + buffer * kW + w_row * 128 + (((step * 4 + q) ^ place(w_row)) * 16) + r * 2048);
@@ -376,50 +329,79 @@ __global__ __launch_bounds__(64 * NT * NR, WT* WR < 64 * 128 ? 2 : 1) void many_
   };
 
   // Results by way of LDS, each wave in a part of its own: 16 vectors x WR rows of
-  // sums, chunk c of 4 at place c ^ vector, so that a store writes whole lines of a
-  // result's row (16 bytes here and there, straight from the sums: 620 us for 16,384 x
-  // 4,096 x 8,192 where this took 509).
+  // sums times the vectors' scales, chunk c of 4 at place c ^ vector, so that a store
+  // writes whole lines of a result's row (16 bytes here and there, straight from the
+  // sums: 620 us for 16,384 x 4,096 x 8,192 where this took 509).
   constexpr int kEach = YT == ST_SCORE_F32 ? 4 : 8;  // results a lane stores at once, 16 bytes
   constexpr int kLanes = WR / kEach;                 // of a vector's
-  i32x4* sums = reinterpret_cast<i32x4*>(lds + 2 * (kX + kW)) + wave * 4 * WR;
-  auto store = [&](const Tile& tile) {
-    const int64_t n = tile.row0 + (wave % NR) * WR + lane % kLanes * kEach;
-    const int count = static_cast<int>(max(static_cast<int64_t>(0), min(a.rows - n, static_cast<int64_t>(kEach))));
-    float scale[kEach], bias[kEach];
+  constexpr int kStores = 16 * kLanes / 64;          // of a block of vectors
+  f32x4* sums = reinterpret_cast<f32x4*>(lds + 2 * (kX + kW)) + wave * 4 * WR;
+  float scale[kEach], bias[kEach], x_scale[BT];
+  Tile now;
+  int64_t n;
+  int count;
+  // What a tile's results need, a part ahead: a load after the next parts' would
+  // have to wait for them.
+  auto prepare = [&](uint32_t id) {
+    now = tile_of(id);
+    const int here = (wave % NR) * WR + lane % kLanes * kEach;
+    n = now.row0 + here;
+    count = max(0, min(static_cast<int>(min(a.rows - now.row0, static_cast<int64_t>(kRows))) - here, kEach));
+    const float* scales = a.scales + now.row0;
+    const float* biases = (a.bias ? a.bias : a.scales) + now.row0;
+    if (count == kEach) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      scale[i] = i < count ? a.scales[n + i] : 0.0f;
-      bias[i] = a.bias && i < count ? a.bias[n + i] : 0.0f;
+      for (int i = 0; i < kEach; i += 4) {
+        const u32x4_by4 s = *reinterpret_cast<const u32x4_by4*>(scales + here + i), b = *reinterpret_cast<const u32x4_by4*>(biases + here + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          scale[i + e] = __uint_as_float(s[e]);
+          bias[i + e] = __uint_as_float(b[e]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        scale[i] = i < count ? scales[here + i] : 0.0f;
+        bias[i] = i < count ? biases[here + i] : 0.0f;
+      }
     }
-    constexpr int kStores = 16 * kLanes / 64;  // of a block of vectors
-    float x_scales[BT][kStores];
+    const float* x_scales = a.x_scales + now.token0;
+    const int last_token = static_cast<int>(min(a.tokens - now.token0, static_cast<int64_t>(kTokens))) - 1;
 #pragma unroll
-    for (int t = 0; t < BT; ++t)
+    for (int t = 0; t < BT; ++t) x_scale[t] = x_scales[min((wave / NR) * WT + t * 16 + in_block, last_token)];
+  };
+  // Returns how many stores this wave has certainly issued, none or all of a full
+  // tile's or one.
+  auto store = [&] {
 #pragma unroll
-      for (int g = 0; g < kStores; ++g)
-        x_scales[t][g] = a.x_scales[min(tile.token0 + (wave / NR) * WT + t * 16 + g * (64 / kLanes) + lane / kLanes, a.tokens - 1)];
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): no load is left for the loop to wait for
+    for (int i = 0; i < kEach; ++i) bias[i] = a.bias ? bias[i] : 0.0f;
+    const int64_t m0 = now.token0 + (wave / NR) * WT;
+    const int tokens = static_cast<int>(max(static_cast<int64_t>(0), min(a.tokens - m0, static_cast<int64_t>(WT))));
 #pragma unroll
     for (int t = 0; t < BT; ++t) {
+      if (t * 16 >= tokens) break;
 #pragma unroll
-      for (int r = 0; r < BR; ++r) sums[in_block * (WR / 4) + ((r * 4 + q) ^ in_block)] = acc[t][r];
-      // LDS serves a wave in order; only the compiler must keep it
+      for (int r = 0; r < BR; ++r) {
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(acc[t][r][i]) * x_scale[t];
+        sums[in_block * (WR / 4) + ((r * 4 + q) ^ (in_block & (WR / 4 - 1)))] = v;
+      }
+      // LDS serves a wave in order; only the compiler must keep to it
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
 #pragma unroll
       for (int g = 0; g < kStores; ++g) {
         const int in = g * (64 / kLanes) + lane / kLanes;
-        const int64_t m = tile.token0 + (wave / NR) * WT + t * 16 + in;
-        if (m >= a.tokens || count == 0) continue;
-        const float x_scale = x_scales[t][g];
+        if (t * 16 + in >= tokens || count == 0) continue;
         float v[8];
 #pragma unroll
         for (int c = 0; c < kEach / 4; ++c) {
-          const i32x4 sum = sums[in * (WR / 4) + ((lane % kLanes * (kEach / 4) + c) ^ in)];
+          const f32x4 sum = sums[in * (WR / 4) + ((lane % kLanes * (kEach / 4) + c) ^ (in & (WR / 4 - 1)))];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[4 * c + i] = fmaf(static_cast<float>(sum[i]) * x_scale, scale[4 * c + i], bias[4 * c + i]);
+          for (int i = 0; i < 4; ++i) v[4 * c + i] = fmaf(sum[i], scale[4 * c + i], bias[4 * c + i]);
         }
-        const int64_t at = m * a.rows + n;
+        const int64_t at = (m0 + t * 16 + in) * a.rows + n;
         if (count == kEach) {
           if constexpr (YT == ST_SCORE_F32) {
             *reinterpret_cast<u32x4_by4*>(static_cast<float*>(a.y) + at) =
@@ -435,13 +417,15 @@ __global__ __launch_bounds__(64 * NT * NR, WT* WR < 64 * 128 ? 2 : 1) void many_
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
     }
+    if (now.row0 + (wave % NR) * WR + WR > a.rows || tokens == 0) return 0;
+    return tokens == WT ? BT * kStores : 1;
   };
 
   aim();
 #pragma unroll
   for (int i = 0; i < kMoves; ++i) bring(i);
   brought();
-  settle(0, 0);
+  settle(0, 0, 0);
   barrier();
   if (bring_id < all) {
 #pragma unroll
@@ -453,16 +437,18 @@ __global__ __launch_bounds__(64 * NT * NR, WT* WR < 64 * 128 ? 2 : 1) void many_
 #pragma unroll
   for (int t = 0; t < kAhead; ++t) read_x(0, 0, t);
   clear();
-  int64_t id = blockIdx.x;
-  int part = 0, buffer = 0;
+  uint32_t id = blockIdx.x;
+  int part = 0, buffer = 0, stored = 0;
 #pragma unroll 1
   while (true) {
     const int next_part = part + 1 < parts ? part + 1 : 0;
+    if (next_part == 0) prepare(id);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const int step = g / BT, t = g % BT;
       if (g == kTurn) {
-        settle(next_part, buffer ^ 1);
+        settle(next_part, buffer ^ 1, stored);
+        stored = 0;
         barrier();
       }
       // reads: the block kAhead groups on; the next step's rows
@@ -479,7 +465,7 @@ __global__ __launch_bounds__(64 * NT * NR, WT* WR < 64 * 128 ? 2 : 1) void many_
       }
 #pragma unroll
       for (int r = 0; r < BR; ++r)
-        acc[t][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[step][r], fx[t & 3], acc[t][r], 0, 0, 0);
+        acc[t][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[step][r], fx[g & 3], acc[t][r], 0, 0, 0);
       // the part after the next, into this one's buffer
       if (g >= kTurn && bring_id < all) {
 #pragma unroll
@@ -491,11 +477,145 @@ __global__ __launch_bounds__(64 * NT * NR, WT* WR < 64 * 128 ? 2 : 1) void many_
     buffer ^= 1;
     part = next_part;
     if (part != 0) continue;
-    store(tile_of(id));
+    stored = store();
     id += gridDim.x;
     if (id >= all) break;
     clear();
   }
+}
+
+// Parts of a wave in long_kernel: what 160 KB hold of eight waves'.
+constexpr int long_depth(int blocks) { return blocks == 1 ? 3 : 2; }
+
+// Few results of long rows, where tiles of all columns would leave most of the
+// chip idle: a workgroup takes 16 TB vectors x 32 rows, and its eight waves take
+// turns with the parts of 128 columns, each by itself, `kDepth` parts in LDS or on
+// the way to it; no barrier but the one before their sums are added.
+template <int YT, int TB>
+__global__ __launch_bounds__(512) void long_kernel(MatmulArgs a) {
+  constexpr int kSplit = 8, kRows = 32;
+  constexpr int LT = 2 * TB, kMoves = LT + kRows / 8;  // loads of 8 rows
+  constexpr int kBuffer = kMoves * 1024, kDepth = long_depth(TB);
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int q = lane / 16, in_block = lane % 16;
+  const int64_t token0 = static_cast<int64_t>(blockIdx.y) * (16 * TB), row0 = static_cast<int64_t>(blockIdx.x) * kRows;
+  const int8_t* x = static_cast<const int8_t*>(a.x) + token0 * a.columns;
+  const int8_t* w = a.codes + row0 * a.columns;
+  const int last_token = static_cast<int>(min(a.tokens - token0, static_cast<int64_t>(16 * TB))) - 1;
+  const int last_row = static_cast<int>(min(a.rows - row0, static_cast<int64_t>(kRows))) - 1;
+  const int parts = (a.columns + 127) / 128;
+
+  // rows and chunks as in many_kernel
+  const auto place = [](int row) { return (row >> 1) & 7; };
+  uint8_t* own = lds + wave * kDepth * kBuffer;
+  uint32_t from[kMoves];
+  int chunk[2];  // of even and odd loads: rows 8 apart are at other places
+#pragma unroll
+  for (int i = 0; i < 2; ++i) chunk[i] = (lane % 8) ^ place(8 * i + lane / 8);
+#pragma unroll
+  for (int i = 0; i < kMoves; ++i) {
+    const int row = i < LT ? min(8 * i + lane / 8, last_token) : min(8 * (i - LT) + lane / 8, last_row);
+    from[i] = static_cast<uint32_t>(row) * a.columns + chunk[i & 1] * 16;
+  }
+  auto past = [&](int part, int i) { return part * 128 + chunk[i & 1] * 16 >= a.columns; };
+  auto bring = [&](int part, int buffer) {
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      const int8_t* base = (i < LT ? x : w) + static_cast<int64_t>(part) * 128;
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(base + (from[i] - (past(part, i) ? chunk[i & 1] * 16 : 0))),
+          (__attribute__((address_space(3))) void*)(own + buffer * kBuffer + i * 1024), 16, 0, 0);
+    }
+  };
+
+  i32x4 acc[TB][2];
+#pragma unroll
+  for (int t = 0; t < TB; ++t)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) acc[t][r] = i32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int d = 0; d < kDepth - 1; ++d)
+    if (wave + d * kSplit < parts) bring(wave + d * kSplit, d);
+  int buffer = 0;
+#pragma unroll 1
+  for (int part = wave; part < parts; part += kSplit, buffer = buffer + 1 < kDepth ? buffer + 1 : 0) {
+    if (part + (kDepth - 1) * kSplit < parts) {
+      bring(part + (kDepth - 1) * kSplit, buffer > 0 ? buffer - 1 : kDepth - 1);
+      constexpr int kLater = (kDepth - 1) * kMoves;  // loads issued after this part's
+      __builtin_amdgcn_s_waitcnt(0x0f70 | (kLater & 15) | ((kLater & 0x30) << 10));
+    } else {
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    uint8_t* here = own + buffer * kBuffer;
+    if (part == parts - 1 && a.columns % 128 != 0) {
+#pragma unroll
+      for (int i = 0; i < LT; ++i)
+        if (past(part, i)) *reinterpret_cast<i32x4*>(here + i * 1024 + lane * 16) = i32x4{0, 0, 0, 0};
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    }
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {
+      i32x4 fx[TB], fw[2];
+      const int at = in_block * 128 + (((step * 4 + q) ^ place(in_block)) * 16);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) fw[r] = *reinterpret_cast<const i32x4*>(here + (LT + 2 * r) * 1024 + at);
+#pragma unroll
+      for (int t = 0; t < TB; ++t) fx[t] = *reinterpret_cast<const i32x4*>(here + 2 * t * 1024 + at);
+#pragma unroll
+      for (int t = 0; t < TB; ++t)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) acc[t][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[r], fx[t], acc[t][r], 0, 0, 0);
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the buffer is free for the next loads
+  }
+
+  // The waves' sums: block (t, r) of wave v at 256 numbers from (v TB + t) 2 + r on.
+  __syncthreads();
+  i32x4* sums = reinterpret_cast<i32x4*>(lds);
+#pragma unroll
+  for (int t = 0; t < TB; ++t)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) sums[((wave * TB + t) * 2 + r) * 64 + lane] = acc[t][r];
+  __syncthreads();
+  const int64_t n = row0 + threadIdx.x % 32;
+  if (n >= a.rows) return;
+  const float scale = a.scales[n], bias = a.bias ? a.bias[n] : 0.0f;
+#pragma unroll
+  for (int t = 0; t < TB; ++t) {
+    const int64_t m = token0 + t * 16 + threadIdx.x / 32;
+    if (m >= a.tokens) break;
+    const int r = threadIdx.x % 32 / 16, of = threadIdx.x % 16;
+    int sum = 0;
+#pragma unroll
+    for (int v = 0; v < kSplit; ++v)
+      sum += reinterpret_cast<const int*>(sums)[(((v * TB + t) * 2 + r) * 64 + of / 4 * 16 + threadIdx.x / 32) * 4 + of % 4];
+    store_score<YT>(a.y, m * a.rows + n, fmaf(static_cast<float>(sum) * a.x_scales[m], scale, bias));
+  }
+}
+
+template <int YT, int TB>
+void launch_long_as(const MatmulArgs& a, hipStream_t s) {
+  constexpr int kLds = 8 * long_depth(TB) * (2 * TB + 4) * 1024;
+  const auto kernel = long_kernel<YT, TB>;
+  static std::once_flag once;
+  std::call_once(once, [&] {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (e != hipSuccess) throw Error(ST_ERR_HIP, cat("hipFuncSetAttribute failed: ", hipGetErrorString(e)));
+  });
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((a.rows + 31) / 32), static_cast<unsigned>((a.tokens + 16 * TB - 1) / (16 * TB))),
+                     dim3(512), kLds, s, a);
+}
+
+template <int TB>
+void launch_long(const MatmulArgs& a, hipStream_t s) {
+  if (a.y_type == ST_SCORE_F32)
+    launch_long_as<ST_SCORE_F32, TB>(a, s);
+  else if (a.y_type == ST_SCORE_F16)
+    launch_long_as<ST_SCORE_F16, TB>(a, s);
+  else
+    launch_long_as<ST_SCORE_BF16, TB>(a, s);
 }
 
 template <int YT, int WT, int WR, int NT, int NR>
@@ -508,6 +628,7 @@ void launch_many_as(const MatmulArgs& a, hipStream_t s) {
     if (e != hipSuccess) throw Error(ST_ERR_HIP, cat("hipFuncSetAttribute failed: ", hipGetErrorString(e)));
   });
   const int64_t tiles = ((a.tokens + NT * WT - 1) / (NT * WT)) * ((a.rows + NR * WR - 1) / (NR * WR));
+  ST_CHECK(tiles < (1ll << 31), "the product has too many results");
   const int64_t grid = std::min<int64_t>(tiles, cu_count() * (160 * 1024 / kLds));
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * NT * NR), kLds, s, a);
 }
@@ -522,11 +643,41 @@ void launch_many(const MatmulArgs& a, hipStream_t s) {
     launch_many_as<ST_SCORE_BF16, WT, WR, NT, NR>(a, s);
 }
 
-// Whether the product takes the vectors to 8 bits itself: each workgroup does it
-// again, so they have to be few; a launch of its own (about 4 us) does it
-// otherwise.
-bool is_fused(int x_type, int64_t tokens, int64_t columns) {
-  return x_type != ST_CODE_I8 && tokens <= 16 && (columns + 255) / 256 * 256 * 16 <= kFusedBytes;
+// Whether the product takes the vectors to 8 bits itself (few_kernel) where a launch
+// of its own does otherwise.  Four vectors: 8,192 x 2,048 6.5 us and 20,000 x 512 7.1
+// us, 8 us with that launch (4 us); but 500,000 x 128, 64 MB, 17.6 us as well.
+bool is_fused(int x_type, int64_t tokens, int64_t rows, int64_t columns) {
+  return x_type != ST_CODE_I8 && tokens <= kFewTokens && columns <= kFewColumns && rows <= kFewBytes / columns;
+}
+
+// The kernel for codes on both sides.
+//
+// Few results of long rows go to long_kernel: 64 x 4,096 x 8,192 12.1 us (20.9 in
+// tiles of 32 x 128), 40 x 1,024 x 8,192 5.6 (6.4), 16 x 512 x 8,192 4.0 (4.1); but 96 x
+// 8,192 x 8,192 47 (36.5), 32 x 512 x 16,384 5.8 (4.6).
+//
+// Else the largest tile that the vectors fill, as long as there are tiles for most
+// of the chip: 200 x 128 x 500,000 in tiles of 256 x 256, 128 x 128, 64 x 128 and 32 x 128
+// 56, 65, 79 and 91 us; 64 x 2,048 x 50,000 29, 20.5, 18 and 26; 512 x 512 x 4,096 12.8,
+// 7.1, 5.8 and 5.7; one vector x 128 x 20,000,000 868, 669, 632 and 573.
+void launch_codes_product(const MatmulArgs& a, hipStream_t s) {
+  const int64_t cus = cu_count();
+  auto tiles = [&](int64_t tokens, int64_t rows) { return ((a.tokens + tokens - 1) / tokens) * ((a.rows + rows - 1) / rows); };
+  const int64_t groups = tiles(32, 32);
+  if ((groups <= cus && a.columns >= 256) || (groups <= 2 * cus && a.columns >= 1024)) {
+    if (a.tokens <= 16)
+      launch_long<1>(a, s);
+    else
+      launch_long<2>(a, s);
+  } else if (a.tokens > 128 && tiles(256, 256) >= cus * 3 / 4) {
+    launch_many<128, 64, 2, 4>(a, s);
+  } else if (a.tokens > 64 && tiles(128, 128) >= cus) {
+    launch_many<64, 64, 2, 2>(a, s);
+  } else if (a.tokens > 32 && tiles(64, 128) >= cus) {
+    launch_many<64, 32, 1, 4>(a, s);
+  } else {
+    launch_many<32, 32, 1, 4>(a, s);
+  }
 }
 
 void check_codes(int64_t rows, int64_t columns) {
@@ -618,9 +769,9 @@ extern "C" int st_int8_quantize(const void* x, int x_type, int64_t rows, int64_t
   });
 }
 
-extern "C" int64_t st_int8_matmul_workspace_bytes(int x_type, int64_t tokens, int64_t columns) {
+extern "C" int64_t st_int8_matmul_workspace_bytes(int x_type, int64_t tokens, int64_t rows, int64_t columns) {
   using namespace st;
-  if (x_type == ST_CODE_I8 || tokens <= 0 || columns <= 0 || is_fused(x_type, tokens, columns)) return 0;
+  if (x_type == ST_CODE_I8 || tokens <= 0 || rows <= 0 || columns <= 0 || is_fused(x_type, tokens, rows, columns)) return 0;
   return codes_bytes(tokens, columns) + tokens * static_cast<int64_t>(sizeof(float));
 }
 
@@ -644,8 +795,8 @@ extern "C" int st_int8_matmul(const int8_t* codes, const float* scales, int64_t 
     hipStream_t s = static_cast<hipStream_t>(stream);
     MatmulArgs a{codes, scales, bias, x, x_scales, y, rows, tokens, x_stride, static_cast<int>(dim), static_cast<int>(columns),
                  x_type, y_type};
-    if (is_fused(x_type, tokens, columns)) {
-      launch_few<1, true>(a, s);
+    if (is_fused(x_type, tokens, rows, columns)) {
+      launch_few(a, s);
       check_launch("few_kernel");
       return;
     }
@@ -656,24 +807,8 @@ extern "C" int st_int8_matmul(const int8_t* codes, const float* scales, int64_t 
       quantize(x, x_type, tokens, dim, x_stride, made, made_scales, s);
       a.x = made;
       a.x_scales = made_scales;
-      a.x_type = ST_CODE_I8;
-      a.x_stride = columns;
-      a.dim = static_cast<int>(columns);
     }
-    if (tokens > 64 && columns >= 256) {
-      if (((tokens + 255) / 256) * ((rows + 255) / 256) >= cu_count() / 2)
-        launch_many<128, 64, 2, 4>(a, s);
-      else
-        launch_many<64, 64, 2, 2>(a, s);
-      check_launch("many_kernel");
-      return;
-    }
-    if (tokens <= 16)
-      launch_few<1, false>(a, s);
-    else if (tokens <= 32)
-      launch_few<2, false>(a, s);
-    else
-      launch_few<4, false>(a, s);
-    check_launch("few_kernel");
+    launch_codes_product(a, s);
+    check_launch("int8_matmul's kernel");
   });
 }

@@ -455,7 +455,7 @@ Tensor int8_matmul_gpu(const Tensor& codes_in, const Tensor& scales_in, const Te
   const int x_type = coded ? ST_CODE_I8 : score_type(x.scalar_type(), "x");
   const int64_t tokens = x.size(0), columns = codes.size(1);
   Tensor y = at::empty(with_last(x_in.sizes(), codes.size(0)), x.options().dtype(out_type)), ws;
-  const int64_t bytes = y.numel() ? st_int8_matmul_workspace_bytes(x_type, tokens, columns) : 0;
+  const int64_t bytes = y.numel() ? st_int8_matmul_workspace_bytes(x_type, tokens, codes.size(0), columns) : 0;
   if (bytes > 0) ws = at::empty({bytes}, x.options().dtype(at::kByte));
   check_st(st_int8_matmul(data_or_null<int8_t>(codes), data_or_null<float>(scales), codes.size(0), columns,
                           bytes_or_null(x), x_type, data_or_null<float>(x_scales), tokens, x.size(1),
