@@ -22,6 +22,12 @@ template <>
 NormShape norm_backward<ST_SCORE_F16>(int dim, bool wide_sum);
 template <>
 NormShape norm_backward<ST_SCORE_BF16>(int dim, bool wide_sum);
+template <>
+const void* norm_columns<ST_SCORE_F32>(bool wide_sum);
+template <>
+const void* norm_columns<ST_SCORE_F16>(bool wide_sum);
+template <>
+const void* norm_columns<ST_SCORE_BF16>(bool wide_sum);
 
 namespace {
 
@@ -52,43 +58,55 @@ NormShape backward_shape_of(int type, int dim, bool wide_sum) {
   return norm_backward<ST_SCORE_BF16>(dim, wide_sum);
 }
 
+const void* columns_kernel_of(int type, bool wide_sum) {
+  if (type == ST_SCORE_F32) return norm_columns<ST_SCORE_F32>(false);
+  if (type == ST_SCORE_F16) return norm_columns<ST_SCORE_F16>(wide_sum);
+  return norm_columns<ST_SCORE_BF16>(wide_sum);
+}
+
+void launch_kernel(const void* kernel, dim3 grid, int threads, void* args, const char* what, hipStream_t s) {
+  void* list[] = {args};
+  const hipError_t e = hipLaunchKernel(kernel, grid, dim3(threads), list, 0, s);
+  if (e != hipSuccess) throw Error(ST_ERR_HIP, cat(what, " launch failed: ", hipGetErrorString(e)));
+}
+
 void launch_forward(NormArgs& a, int type, bool wide_sum, bool codes, hipStream_t s) {
   const NormShape shape = forward_shape_of(type, a.dim, wide_sum, codes);
   const int64_t grid = std::min<int64_t>((a.rows + shape.rows - 1) / shape.rows, static_cast<int64_t>(shape.per_cu) * cu_count());
-  void* args[] = {&a};
-  const hipError_t e = hipLaunchKernel(shape.kernel, dim3(static_cast<unsigned>(grid)), dim3(shape.threads), args, 0, s);
-  if (e != hipSuccess) throw Error(ST_ERR_HIP, cat("norm_kernel launch failed: ", hipGetErrorString(e)));
+  launch_kernel(shape.kernel, dim3(static_cast<unsigned>(grid)), shape.threads, &a, "norm_kernel", s);
 }
 
-// Rows that a workgroup of the backward kernel takes at once (norm_backward's
-// shapes).
-int backward_rows(int64_t dim) { return dim <= 64 ? 32 : dim <= 128 ? 16 : dim <= 256 ? 8 : dim <= 1024 ? 4 : 1; }
-
-// Its workgroups: each adds two rows of sums in 32 bits to the traffic, so there
-// are no more of them than the chip holds at once, and each takes four turns at
-// least where that leaves one a CU.
+// The backward kernel's workgroups: each adds two rows of sums in 32 bits to the
+// traffic, so there are no more of them than the chip holds at once, and each takes
+// four turns at least where that leaves one a CU.
 int64_t backward_groups(int64_t rows, int64_t dim) {
-  const int64_t turns = (rows + backward_rows(dim) - 1) / backward_rows(dim);
-  const int64_t most = dim <= 4096 ? 1024 : 512;
+  const NormLayout l = kNormLayouts[norm_layout(dim, false)];
+  const int64_t turns = (rows + norm_rows(l.lanes) - 1) / norm_rows(l.lanes);
+  const int64_t most = 256 * std::max(1, norm_backward_waves(l.lanes, l.steps) * 256 / norm_threads(l.lanes));
   return std::max<int64_t>(1, std::min(most, std::max(std::min<int64_t>(turns, 256), turns / 4)));
 }
 
-// out[c] = sum over the parts, for 16 columns of gw and gb side by side: 64
-// threads a column take every 64th part each.
-__global__ __launch_bounds__(1024) void norm_finish_kernel(const float* partial, int64_t parts, int dim, void* gw, void* gb,
+// out[c] = sum over the parts, for C columns of gw and gb side by side: 1,024 / C
+// threads a column take turns with the parts.
+template <int C>
+__global__ __launch_bounds__(1024) void norm_finish_kernel(const float* partial, int parts, int dim, void* gw, void* gb,
                                                            int type) {
   __shared__ float sums[1024];
-  const int column = blockIdx.x * 16 + threadIdx.x % 16;
+  const int column = blockIdx.x * C + threadIdx.x % C;
   float t = 0.0f;
-  if (column < 2 * dim)
-    for (int64_t p = threadIdx.x / 16; p < parts; p += 64) t += partial[p * 2 * dim + column];
+  if (column < 2 * dim) {
+    const float* from = partial + column;
+    const int64_t step = 2 * static_cast<int64_t>(dim);
+#pragma unroll 8
+    for (int p = threadIdx.x / C; p < parts; p += 1024 / C) t += from[p * step];
+  }
   sums[threadIdx.x] = t;
   __syncthreads();
-  for (int half = 512; half >= 16; half /= 2) {
+  for (int half = 512; half >= C; half /= 2) {
     if (threadIdx.x < half) sums[threadIdx.x] += sums[threadIdx.x + half];
     __syncthreads();
   }
-  if (threadIdx.x >= 16 || column >= 2 * dim) return;
+  if (threadIdx.x >= C || column >= 2 * dim) return;
   void* out = column < dim ? gw : gb;
   if (!out) return;
   const int c = column < dim ? column : column - dim;
@@ -237,14 +255,21 @@ extern "C" int st_layer_norm_backward(const void* grad_y, int y_type, const void
       a.dim = static_cast<int>(dim);
       a.weight_type = weight_type;
       a.inverse_dim = 1.0f / static_cast<float>(dim);
-      ST_CHECK(shape.rows == backward_rows(dim), "the backward kernel's rows differ from the workspace's");
-      void* args[] = {&a};
-      const hipError_t e = hipLaunchKernel(shape.kernel, dim3(static_cast<unsigned>(groups)), dim3(shape.threads), args, 0, s);
-      if (e != hipSuccess) throw Error(ST_ERR_HIP, cat("norm_backward_kernel launch failed: ", hipGetErrorString(e)));
+      const bool apart = norm_columns_apart(dim), wide = h_type != y_type;
+      if (!apart || grad_x || grad_residual)
+        launch_kernel(shape.kernel, dim3(static_cast<unsigned>(groups)), shape.threads, &a, "norm_backward_kernel", s);
+      if (apart && sums) {
+        groups = std::min<int64_t>(groups, 128);  // times 2,048 columns each
+        launch_kernel(columns_kernel_of(y_type, wide), dim3(static_cast<unsigned>((dim + 2047) / 2048), static_cast<unsigned>(groups)),
+                      256, &a, "norm_columns_kernel", s);
+      }
     }
     if (sums) {  // without rows the sums are zeros
-      hipLaunchKernelGGL(norm_finish_kernel, dim3(static_cast<unsigned>((2 * dim + 15) / 16)), dim3(1024), 0, s,
-                         static_cast<const float*>(workspace), groups, static_cast<int>(dim), grad_weight, grad_bias, weight_type);
+      const float* partial = static_cast<const float*>(workspace);
+      const int columns = dim < 2048 ? 16 : 32, parts = static_cast<int>(groups), d = static_cast<int>(dim);
+      hipLaunchKernelGGL(columns == 16 ? norm_finish_kernel<16> : norm_finish_kernel<32>,
+                         dim3(static_cast<unsigned>((2 * dim + columns - 1) / columns)), dim3(1024), 0, s, partial, parts, d,
+                         grad_weight, grad_bias, weight_type);
       check_launch("norm_finish_kernel");
     }
   });

@@ -49,6 +49,28 @@ struct NormBackwardArgs {
   DropoutArgs dropout;
 };
 
+// Lanes of a row and steps of 8 columns a lane: the first that holds a row.
+struct NormLayout {
+  int lanes, steps;
+};
+constexpr NormLayout kNormLayouts[] = {{1, 1},  {2, 1},  {4, 1},   {8, 1},   {16, 1},  {8, 3},   {32, 1},  {16, 3},   {64, 1},
+                                       {32, 3}, {64, 2}, {64, 3},  {256, 1}, {128, 3}, {256, 2}, {256, 3}, {512, 2}, {512, 3},
+                                       {1024, 2}, {1024, 4}};
+constexpr int kNormLayoutCount = sizeof(kNormLayouts) / sizeof(kNormLayouts[0]);
+
+constexpr int norm_layout(int64_t dim, bool codes) {
+  int i = codes ? 1 : 0;  // codes take 16 columns at least
+  while (kNormLayouts[i].lanes * kNormLayouts[i].steps * 8 < dim) ++i;
+  return i;
+}
+constexpr int norm_threads(int lanes) { return lanes <= 64 ? 256 : lanes; }
+constexpr int norm_rows(int lanes) { return lanes <= 64 ? 256 / lanes : 1; }
+
+// Waves a SIMD that the backward kernel's registers leave room for.
+constexpr int norm_backward_waves(int lanes, int steps) {
+  return lanes == 1024 || steps == 1 ? 4 : lanes <= 256 && steps == 2 ? 3 : 2;
+}
+
 struct NormShape {
   const void* kernel;
   int threads, rows;  // of a workgroup
@@ -67,6 +89,15 @@ template <int DT>
 NormShape norm_forward(int dim, bool wide_sum, bool codes);
 template <int DT>
 NormShape norm_backward(int dim, bool wide_sum);
+template <int DT>
+const void* norm_columns(bool wide_sum);
+
+// Whether the backward kernel leaves the weight's and the bias's gradients to
+// norm_columns_kernel.
+constexpr bool norm_columns_apart(int64_t dim) {
+  const NormLayout l = kNormLayouts[norm_layout(dim, false)];
+  return l.lanes * l.steps > 2048;
+}
 
 #ifdef ST_NORM_TYPE
 namespace {
@@ -77,15 +108,25 @@ __device__ __forceinline__ float load_typed(const void* p, int64_t i, int type) 
   return load_score<ST_SCORE_BF16>(p, i);
 }
 
-// Columns [col, col + 8) of a row; 0 past its end.
+// Columns [col, col + 8) of a row as they are stored; 0 past its end.
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load_raw_columns(const void* row, int col, int dim) {
+  if (col + 8 <= dim) return load_raw8<DT>(row, col);
+  Raw8<DT> r{};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (col + i >= dim) continue;
+    if constexpr (DT == ST_SCORE_F32)
+      r.w[i / 4][i % 4] = static_cast<const uint32_t*>(row)[col + i];
+    else
+      r.w[0][i / 2] |= static_cast<uint32_t>(static_cast<const uint16_t*>(row)[col + i]) << (16 * (i & 1));
+  }
+  return r;
+}
+
 template <int DT>
 __device__ __forceinline__ void load_columns(const void* row, int col, int dim, float v[8]) {
-  if (col + 8 <= dim) {
-    unpack8<DT>(load_raw8<DT>(row, col), v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < dim ? load_score<DT>(row, col + i) : 0.0f;
-  }
+  unpack8<DT>(load_raw_columns<DT>(row, col, dim), v);
 }
 
 __device__ __forceinline__ void load_columns_typed(const void* row, int col, int dim, int type, float v[8]) {
@@ -112,7 +153,9 @@ __device__ __forceinline__ void store_columns(void* row, int col, int dim, const
 // order.
 template <int L, typename F>
 __device__ __forceinline__ float join_lanes(float x, F f) {
-  x = join8(x, f);
+  if constexpr (L >= 2) x = f(x, dpp_move<0xB1>(x));    // quad_perm [1, 0, 3, 2]
+  if constexpr (L >= 4) x = f(x, dpp_move<0x4E>(x));    // quad_perm [2, 3, 0, 1]
+  if constexpr (L >= 8) x = f(x, dpp_move<0x141>(x));   // row_half_mirror
   if constexpr (L >= 16) x = f(x, dpp_move<0x140>(x));  // row_mirror
   if constexpr (L >= 32) {
     const int i = __float_as_int(x);
@@ -152,13 +195,11 @@ __device__ __forceinline__ void join_row(float (&x)[N], float* room, F f) {
 constexpr auto kAdd = [](float a, float b) { return a + b; };
 constexpr auto kMost = [](float a, float b) { return fmaxf(a, b); };
 
-constexpr int norm_threads(int lanes) { return lanes <= 256 ? 256 : lanes; }
-
 // HT: the type of h.  CODES: the result goes to 8 bits with a scale for each
 // row, from its 32-bit values.
 template <int DT, int HT, int L, int S, bool CODES>
 __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
-  constexpr int kRows = L <= 64 ? norm_threads(L) / L : 1;
+  constexpr int kRows = norm_rows(L);
   // Weights stay in registers from row to row where there is room for them.
   constexpr bool kHold = S <= 2;
   __shared__ float room[L > 64 ? 4 * (L / 64) : 1];
@@ -167,112 +208,136 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
   if (a.dropout.used && blockIdx.x == 0 && threadIdx.x < 2) a.dropout.used[threadIdx.x] = a.dropout.state[threadIdx.x];
 
   float w[kHold ? S : 1][8], b[kHold ? S : 1][8];
-  auto load_weights = [&](int s, float (&ws)[8], float (&bs)[8]) {
+  auto load_weights = [&](const void* weight, const void* bias, int s, float (&ws)[8], float (&bs)[8]) {
     const int col = (s * L + lane) * 8;
-    if (a.weight)
-      load_columns_typed(a.weight, col, a.dim, a.weight_type, ws);
+    if (weight)
+      load_columns_typed(weight, col, a.dim, a.weight_type, ws);
     else
 #pragma unroll
       for (int i = 0; i < 8; ++i) ws[i] = 1.0f;
-    if (a.bias)
-      load_columns_typed(a.bias, col, a.dim, a.weight_type, bs);
+    if (bias)
+      load_columns_typed(bias, col, a.dim, a.weight_type, bs);
     else
 #pragma unroll
       for (int i = 0; i < 8; ++i) bs[i] = 0.0f;
   };
   if constexpr (kHold) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) load_weights(s, w[s], b[s]);
+    for (int s = 0; s < S; ++s) load_weights(a.weight, a.bias, s, w[s], b[s]);
   }
 
   // A wave's rows go through the loop together; what a lane of a row past the
-  // last computes is not stored.
+  // last computes is not stored.  The next row is on its way while one is worked on,
+  // where there are registers for it.
+  constexpr bool kNext = L * S <= 2048;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / (L < 64 ? 64 : L) * (L < 64 ? 64 / L : 1);
-  for (int64_t base = first; base < a.rows; base += static_cast<int64_t>(gridDim.x) * kRows) {
-    const int64_t at = base + (L < 64 ? threadIdx.x % 64 / L : 0);
-    const bool live = at < a.rows;
-    const int64_t row = live ? at : a.rows - 1;
+  const int within = L < 64 ? threadIdx.x % 64 / L : 0;
+  Raw8<DT> next_x[S];
+  Raw8<HT> next_residual[S];
+  auto fetch = [&](int64_t base) {
+    if (base >= a.rows) return;
+    const int64_t row = min(base + within, a.rows - 1);
     const char* x = static_cast<const char*>(a.x) + row * a.x_stride * kScoreBytes<DT>;
-    float h[S][8];
 #pragma unroll
-    for (int s = 0; s < S; ++s) load_columns<DT>(x, (s * L + lane) * 8, a.dim, h[s]);
+    for (int s = 0; s < S; ++s) next_x[s] = load_raw_columns<DT>(x, (s * L + lane) * 8, a.dim);
     if constexpr (!CODES) {
       if (a.residual) {
         const char* residual = static_cast<const char*>(a.residual) + row * a.residual_stride * kScoreBytes<HT>;
-        char* sum = static_cast<char*>(a.sum) + row * a.dim * kScoreBytes<HT>;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const int col = (s * L + lane) * 8;
-          float more[8];
-          load_columns<HT>(residual, col, a.dim, more);
-          uint32_t keeps = 0xFF;
-          if (a.dropout.state)
-            keeps = dropout_keeps(key, static_cast<uint64_t>(row) * a.dim + col, a.dropout.dropped);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float kept = (keeps >> i) & 1 ? __fmul_rn(h[s][i], a.dropout.times) : 0.0f;
-            // the norm is of the sum as it is returned
-            h[s][i] = score_of_bits<HT>(score_bits<HT>(__fadd_rn(more[i], kept)));
-          }
-          if (live) store_columns<HT>(sum, col, a.dim, h[s]);
-        }
+        for (int s = 0; s < S; ++s) next_residual[s] = load_raw_columns<HT>(residual, (s * L + lane) * 8, a.dim);
       }
     }
-
-    if (!CODES || a.normalise) {
-      float total[1] = {0.0f};
+  };
+  if constexpr (kNext) fetch(first);
+  for (int64_t base = first; base < a.rows; base += step) {
+    const int64_t at = base + within;
+    const bool live = at < a.rows;
+    const int64_t row = live ? at : a.rows - 1;
+    if constexpr (!kNext) fetch(base);
+    char* sum = static_cast<char*>(a.sum) + row * a.dim * kScoreBytes<HT>;
+    float h[S][8];
+    // h of step s
+    auto values = [&](int s, float (&v)[8]) {
+      const int col = (s * L + lane) * 8;
+      unpack8<DT>(next_x[s], v);
+      if constexpr (!CODES) {
+        if (!a.residual) return;
+        float more[8];
+        unpack8<HT>(next_residual[s], more);
+        uint32_t keeps = 0xFF;
+        if (a.dropout.state) keeps = dropout_keeps(key, static_cast<uint64_t>(row) * a.dim + col, a.dropout.dropped);
 #pragma unroll
-      for (int s = 0; s < S; ++s)
+        for (int i = 0; i < 8; ++i) {
+          const float kept = (keeps >> i) & 1 ? __fmul_rn(v[i], a.dropout.times) : 0.0f;
+          // the norm is of the sum as it is returned
+          v[i] = score_of_bits<HT>(score_bits<HT>(__fadd_rn(more[i], kept)));
+        }
+        if (live) store_columns<HT>(sum, col, a.dim, v);
+      }
+    };
+    const void *weight = a.weight, *bias = a.bias;
+    if constexpr (!kHold) asm volatile("" : "+s"(weight), "+s"(bias));  // else the compiler holds them after all, and spills
+
+    float mean = 0.0f, rest = 0.0f, r = 1.0f;
+    float total[1] = {0.0f};
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      values(s, h[s]);
+      if (!CODES || a.normalise)
 #pragma unroll
         for (int i = 0; i < 8; ++i) total[0] += h[s][i];
+    }
+    if constexpr (kNext) fetch(base + step);
+    if (!CODES || a.normalise) {
       join_row<L>(total, room, kAdd);
-      const float mean = __fdiv_rn(total[0], static_cast<float>(a.dim));
+      mean = __fdiv_rn(total[0], static_cast<float>(a.dim));
       // what the mean's rounding left, and the squares about the rounded one
       float left[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const int col = (s * L + lane) * 8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          h[s][i] = col + i < a.dim ? h[s][i] - mean : 0.0f;
+          h[s][i] = (s * L + lane) * 8 + i < a.dim ? h[s][i] - mean : 0.0f;
           left[0] += h[s][i];
           left[1] = fmaf(h[s][i], h[s][i], left[1]);
         }
       }
       join_row<L>(left, room + (L > 64 ? L / 64 : 0), kAdd);
-      const float rest = __fdiv_rn(left[0], static_cast<float>(a.dim));
+      rest = __fdiv_rn(left[0], static_cast<float>(a.dim));
       // a maximum with 0 would turn NaN into it
       float squares = fmaf(-rest, left[0], left[1]);
       squares = squares < 0.0f ? 0.0f : squares;
-      const float r = __fdiv_rn(1.0f, __fsqrt_rn(fmaf(squares, 1.0f / static_cast<float>(a.dim), a.eps)));
+      r = __fdiv_rn(1.0f, __fsqrt_rn(fmaf(squares, 1.0f / static_cast<float>(a.dim), a.eps)));
       if (a.stats && live && lane == 0) {
         a.stats[kNormStats * row] = mean;
         a.stats[kNormStats * row + 1] = rest;
         a.stats[kNormStats * row + 2] = r;
       }
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        if constexpr (!kHold) load_weights(s, w[0], b[0]);
-        const int hold = kHold ? s : 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[s][i] = fmaf((h[s][i] - rest) * r, w[hold][i], b[hold][i]);
-      }
     }
-
+    // the result's values of step s
+    auto result = [&](int s, float (&v)[8]) {
+      if (CODES && !a.normalise) return;
+      if constexpr (!kHold) load_weights(weight, bias, s, w[0], b[0]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = fmaf((v[i] - rest) * r, w[kHold ? s : 0][i], b[kHold ? s : 0][i]);
+    };
     if constexpr (!CODES) {
       char* y = static_cast<char*>(a.y) + row * a.dim * kScoreBytes<DT>;
-      if (live)
 #pragma unroll
-        for (int s = 0; s < S; ++s) store_columns<DT>(y, (s * L + lane) * 8, a.dim, h[s]);
+      for (int s = 0; s < S; ++s) {
+        result(s, h[s]);
+        if (live) store_columns<DT>(y, (s * L + lane) * 8, a.dim, h[s]);
+      }
     } else {
       float most[1] = {0.0f};
       float odd = 0.0f;  // NaN if there is one, or an infinity, in the row
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const int col = (s * L + lane) * 8;
+        result(s, h[s]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (col + i >= a.dim) h[s][i] = 0.0f;
+          if ((s * L + lane) * 8 + i >= a.dim) h[s][i] = 0.0f;
           most[0] = fmaxf(most[0], fabsf(h[s][i]));
           odd = fmaf(h[s][i], 0.0f, odd);
         }
@@ -296,61 +361,80 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
 
 // Lanes own the same columns in every row, so the weight's and the bias's
 // gradients are sums in registers, joined once a workgroup and then, in a fixed
-// order, by norm_finish_kernel: no atomics, the same bits every time.
+// order, by norm_finish_kernel: no atomics, the same bits every time.  The longest
+// rows leave no registers for them (spilled, they took 3,051 x 32,768 to 640 us):
+// norm_columns_kernel reads everything once more.
 template <int DT, int HT, int L, int S>
-__global__ __launch_bounds__(norm_threads(L)) void norm_backward_kernel(NormBackwardArgs a) {
-  constexpr int kRows = L <= 64 ? norm_threads(L) / L : 1;
-  constexpr bool kHold = S <= 2;
+__global__ __launch_bounds__(norm_threads(L), norm_backward_waves(L, S)) void norm_backward_kernel(NormBackwardArgs a) {
+  constexpr int kRows = norm_rows(L);
+  constexpr bool kHold = S <= 2, kSums = L * S <= 2048, kNext = L * S <= 1024;
   __shared__ float room[L > 64 ? 4 * (L / 64) : 1];
   __shared__ float joined[L <= 64 ? 256 * 8 : 1];
   const int lane = threadIdx.x % L;
   const DropoutKey key = a.dropout.state ? dropout_key(a.dropout.state) : DropoutKey{};
 
-  float w[kHold ? S : 1][8], gw[S][8], gb[S][8];
-  auto load_weights = [&](int s, float (&ws)[8]) {
-    if (a.weight)
-      load_columns_typed(a.weight, (s * L + lane) * 8, a.dim, a.weight_type, ws);
+  float w[kHold ? S : 1][8], gw[kSums ? S : 1][8], gb[kSums ? S : 1][8];
+  auto load_weights = [&](const void* weight, int s, float (&ws)[8]) {
+    if (weight)
+      load_columns_typed(weight, (s * L + lane) * 8, a.dim, a.weight_type, ws);
     else
 #pragma unroll
       for (int i = 0; i < 8; ++i) ws[i] = 1.0f;
   };
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    if constexpr (kHold) load_weights(s, w[s]);
+    if constexpr (kHold) load_weights(a.weight, s, w[s]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) gw[s][i] = gb[s][i] = 0.0f;
+    for (int i = 0; i < 8; ++i) gw[kSums ? s : 0][i] = gb[kSums ? s : 0][i] = 0.0f;
   }
 
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / (L < 64 ? 64 : L) * (L < 64 ? 64 / L : 1);
-  int turn = 0;
-  for (int64_t base = first; base < a.rows; base += static_cast<int64_t>(gridDim.x) * kRows, turn ^= 1) {
-    const int64_t at = base + (L < 64 ? threadIdx.x % 64 / L : 0);
-    const bool live = at < a.rows;
-    const int64_t row = live ? at : a.rows - 1;
+  const int within = L < 64 ? threadIdx.x % 64 / L : 0;
+  // The next row is on its way while one is worked on, where there are registers for
+  // it.
+  Raw8<DT> next_g[S];
+  Raw8<HT> next_h[S];
+  auto fetch = [&](int64_t base) {
+    if (base >= a.rows) return;
+    const int64_t row = min(base + within, a.rows - 1);
     const char* gy = static_cast<const char*>(a.gy) + row * a.dim * kScoreBytes<DT>;
     const char* hs = static_cast<const char*>(a.h) + row * a.h_stride * kScoreBytes<HT>;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      next_g[s] = load_raw_columns<DT>(gy, (s * L + lane) * 8, a.dim);
+      next_h[s] = load_raw_columns<HT>(hs, (s * L + lane) * 8, a.dim);
+    }
+  };
+  int turn = 0;
+  if constexpr (kNext) fetch(first);
+  for (int64_t base = first; base < a.rows; base += step, turn ^= 1) {
+    const int64_t at = base + within;
+    const bool live = at < a.rows;
+    const int64_t row = live ? at : a.rows - 1;
     const float mean = a.stats[kNormStats * row], rest = a.stats[kNormStats * row + 1], r = a.stats[kNormStats * row + 2];
+    if constexpr (!kNext) fetch(base);
     float g[S][8], n[S][8];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const int col = (s * L + lane) * 8;
-      load_columns<DT>(gy, col, a.dim, g[s]);
-      load_columns<HT>(hs, col, a.dim, n[s]);
+      unpack8<DT>(next_g[s], g[s]);
+      unpack8<HT>(next_h[s], n[s]);
     }
+    if constexpr (kNext) fetch(base + step);
+    const void* weight = a.weight;
+    if constexpr (!kHold) asm volatile("" : "+s"(weight));  // as in norm_kernel
     float sums[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const int col = (s * L + lane) * 8;
-      if constexpr (!kHold) load_weights(s, w[0]);
-      const int hold = kHold ? s : 0;
+      if constexpr (!kHold) load_weights(weight, s, w[0]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        n[s][i] = col + i < a.dim ? ((n[s][i] - mean) - rest) * r : 0.0f;
-        if (live) {
-          gw[s][i] = fmaf(g[s][i], n[s][i], gw[s][i]);
-          gb[s][i] += g[s][i];
+        n[s][i] = (s * L + lane) * 8 + i < a.dim ? ((n[s][i] - mean) - rest) * r : 0.0f;
+        if (kSums && live) {
+          gw[kSums ? s : 0][i] = fmaf(g[s][i], n[s][i], gw[kSums ? s : 0][i]);
+          gb[kSums ? s : 0][i] += g[s][i];
         }
-        g[s][i] *= w[hold][i];
+        g[s][i] *= w[kHold ? s : 0][i];
         sums[0] += g[s][i];
         sums[1] = fmaf(g[s][i], n[s][i], sums[1]);
       }
@@ -381,13 +465,13 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_backward_kernel(NormBack
     }
   }
 
-  if (!a.partial) return;
+  if (!kSums || !a.partial) return;
   float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
   if constexpr (L > 64) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      store_columns<ST_SCORE_F32>(out, (s * L + lane) * 8, a.dim, gw[s]);
-      store_columns<ST_SCORE_F32>(out + a.dim, (s * L + lane) * 8, a.dim, gb[s]);
+      store_columns<ST_SCORE_F32>(out, (s * L + lane) * 8, a.dim, gw[kSums ? s : 0]);
+      store_columns<ST_SCORE_F32>(out + a.dim, (s * L + lane) * 8, a.dim, gb[kSums ? s : 0]);
     }
   } else {
     // the workgroup's rows, a step and a gradient at a time
@@ -406,65 +490,88 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_backward_kernel(NormBack
     };
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      join(gw[s], s, out);
-      join(gb[s], s, out + a.dim);
+      join(gw[kSums ? s : 0], s, out);
+      join(gb[kSums ? s : 0], s, out + a.dim);
     }
   }
 }
 
-template <int DT, int HT, int L, int S, bool CODES>
-NormShape forward_shape() {
-  static const NormShape shape = norm_shape(norm_kernel<DT, HT, L, S, CODES>, norm_threads(L), L <= 64 ? norm_threads(L) / L : 1);
-  return shape;
+// The weight's and the bias's gradients alone: a workgroup has 2,048 columns of
+// every gridDim.y-th row.
+template <int DT, int HT>
+__global__ __launch_bounds__(256) void norm_columns_kernel(NormBackwardArgs a) {
+  const int col = (blockIdx.x * 256 + threadIdx.x) * 8;
+  if (col >= a.dim) return;
+  float gw[8] = {}, gb[8] = {};
+#pragma unroll 2
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    float g[8], h[8];
+    load_columns<DT>(static_cast<const char*>(a.gy) + row * a.dim * kScoreBytes<DT>, col, a.dim, g);
+    load_columns<HT>(static_cast<const char*>(a.h) + row * a.h_stride * kScoreBytes<HT>, col, a.dim, h);
+    const float mean = a.stats[kNormStats * row], rest = a.stats[kNormStats * row + 1], r = a.stats[kNormStats * row + 2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      gw[i] = fmaf(g[i], ((h[i] - mean) - rest) * r, gw[i]);
+      gb[i] += g[i];
+    }
+  }
+  float* out = a.partial + static_cast<int64_t>(blockIdx.y) * 2 * a.dim;
+  store_columns<ST_SCORE_F32>(out, col, a.dim, gw);
+  store_columns<ST_SCORE_F32>(out + a.dim, col, a.dim, gb);
 }
 
-template <int DT, int HT, bool CODES>
-NormShape forward_for(int dim) {
-  if (dim <= 64) return forward_shape<DT, HT, 8, 1, CODES>();
-  if (dim <= 128) return forward_shape<DT, HT, 16, 1, CODES>();
-  if (dim <= 256) return forward_shape<DT, HT, 32, 1, CODES>();
-  if (dim <= 512) return forward_shape<DT, HT, 64, 1, CODES>();
-  if (dim <= 1024) return forward_shape<DT, HT, 64, 2, CODES>();
-  if (dim <= 2048) return forward_shape<DT, HT, 256, 1, CODES>();
-  if (dim <= 4096) return forward_shape<DT, HT, 256, 2, CODES>();
-  if (dim <= 8192) return forward_shape<DT, HT, 1024, 1, CODES>();
-  if (dim <= 16384) return forward_shape<DT, HT, 1024, 2, CODES>();
-  return forward_shape<DT, HT, 1024, 4, CODES>();
+template <int DT, int HT, int L, int S, bool CODES>
+NormShape forward_shape() {
+  if constexpr (CODES && L == 1) return {};  // norm_layout gives none
+  static const NormShape shape = norm_shape(norm_kernel<DT, HT, L, S, CODES>, norm_threads(L), norm_rows(L));
+  return shape;
 }
 
 template <int DT, int HT, int L, int S>
 NormShape backward_shape() {
-  static const NormShape shape = norm_shape(norm_backward_kernel<DT, HT, L, S>, norm_threads(L), L <= 64 ? norm_threads(L) / L : 1);
+  static const NormShape shape = norm_shape(norm_backward_kernel<DT, HT, L, S>, norm_threads(L), norm_rows(L));
   return shape;
 }
 
-template <int DT, int HT>
-NormShape backward_for(int dim) {
-  if (dim <= 64) return backward_shape<DT, HT, 8, 1>();
-  if (dim <= 128) return backward_shape<DT, HT, 16, 1>();
-  if (dim <= 256) return backward_shape<DT, HT, 32, 1>();
-  if (dim <= 512) return backward_shape<DT, HT, 64, 1>();
-  if (dim <= 1024) return backward_shape<DT, HT, 64, 2>();
-  if (dim <= 2048) return backward_shape<DT, HT, 256, 1>();
-  if (dim <= 4096) return backward_shape<DT, HT, 256, 2>();
-  if (dim <= 8192) return backward_shape<DT, HT, 1024, 1>();
-  if (dim <= 16384) return backward_shape<DT, HT, 1024, 2>();
-  return backward_shape<DT, HT, 1024, 4>();
+template <int DT, int HT, bool CODES, int I = 0>
+NormShape forward_for(int layout) {
+  if constexpr (I < kNormLayoutCount) {
+    if (layout == I) return forward_shape<DT, HT, kNormLayouts[I].lanes, kNormLayouts[I].steps, CODES>();
+    return forward_for<DT, HT, CODES, I + 1>(layout);
+  }
+  return {};
+}
+
+template <int DT, int HT, int I = 0>
+NormShape backward_for(int layout) {
+  if constexpr (I < kNormLayoutCount) {
+    if (layout == I) return backward_shape<DT, HT, kNormLayouts[I].lanes, kNormLayouts[I].steps>();
+    return backward_for<DT, HT, I + 1>(layout);
+  }
+  return {};
 }
 
 }  // namespace
 
 template <>
 NormShape norm_forward<ST_NORM_TYPE>(int dim, bool wide_sum, bool codes) {
-  if (codes) return forward_for<ST_NORM_TYPE, ST_NORM_TYPE, true>(dim);
-  if (wide_sum) return forward_for<ST_NORM_TYPE, ST_SCORE_F32, false>(dim);
-  return forward_for<ST_NORM_TYPE, ST_NORM_TYPE, false>(dim);
+  const int layout = norm_layout(dim, codes);
+  if (codes) return forward_for<ST_NORM_TYPE, ST_NORM_TYPE, true>(layout);
+  if (wide_sum) return forward_for<ST_NORM_TYPE, ST_SCORE_F32, false>(layout);
+  return forward_for<ST_NORM_TYPE, ST_NORM_TYPE, false>(layout);
 }
 
 template <>
 NormShape norm_backward<ST_NORM_TYPE>(int dim, bool wide_sum) {
-  if (wide_sum) return backward_for<ST_NORM_TYPE, ST_SCORE_F32>(dim);
-  return backward_for<ST_NORM_TYPE, ST_NORM_TYPE>(dim);
+  const int layout = norm_layout(dim, false);
+  if (wide_sum) return backward_for<ST_NORM_TYPE, ST_SCORE_F32>(layout);
+  return backward_for<ST_NORM_TYPE, ST_NORM_TYPE>(layout);
+}
+
+template <>
+const void* norm_columns<ST_NORM_TYPE>(bool wide_sum) {
+  if (wide_sum) return reinterpret_cast<const void*>(&norm_columns_kernel<ST_NORM_TYPE, ST_SCORE_F32>);
+  return reinterpret_cast<const void*>(&norm_columns_kernel<ST_NORM_TYPE, ST_NORM_TYPE>);
 }
 #endif
 
