@@ -655,8 +655,8 @@ int st_layer_norm_int8(const void* x, int x_type, int64_t rows, int64_t dim, int
  *
  * st_int8_quantize: x [rows, dim] (x_type; rows x_stride apart) to codes int8
  * [rows, st_int8_columns(dim)] (whole blocks of 16 columns, zeros past dim;
- * 16-byte aligned) and scales [rows]: scale = max |x| / 127, code = x * (127 /
- * max |x|) to the nearest even, both quotients rounded to 32 bits.  A row whose
+ * 16-byte aligned) and scales [rows]: scale = max |x| / 127, code = x * (127 * (1 /
+ * max |x|)) to the nearest even, every step rounded to 32 bits.  A row whose
  * largest magnitude is below 2^-119 has scale 0; one with a value that is not
  * finite has codes 0 and scale NaN.
  *

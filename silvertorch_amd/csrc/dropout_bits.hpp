@@ -77,4 +77,11 @@ __device__ __forceinline__ uint32_t dropout_keeps(const DropoutKey& k, uint64_t 
   return keeps;
 }
 
+// residual + what is left of x, the product rounded by itself.
+__device__ __forceinline__ float dropout_add(float residual, float x, bool keep, float times) {
+#pragma clang fp contract(off)
+  const float kept = keep ? x * times : 0.0f;
+  return residual + kept;
+}
+
 }  // namespace st

@@ -269,9 +269,8 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
         if (a.dropout.state) keeps = dropout_keeps(key, static_cast<uint64_t>(row) * a.dim + col, a.dropout.dropped);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float kept = (keeps >> i) & 1 ? __fmul_rn(v[i], a.dropout.times) : 0.0f;
           // the norm is of the sum as it is returned
-          v[i] = score_of_bits<HT>(score_bits<HT>(__fadd_rn(more[i], kept)));
+          v[i] = score_of_bits<HT>(score_bits<HT>(dropout_add(more[i], v[i], (keeps >> i) & 1, a.dropout.times)));
         }
         if (live) store_columns<HT>(sum, col, a.dim, v);
       }

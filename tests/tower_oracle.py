@@ -64,8 +64,9 @@ def codes(x):
     most = f.abs().amax(-1)
     fine = torch.isfinite(f).all(-1)
     small = most < 2.0 ** -119
-    times_ = torch.where(fine & ~small, torch.full_like(most, 127.0) / most, 0.0)
-    scales = torch.where(fine, torch.where(small, 0.0, most / 127.0), torch.nan)
+    # quotients of two tensors, which are rounded once
+    times_ = torch.where(fine & ~small, torch.ones_like(most) / most * 127.0, 0.0)
+    scales = torch.where(fine, torch.where(small, 0.0, most / torch.full_like(most, 127.0)), torch.nan)
     q = torch.where((times_ != 0).unsqueeze(-1), (f * times_.unsqueeze(-1)).round(), 0.0)
     return torch.nn.functional.pad(q, (0, -dim % 16)).to(torch.int8), scales
 
