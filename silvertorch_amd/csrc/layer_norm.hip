@@ -80,7 +80,7 @@ void launch_forward(NormArgs& a, int type, bool wide_sum, bool codes, hipStream_
 // traffic, so there are no more of them than the chip holds at once, and each takes
 // four turns at least where that leaves one a CU.
 int64_t backward_groups(int64_t rows, int64_t dim) {
-  const NormLayout l = kNormLayouts[norm_layout(dim, false)];
+  const NormLayout l = kNormLayouts[norm_layout(dim)];
   const int64_t turns = (rows + norm_rows(l.lanes) - 1) / norm_rows(l.lanes);
   const int64_t most = 256 * std::max(1, norm_backward_waves(l.lanes, l.steps) * 256 / norm_threads(l.lanes));
   return std::max<int64_t>(1, std::min(most, std::max(std::min<int64_t>(turns, 256), turns / 4)));

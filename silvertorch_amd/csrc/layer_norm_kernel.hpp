@@ -56,11 +56,16 @@ struct NormLayout {
 constexpr NormLayout kNormLayouts[] = {{1, 1},  {2, 1},  {4, 1},   {8, 1},   {16, 1},  {8, 3},   {32, 1},  {16, 3},   {64, 1},
                                        {32, 3}, {64, 2}, {64, 3},  {256, 1}, {128, 3}, {256, 2}, {256, 3}, {512, 2}, {512, 3},
                                        {1024, 2}, {1024, 4}};
+// Where codes are the result, instructions bound it, a good part of them the same
+// for any number of columns a lane has: 16,384 x 4,096 with 256 lanes 62 us.
+constexpr NormLayout kCodeLayouts[] = {{2, 1},  {4, 1},  {8, 1},   {16, 1},  {16, 2}, {16, 4},
+                                       {32, 4}, {64, 4}, {128, 4}, {256, 4}, {512, 4}, {1024, 4}};
 constexpr int kNormLayoutCount = sizeof(kNormLayouts) / sizeof(kNormLayouts[0]);
+constexpr int kCodeLayoutCount = sizeof(kCodeLayouts) / sizeof(kCodeLayouts[0]);
 
-constexpr int norm_layout(int64_t dim, bool codes) {
-  int i = codes ? 1 : 0;  // codes take 16 columns at least
-  while (kNormLayouts[i].lanes * kNormLayouts[i].steps * 8 < dim) ++i;
+constexpr int norm_layout(int64_t dim, const NormLayout* layouts = kNormLayouts) {
+  int i = 0;
+  while (layouts[i].lanes * layouts[i].steps * 8 < dim) ++i;
   return i;
 }
 constexpr int norm_threads(int lanes) { return lanes <= 64 ? 256 : lanes; }
@@ -95,7 +100,7 @@ const void* norm_columns(bool wide_sum);
 // Whether the backward kernel leaves the weight's and the bias's gradients to
 // norm_columns_kernel.
 constexpr bool norm_columns_apart(int64_t dim) {
-  const NormLayout l = kNormLayouts[norm_layout(dim, false)];
+  const NormLayout l = kNormLayouts[norm_layout(dim)];
   return l.lanes * l.steps > 2048;
 }
 
@@ -201,7 +206,7 @@ template <int DT, int HT, int L, int S, bool CODES>
 __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
   constexpr int kRows = norm_rows(L);
   // Weights stay in registers from row to row where there is room for them.
-  constexpr bool kHold = S <= 2;
+  constexpr bool kHold = CODES ? L * S <= 2048 : S <= 2;
   __shared__ float room[L > 64 ? 4 * (L / 64) : 1];
   const int lane = threadIdx.x % L;
   const DropoutKey key = a.dropout.state ? dropout_key(a.dropout.state) : DropoutKey{};
@@ -521,7 +526,6 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(NormBackwardArgs a) {
 
 template <int DT, int HT, int L, int S, bool CODES>
 NormShape forward_shape() {
-  if constexpr (CODES && L == 1) return {};  // norm_layout gives none
   static const NormShape shape = norm_shape(norm_kernel<DT, HT, L, S, CODES>, norm_threads(L), norm_rows(L));
   return shape;
 }
@@ -534,8 +538,9 @@ NormShape backward_shape() {
 
 template <int DT, int HT, bool CODES, int I = 0>
 NormShape forward_for(int layout) {
-  if constexpr (I < kNormLayoutCount) {
-    if (layout == I) return forward_shape<DT, HT, kNormLayouts[I].lanes, kNormLayouts[I].steps, CODES>();
+  constexpr const NormLayout* layouts = CODES ? kCodeLayouts : kNormLayouts;
+  if constexpr (I < (CODES ? kCodeLayoutCount : kNormLayoutCount)) {
+    if (layout == I) return forward_shape<DT, HT, layouts[I].lanes, layouts[I].steps, CODES>();
     return forward_for<DT, HT, CODES, I + 1>(layout);
   }
   return {};
@@ -554,15 +559,15 @@ NormShape backward_for(int layout) {
 
 template <>
 NormShape norm_forward<ST_NORM_TYPE>(int dim, bool wide_sum, bool codes) {
-  const int layout = norm_layout(dim, codes);
-  if (codes) return forward_for<ST_NORM_TYPE, ST_NORM_TYPE, true>(layout);
+  if (codes) return forward_for<ST_NORM_TYPE, ST_NORM_TYPE, true>(norm_layout(dim, kCodeLayouts));
+  const int layout = norm_layout(dim);
   if (wide_sum) return forward_for<ST_NORM_TYPE, ST_SCORE_F32, false>(layout);
   return forward_for<ST_NORM_TYPE, ST_NORM_TYPE, false>(layout);
 }
 
 template <>
 NormShape norm_backward<ST_NORM_TYPE>(int dim, bool wide_sum) {
-  const int layout = norm_layout(dim, false);
+  const int layout = norm_layout(dim);
   if (wide_sum) return backward_for<ST_NORM_TYPE, ST_SCORE_F32>(layout);
   return backward_for<ST_NORM_TYPE, ST_NORM_TYPE>(layout);
 }
