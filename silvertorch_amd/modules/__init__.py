@@ -1,7 +1,7 @@
 """nn.Module surface of the bloom retrieval path, mirroring the reference's
 silvertorch.modules (bloom_index_search_module.py, filter_query_parser_module.py
 and their builders) over this build's torch.ops.st operators, and the
-retrieval head on them, which has no counterpart there."""
+retrieval head and the query tower on them, which have no counterpart there."""
 
 from silvertorch_amd.modules.bloom_index_search_module import BloomIndexSearchModule  # noqa: F401
 from silvertorch_amd.modules.bloom_index_search_module_builder import (  # noqa: F401
@@ -11,6 +11,11 @@ from silvertorch_amd.modules.filter_query_parser_module import FilterQueryParser
 from silvertorch_amd.modules.filter_query_parser_module_builder import (  # noqa: F401
     FilterQueryParserModuleBuilder,
 )
+from silvertorch_amd.modules.query_tower_module import (  # noqa: F401
+    Int8Linear,
+    PackedQueryTowerModule,
+    QueryTowerModule,
+)
 from silvertorch_amd.modules.retrieval_head_module import RetrievalHeadModule  # noqa: F401
 
 __all__ = [
@@ -18,5 +23,8 @@ __all__ = [
     "BloomIndexSearchModuleBuilder",
     "FilterQueryParserModule",
     "FilterQueryParserModuleBuilder",
+    "Int8Linear",
+    "PackedQueryTowerModule",
+    "QueryTowerModule",
     "RetrievalHeadModule",
 ]

@@ -178,3 +178,33 @@ def test_tangents_are_refused(name, requires_grad):
         dual = fwAD.make_dual(value.clone().requires_grad_(requires_grad), torch.ones_like(value))
         with pytest.raises(RuntimeError, match=f"{name.split()[0]} has no forward-mode derivative"):
             call(dual)
+
+
+def test_head_holds_an_eight_bit_table():
+    """A table of `int8_quantize`, set or loaded, keeps its types; its scales stay float32."""
+    from silvertorch_amd.modules import RetrievalHeadModule
+
+    with pytest.raises(RuntimeError, match="bits must be 4 or 8"):
+        RetrievalHeadModule(bits=3)
+    a, b = RetrievalHeadModule(bits=8), RetrievalHeadModule()
+    a.set_table(torch.ones((7, 48), dtype=torch.int8), torch.rand(7))
+    b.load_state_dict(a.state_dict())
+    assert b.packed.dtype == torch.int8 and b.packed.shape == (7, 48) and torch.equal(b.scales, a.scales)
+    want = a.scales.clone()
+    assert a.half().packed.dtype == torch.int8 and torch.equal(a.scales, want)
+    four = RetrievalHeadModule()
+    four.set_table(torch.ones((7, 16), dtype=torch.uint8), torch.rand((7, 1)), torch.full((7, 1), 8, dtype=torch.uint8))
+    assert four.half().scales.dtype == torch.float16
+
+
+def test_query_tower_state():
+    """Parameters, dropout's state among the saved buffers, one state for each place that drops."""
+    from silvertorch_amd.modules import QueryTowerModule
+
+    a, b = QueryTowerModule(5, 8, 16, layers=3, seed=7), QueryTowerModule(5, 8, 16, layers=3)
+    a.rng[1] += 12
+    b.load_state_dict(a.state_dict())
+    assert b.rng.tolist() == [7, 12] and "places" not in a.state_dict()
+    assert (b.rng + b.places).tolist() == [[7, 12], [7, 13], [7, 14], [7, 15]]
+    assert a.half().rng.dtype == torch.int64
+    assert QueryTowerModule(5, 8, 16, layers=0).places.tolist() == [[0, 0]]
