@@ -200,15 +200,20 @@ __device__ __forceinline__ void join_row(float (&x)[N], float* room, F f) {
 constexpr auto kAdd = [](float a, float b) { return a + b; };
 constexpr auto kMost = [](float a, float b) { return fmaxf(a, b); };
 
+// Whether what the mean's rounding left (2^-24 of it) counts: beside steps of
+// 16-bit values it does not.
+template <int HT>
+constexpr bool kRest = HT == ST_SCORE_F32;
+
 // HT: the type of h.  CODES: the result goes to 8 bits with a scale for each
 // row, from its 32-bit values.
 template <int DT, int HT, int L, int S, bool CODES>
 __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
   constexpr int kRows = norm_rows(L);
   // Weights stay in registers from row to row where there is room for them.
-  constexpr bool kHold = CODES ? L * S <= 2048 : S <= 2;
+  constexpr bool kHold = CODES ? L * S <= 2048 : S <= 3;
   __shared__ float room[L > 64 ? 4 * (L / 64) : 1];
-  const int lane = threadIdx.x % L;
+  const int lane = threadIdx.x % L, wave_lane = __builtin_amdgcn_readfirstlane(lane);  // of the wave's first
   const DropoutKey key = a.dropout.state ? dropout_key(a.dropout.state) : DropoutKey{};
   if (a.dropout.used && blockIdx.x == 0 && threadIdx.x < 2) a.dropout.used[threadIdx.x] = a.dropout.state[threadIdx.x];
 
@@ -283,6 +288,8 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
     const void *weight = a.weight, *bias = a.bias;
     if constexpr (!kHold) asm volatile("" : "+s"(weight), "+s"(bias));  // else the compiler holds them after all, and spills
 
+    // Whether all lanes of this wave have eight columns of the row in step s.
+    auto whole = [&](int s) { return (s * L + (L > 64 ? wave_lane + 64 : L)) * 8 <= a.dim; };
     float mean = 0.0f, rest = 0.0f, r = 1.0f;
     float total[1] = {0.0f};
 #pragma unroll
@@ -296,22 +303,29 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
     if (!CODES || a.normalise) {
       join_row<L>(total, room, kAdd);
       mean = __fdiv_rn(total[0], static_cast<float>(a.dim));
-      // what the mean's rounding left, and the squares about the rounded one
-      float left[2] = {0.0f, 0.0f};
+      // the squares about the rounded mean, and what its rounding left
+      float left[kRest<HT> ? 2 : 1] = {};
 #pragma unroll
       for (int s = 0; s < S; ++s) {
 #pragma unroll
+        for (int i = 0; i < 8; ++i) h[s][i] -= mean;
+        if (!whole(s))
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[s][i] = (s * L + lane) * 8 + i < a.dim ? h[s][i] : 0.0f;
+#pragma unroll
         for (int i = 0; i < 8; ++i) {
-          h[s][i] = (s * L + lane) * 8 + i < a.dim ? h[s][i] - mean : 0.0f;
-          left[0] += h[s][i];
-          left[1] = fmaf(h[s][i], h[s][i], left[1]);
+          left[0] = fmaf(h[s][i], h[s][i], left[0]);
+          if constexpr (kRest<HT>) left[1] += h[s][i];
         }
       }
       join_row<L>(left, room + (L > 64 ? L / 64 : 0), kAdd);
-      rest = __fdiv_rn(left[0], static_cast<float>(a.dim));
-      // a maximum with 0 would turn NaN into it
-      float squares = fmaf(-rest, left[0], left[1]);
-      squares = squares < 0.0f ? 0.0f : squares;
+      float squares = left[0];
+      if constexpr (kRest<HT>) {
+        rest = __fdiv_rn(left[1], static_cast<float>(a.dim));
+        // a maximum with 0 would turn NaN into it
+        squares = fmaf(-rest, left[1], squares);
+        squares = squares < 0.0f ? 0.0f : squares;
+      }
       r = __fdiv_rn(1.0f, __fsqrt_rn(fmaf(squares, 1.0f / static_cast<float>(a.dim), a.eps)));
       if (a.stats && live && lane == 0) {
         a.stats[kNormStats * row] = mean;
@@ -324,7 +338,10 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
       if (CODES && !a.normalise) return;
       if constexpr (!kHold) load_weights(weight, bias, s, w[0], b[0]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmaf((v[i] - rest) * r, w[kHold ? s : 0][i], b[kHold ? s : 0][i]);
+      for (int i = 0; i < 8; ++i) {
+        const float n = kRest<HT> ? fmaf(v[i], r, -rest * r) : v[i] * r;
+        v[i] = fmaf(n, w[kHold ? s : 0][i], b[kHold ? s : 0][i]);
+      }
     };
     if constexpr (!CODES) {
       char* y = static_cast<char*>(a.y) + row * a.dim * kScoreBytes<DT>;
@@ -339,9 +356,11 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         result(s, h[s]);
+        if (!whole(s))
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[s][i] = (s * L + lane) * 8 + i < a.dim ? h[s][i] : 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if ((s * L + lane) * 8 + i >= a.dim) h[s][i] = 0.0f;
           most[0] = fmaxf(most[0], fabsf(h[s][i]));
           odd = fmaf(h[s][i], 0.0f, odd);
         }
@@ -371,10 +390,10 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
 template <int DT, int HT, int L, int S>
 __global__ __launch_bounds__(norm_threads(L), norm_backward_waves(L, S)) void norm_backward_kernel(NormBackwardArgs a) {
   constexpr int kRows = norm_rows(L);
-  constexpr bool kHold = S <= 2, kSums = L * S <= 2048, kNext = L * S <= 1024;
+  constexpr bool kHold = S <= 3, kSums = L * S <= 2048, kNext = L * S <= 1024;
   __shared__ float room[L > 64 ? 4 * (L / 64) : 1];
   __shared__ float joined[L <= 64 ? 256 * 8 : 1];
-  const int lane = threadIdx.x % L;
+  const int lane = threadIdx.x % L, wave_lane = __builtin_amdgcn_readfirstlane(lane);  // of the wave's first
   const DropoutKey key = a.dropout.state ? dropout_key(a.dropout.state) : DropoutKey{};
 
   float w[kHold ? S : 1][8], gw[kSums ? S : 1][8], gb[kSums ? S : 1][8];
@@ -432,12 +451,19 @@ __global__ __launch_bounds__(norm_threads(L), norm_backward_waves(L, S)) void no
     for (int s = 0; s < S; ++s) {
       if constexpr (!kHold) load_weights(weight, s, w[0]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        n[s][i] = (s * L + lane) * 8 + i < a.dim ? ((n[s][i] - mean) - rest) * r : 0.0f;
-        if (kSums && live) {
+      for (int i = 0; i < 8; ++i) n[s][i] = kRest<HT> ? ((n[s][i] - mean) - rest) * r : fmaf(n[s][i], r, -mean * r);
+      if ((s * L + (L > 64 ? wave_lane + 64 : L)) * 8 > a.dim)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n[s][i] = (s * L + lane) * 8 + i < a.dim ? n[s][i] : 0.0f;
+      if (kSums && live) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
           gw[kSums ? s : 0][i] = fmaf(g[s][i], n[s][i], gw[kSums ? s : 0][i]);
           gb[kSums ? s : 0][i] += g[s][i];
         }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
         g[s][i] *= w[kHold ? s : 0][i];
         sums[0] += g[s][i];
         sums[1] = fmaf(g[s][i], n[s][i], sums[1]);
@@ -450,7 +476,7 @@ __global__ __launch_bounds__(norm_threads(L), norm_backward_waves(L, S)) void no
     for (int s = 0; s < S; ++s) {
       const int col = (s * L + lane) * 8;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[s][i] = r * ((g[s][i] - mean_g) - n[s][i] * mean_gn);
+      for (int i = 0; i < 8; ++i) g[s][i] = fmaf(n[s][i], -mean_gn * r, fmaf(g[s][i], r, -mean_g * r));
       if (a.gsum) {
         float more[8];
         load_columns<HT>(static_cast<const char*>(a.gsum) + row * a.dim * kScoreBytes<HT>, col, a.dim, more);
@@ -515,7 +541,7 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(NormBackwardArgs a) {
     const float mean = a.stats[kNormStats * row], rest = a.stats[kNormStats * row + 1], r = a.stats[kNormStats * row + 2];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      gw[i] = fmaf(g[i], ((h[i] - mean) - rest) * r, gw[i]);
+      gw[i] = fmaf(g[i], kRest<HT> ? ((h[i] - mean) - rest) * r : fmaf(h[i], r, -mean * r), gw[i]);
       gb[i] += g[i];
     }
   }

@@ -104,6 +104,25 @@ __device__ __forceinline__ void store_score(void* row, int64_t col, float f) {
     static_cast<uint16_t*>(row)[col] = static_cast<uint16_t>(score_bits<DT>(f));
 }
 
+typedef float float2_t __attribute__((ext_vector_type(2)));
+
+// Two scores, each rounded once, the first in the low half (DT: a 16-bit type).
+template <int DT>
+__device__ __forceinline__ uint32_t score_bits2(float a, float b) {
+  const float2_t f = {a, b};
+  uint32_t u;
+  if constexpr (DT == ST_SCORE_F16) {
+    typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+    const half2_t h = __builtin_convertvector(f, half2_t);
+    __builtin_memcpy(&u, &h, 4);
+  } else {
+    typedef __bf16 bfloat2_t __attribute__((ext_vector_type(2)));
+    const bfloat2_t h = __builtin_convertvector(f, bfloat2_t);
+    __builtin_memcpy(&u, &h, 4);
+  }
+  return u;
+}
+
 template <int DT>
 __device__ __forceinline__ void store8(void* row, int64_t col, const float v[8]) {
   if constexpr (DT == ST_SCORE_F32) {
@@ -118,7 +137,7 @@ __device__ __forceinline__ void store8(void* row, int64_t col, const float v[8])
   } else {
     u32x4_by2 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = score_bits<DT>(v[2 * i]) | (score_bits<DT>(v[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) w[i] = score_bits2<DT>(v[2 * i], v[2 * i + 1]);
     *reinterpret_cast<u32x4_by2*>(static_cast<uint16_t*>(row) + col) = w;
   }
 }
