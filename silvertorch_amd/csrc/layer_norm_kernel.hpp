@@ -8,10 +8,10 @@
 //
 // A row lies in registers from its one read on, 8 columns a lane and step: the
 // mean first, then what its rounding left and the squares of what is apart from
-// it, so that rows far from 0 lose no digits.  Rows of up
-// to 512 columns take 8 to 64 lanes of a wave, longer ones a wave, then a
-// workgroup, with the fewest steps (S) that hold them.  HBM bounds both
-// directions.
+// it, so that rows far from 0 lose no digits.  HBM bounds both directions: 100
+// million bfloat16 elements take 67 to 72 us forward and 120 to 130 us backward in
+// rows of 128 to 16,384 columns (5.6 to 6.0 and 4.6 to 5.0 TB/s); rows of 16-bit
+// types whose start is at odd multiples of 8 bytes or less, up to twice that.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -49,13 +49,16 @@ struct NormBackwardArgs {
   DropoutArgs dropout;
 };
 
-// Lanes of a row and steps of 8 columns a lane: the first that holds a row.
+// Lanes of a row and steps of 8 columns a lane: the first that holds a row.  Two or
+// three steps: what a row costs besides its columns is shared by more of them, and a
+// wave has more rows under way (one step, 500,000 x 200 bfloat16: 107 and 165 us
+// forward and backward, with two 82 and 136).
 struct NormLayout {
   int lanes, steps;
 };
-constexpr NormLayout kNormLayouts[] = {{1, 1},  {2, 1},  {4, 1},   {8, 1},   {16, 1},  {8, 3},   {32, 1},  {16, 3},   {64, 1},
-                                       {32, 3}, {64, 2}, {64, 3},  {256, 1}, {128, 3}, {256, 2}, {256, 3}, {512, 2}, {512, 3},
-                                       {1024, 2}, {1024, 4}};
+constexpr NormLayout kNormLayouts[] = {{1, 1},   {1, 2},   {1, 3},   {2, 2},   {2, 3},   {4, 2},   {4, 3},  {8, 2},
+                                       {8, 3},   {16, 2},  {16, 3},  {32, 2},  {32, 3},  {64, 2},  {64, 3}, {128, 2},
+                                       {128, 3}, {256, 2}, {256, 3}, {512, 2}, {512, 3}, {1024, 2}, {1024, 4}};
 // Where codes are the result, instructions bound it, a good part of them the same
 // for any number of columns a lane has: 16,384 x 4,096 with 256 lanes 62 us.
 constexpr NormLayout kCodeLayouts[] = {{2, 1},  {4, 1},  {8, 1},   {16, 1},  {16, 2}, {16, 4},
