@@ -18,6 +18,7 @@ result's type; A = max |h| of a row, r = 1 / sqrt(var + eps)):
 """
 
 import math
+import threading
 
 import pytest
 import torch
@@ -311,6 +312,51 @@ def test_dropout_add_layer_norm(rows, dim, dtype, residual_type):
         grads = torch.autograd.grad([y, total], leaves, [gy.cuda(), gs.cuda()])
         assert [g.dtype for g in grads] == [dtype, residual_type, torch.float32, torch.float32]
         _check_gradients(held, w.double(), gy, gs, grads, (gx, gh, gw, gb), 1e-5, p, state)
+
+
+@pytest.mark.parametrize("dtype,residual_type", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                                 (torch.float16, torch.float32)])
+@pytest.mark.parametrize("dim", [10, 16, 20, 24, 30, 32, 41, 48, 90, 96, 180, 370, 384, 750, 768, 1500, 1536, 6000, 12_000])
+def test_dropout_add_layer_norm_of_whole_and_ragged_rows(dim, dtype, residual_type):
+    """Lanes whose last step of columns is whole, in part or empty, in workgroups of many rows and of one."""
+    test_dropout_add_layer_norm(37, dim, dtype, residual_type)
+
+
+def test_two_threads_at_once():
+    """Passes of two threads on streams of their own give the bits that they give alone."""
+    H.note("[tower] two threads")
+    w = _data((900,), torch.float32, 3, 0.2, 1.0).cuda()
+    table, scales, _ = (t.cuda() for t in _table(700, 900, 1))
+
+    def step(seed):
+        x, res = (_data((400, 900), torch.bfloat16, seed + i).cuda().requires_grad_() for i in range(2))
+        own = w.clone().requires_grad_()
+        y, total = st.dropout_add_layer_norm(x, res, own, None, 0.2, _state(seed).cuda())
+        grads = torch.autograd.grad([y, total], [x, res, own], [x.detach(), res.detach()])
+        return [y.detach(), total.detach(), *grads, st.int8_matmul(table, scales, x.detach()),
+                st.int8_matmul(table, scales, x.detach()[:2])]
+
+    alone = [[step(10 * k + i) for i in range(4)] for k in range(2)]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[k] = [step(10 * k + i) for i in range(4)]
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for a, b in zip(alone, got):
+        for c, d in zip(a, b):
+            assert all(torch.equal(p, q) for p, q in zip(c, d))
 
 
 def test_dropout_add_layer_norm_forms():
