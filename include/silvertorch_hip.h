@@ -660,9 +660,10 @@ int st_layer_norm_int8(const void* x, int x_type, int64_t rows, int64_t dim, int
  * largest magnitude is below 2^-119 has scale 0; one with a value that is not
  * finite has codes 0 and scale NaN.
  *
- * st_int8_matmul: y [tokens, rows] (y_type) = x_scales[m] * scales[n] * sum_k
- * x[m, k] codes[n, k] + bias[n] (bias: float32 or null).  The sum is exact, the
- * rest in 32 bits, rounded once.  x [tokens, dim] of floats (rows x_stride apart)
+ * st_int8_matmul: y [tokens, rows] (y_type) = (sum_k x[m, k] codes[n, k] *
+ * x_scales[m]) * scales[n] + bias[n] (bias: float32 or null).  The sum is exact,
+ * the rest in 32 bits, rounded to y's type once: vectors of magnitudes up to 2^121 /
+ * columns pass no 32-bit number on the way.  x [tokens, dim] of floats (rows x_stride apart)
  * is held as st_int8_quantize would hold it, with x_scales null; codes
  * (ST_CODE_I8, dim = columns = x_stride) come with x_scales [tokens].  columns, a
  * multiple of 16, is at most 2^17 - 16, whatever the codes (-128 among them).

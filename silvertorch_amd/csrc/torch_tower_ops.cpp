@@ -41,9 +41,14 @@ Tensor as_rows(const Tensor& t) {
   return t.contiguous().view({t.numel() / columns, columns});
 }
 
-// A gradient of t's shape as the kernels take it.
+// `t` on d; what is there already does not go through the dispatcher, which counts
+// where a pass is a few launches.
+Tensor placed(const Tensor& t, at::Device d) { return !t.defined() || t.device() == d ? t : t.to(d); }
+
+// A gradient as the kernels take it.
 Tensor grad_rows(const Tensor& g, at::ScalarType type, at::Device d) {
-  return g.defined() ? g.to(d, type).contiguous() : g;
+  const Tensor t = placed(g, d);
+  return !t.defined() || (t.scalar_type() == type && t.is_contiguous()) ? t : t.to(type).contiguous();
 }
 
 Tensor back(const Tensor& t, bool on_gpu) { return t.defined() && !on_gpu ? t.cpu() : t; }
@@ -224,12 +229,11 @@ NormGrads norm_gradients(const Tensor& h_in, at::ScalarType y_type, const Tensor
   const bool on_gpu = h_in.is_cuda();
   const at::Device dev = on_gpu ? h_in.device() : gpu_for_cpu_call();
   c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
-  const Tensor h = as_rows(h_in.to(dev)), stats = stats_in.to(dev);
+  const Tensor h = as_rows(placed(h_in, dev)), stats = placed(stats_in, dev), used = placed(used_in, dev);
   const int64_t rows = h.size(0), dim = h.size(1);
   const auto options = h.options();
-  Tensor weight, used;
-  if (weight_in.defined()) weight = weight_in.to(dev).contiguous();
-  if (used_in.defined()) used = used_in.to(dev);
+  Tensor weight;
+  if (weight_in.defined()) weight = placed(weight_in, dev).contiguous();
   // without a gradient of its own the norm's result has one of zeros
   const Tensor gy = grad_y.defined() ? grad_rows(grad_y, y_type, dev) : at::zeros(h_in.sizes(), options.dtype(y_type));
   const Tensor gsum = grad_rows(grad_sum, h.scalar_type(), dev);
