@@ -656,10 +656,14 @@ bool is_fused(int x_type, int64_t tokens, int64_t rows, int64_t columns) {
 // tiles of 32 x 128), 40 x 1,024 x 8,192 5.6 (6.4), 16 x 512 x 8,192 4.0 (4.1); but 96 x
 // 8,192 x 8,192 47 (36.5), 32 x 512 x 16,384 5.8 (4.6).
 //
-// Else the largest tile that the vectors fill, as long as there are tiles for most
-// of the chip: 200 x 128 x 500,000 in tiles of 256 x 256, 128 x 128, 64 x 128 and 32 x 128
-// 56, 65, 79 and 91 us; 64 x 2,048 x 50,000 29, 20.5, 18 and 26; 512 x 512 x 4,096 12.8,
-// 7.1, 5.8 and 5.7; one vector x 128 x 20,000,000 868, 669, 632 and 573.
+// Else the tile whose rounds over the chip take least: `full` with as many
+// workgroups as it holds, `first` for less than one a CU and nothing before, `last` for
+// that after full rounds (two a CU of three: `two`), in hundredths of a round of
+// 256 x 256.  In tiles of 256 x 256, 128 x 128, 64 x 128 and 32 x 128: 200 x 128 x 500,000
+// 56, 65, 79 and 91 us; 64 x 2,048 x 50,000 29, 20.5, 18 and 26; 4,097 x 4,096 x 4,096 100,
+// 85, 107 and 130; 2,048 x 4,096 x 4,096 53, 40, 48 and 66; 300 x 4,096 x 4,096 47, 22, 17
+// and 20; 512 x 512 x 4,096 12.3, 7.0, 5.7 and 5.7; one vector x 128 x 20,000,000 868,
+// 669, 632 and 573.
 void launch_codes_product(const MatmulArgs& a, hipStream_t s) {
   const int64_t cus = cu_count();
   auto tiles = [&](int64_t tokens, int64_t rows) { return ((a.tokens + tokens - 1) / tokens) * ((a.rows + rows - 1) / rows); };
@@ -669,15 +673,23 @@ void launch_codes_product(const MatmulArgs& a, hipStream_t s) {
       launch_long<1>(a, s);
     else
       launch_long<2>(a, s);
-  } else if (a.tokens > 128 && tiles(256, 256) >= cus * 3 / 4) {
-    launch_many<128, 64, 2, 4>(a, s);
-  } else if (a.tokens > 64 && tiles(128, 128) >= cus) {
-    launch_many<64, 64, 2, 2>(a, s);
-  } else if (a.tokens > 32 && tiles(64, 128) >= cus) {
-    launch_many<64, 32, 1, 4>(a, s);
-  } else {
-    launch_many<32, 32, 1, 4>(a, s);
+    return;
   }
+  auto cost = [&](int64_t count, int per_cu, int full, int first, int last, int two) {
+    const int64_t rounds = count / (per_cu * cus), rest = count % (per_cu * cus);
+    return rounds * full + (rest == 0 ? 0 : rest > 2 * cus ? full : rest > cus ? two : rounds == 0 ? first : last);
+  };
+  const int64_t of_256 = cost(tiles(256, 256), 1, 100, 100, 100, 100), of_128 = cost(tiles(128, 128), 2, 70, 50, 30, 70);
+  const int64_t of_64 = cost(tiles(64, 128), 2, 46, 35, 33, 46), of_32 = cost(tiles(32, 128), 3, 48, 28, 28, 42);
+  const int64_t least = std::min(std::min(of_256, of_128), std::min(of_64, of_32));
+  if (of_256 == least)
+    launch_many<128, 64, 2, 4>(a, s);
+  else if (of_128 == least)
+    launch_many<64, 64, 2, 2>(a, s);
+  else if (of_64 == least)
+    launch_many<64, 32, 1, 4>(a, s);
+  else
+    launch_many<32, 32, 1, 4>(a, s);
 }
 
 void check_codes(int64_t rows, int64_t columns) {

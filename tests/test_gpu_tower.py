@@ -498,6 +498,16 @@ def test_int8_matmul_large(tokens, rows, dim):
     _check_matmul(table, scales, *O.codes(x), bias, torch.float32, x.cuda())
 
 
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("tokens,rows,dim", [(300, 20_001, 64), (1100, 9001, 80), (700, 30_001, 128), (64, 40_000, 72), (2000, 1001, 48),
+                                             (257, 33_000, 200)])
+def test_int8_matmul_tiles(tokens, rows, dim, out):
+    """Tiles of every size, in one round over the chip and in several, the last one in part."""
+    H.note(f"[tower] int8_matmul {tokens} x {dim} x {rows} {out}")
+    table, scales, bias = _table(rows, dim, 1)
+    _check_matmul(table, scales, *O.codes(_data((tokens, dim), torch.float32, 2)), bias, out)
+
+
 @pytest.mark.parametrize("tokens", [1, 20, 100])
 def test_int8_matmul_extremes(tokens):
     """The longest rows with every code -128: sums of 2^31 - 2^18; mixed ones; no reads past a table's end."""
