@@ -16,6 +16,16 @@ struct CodeScale {
   float scale, times;
 };
 
+// max(most, |v|), NaN if there is one: one instruction for two values.
+__device__ __forceinline__ float most_of8(float most, const float v[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = __builtin_elementwise_maximum(most, fabsf(v[i]));
+  return most;
+}
+
+// Infinity for NaN, which the maximum over lanes would pass by.
+__device__ __forceinline__ float most_or_infinity(float most) { return most < __builtin_inff() ? most : __builtin_inff(); }
+
 // `most`: max |x|, infinite where a value is not finite.
 __device__ __forceinline__ CodeScale code_scale(float most) {
   if (most == __builtin_inff()) return {__builtin_nanf(""), 0.0f};

@@ -69,16 +69,12 @@ __device__ __forceinline__ void load_eight(const void* row, int col, int dim, fl
 template <int DT>
 __device__ __forceinline__ float codes_to_lds(const void* row, int dim, int padded, uint8_t* to) {
   const int lane = threadIdx.x % 64;
-  float most = 0.0f, odd = 0.0f, v[8];
+  float most = 0.0f, v[8];
   for (int col = lane * 8; col < dim; col += 512) {
     load_eight<DT>(row, col, dim, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      most = fmaxf(most, fabsf(v[i]));
-      odd = fmaf(v[i], 0.0f, odd);
-    }
+    most = most_of8(most, v);
   }
-  const CodeScale c = code_scale(wave_max(odd != odd ? __builtin_inff() : most));
+  const CodeScale c = code_scale(wave_max(most_or_infinity(most)));
   for (int col = lane * 8; col < padded; col += 512) {
     load_eight<DT>(row, col, dim, v);
     *reinterpret_cast<uint64_t*>(to + (col >> 6) * 1024 + ((col >> 4) & 3) * 256 + (col & 15)) = codes8(v, c);
@@ -715,16 +711,12 @@ __global__ __launch_bounds__(1024) void long_codes_kernel(const void* x, int64_t
                                                           float* scales) {
   __shared__ float room[16];
   const char* row = static_cast<const char*>(x) + blockIdx.x * x_stride * kScoreBytes<DT>;
-  float most = 0.0f, odd = 0.0f, v[8];
+  float most = 0.0f, v[8];
   for (int col = threadIdx.x * 8; col < dim; col += 8192) {
     load_eight<DT>(row, col, dim, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      most = fmaxf(most, fabsf(v[i]));
-      odd = fmaf(v[i], 0.0f, odd);
-    }
+    most = most_of8(most, v);
   }
-  most = wave_max(odd != odd ? __builtin_inff() : most);
+  most = wave_max(most_or_infinity(most));
   if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = most;
   __syncthreads();
 #pragma unroll

@@ -355,20 +355,15 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
       }
     } else {
       float most[1] = {0.0f};
-      float odd = 0.0f;  // NaN if there is one, or an infinity, in the row
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         result(s, h[s]);
         if (!whole(s))
 #pragma unroll
           for (int i = 0; i < 8; ++i) h[s][i] = (s * L + lane) * 8 + i < a.dim ? h[s][i] : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          most[0] = fmaxf(most[0], fabsf(h[s][i]));
-          odd = fmaf(h[s][i], 0.0f, odd);
-        }
+        most[0] = most_of8(most[0], h[s]);
       }
-      if (odd != odd) most[0] = __builtin_inff();
+      most[0] = most_or_infinity(most[0]);
       join_row<L>(most, room + (L > 64 ? 3 * (L / 64) : 0), kMost);
       const CodeScale c = code_scale(most[0]);
       if (live && lane == 0) a.scales[row] = c.scale;
