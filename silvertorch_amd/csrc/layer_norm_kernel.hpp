@@ -9,9 +9,9 @@
 // A row lies in registers from its one read on, 8 columns a lane and step: the
 // mean first, then what its rounding left and the squares of what is apart from
 // it, so that rows far from 0 lose no digits.  HBM bounds both directions: 100
-// million bfloat16 elements take 67 to 72 us forward and 120 to 130 us backward in
-// rows of 128 to 16,384 columns (5.6 to 6.0 and 4.6 to 5.0 TB/s); rows of 16-bit
-// types whose start is at odd multiples of 8 bytes or less, up to twice that.
+// million bfloat16 elements take 76 to 88 us forward and 118 to 136 us backward in
+// rows of 64 to 16,384 columns, odd lengths among them, but 105 and 145 in rows of 24
+// and 110 and 235 in rows of 32,768 (all without a warm cache).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -51,8 +51,8 @@ struct NormBackwardArgs {
 
 // Lanes of a row and steps of 8 columns a lane: the first that holds a row.  Two or
 // three steps: what a row costs besides its columns is shared by more of them, and a
-// wave has more rows under way (one step, 500,000 x 200 bfloat16: 107 and 165 us
-// forward and backward, with two 82 and 136).
+// wave has more rows under way (500,000 x 200 bfloat16 in one step 107 and 165 us
+// forward and backward, in two 83 and 120).
 struct NormLayout {
   int lanes, steps;
 };
@@ -116,11 +116,18 @@ __device__ __forceinline__ float load_typed(const void* p, int64_t i, int type) 
   return load_score<ST_SCORE_BF16>(p, i);
 }
 
-// Columns [col, col + 8) of a row as they are stored; 0 past its end.
-template <int DT>
+// Columns [col, col + 8) of a row as they are stored; 0 past its end.  LAST: where
+// the row ends inside, its last eight for `settle`, one load; put together one by one,
+// those of 16-bit types had to be waited for before their row was due (20,000 x 5,004
+// bfloat16 104 and 210 us forward and backward, so 77 and 121).
+template <int DT, bool LAST = false>
 __device__ __forceinline__ Raw8<DT> load_raw_columns(const void* row, int col, int dim) {
-  if (col + 8 <= dim) return load_raw8<DT>(row, col);
   Raw8<DT> r{};
+  if constexpr (LAST) {
+    if (col < dim) r = load_raw8<DT>(row, min(col, dim - 8));
+    return r;
+  }
+  if (col + 8 <= dim) return load_raw8<DT>(row, col);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if (col + i >= dim) continue;
@@ -131,6 +138,26 @@ __device__ __forceinline__ Raw8<DT> load_raw_columns(const void* row, int col, i
   }
   return r;
 }
+
+// What load_raw_columns gave, in its place.
+template <int DT, bool LAST>
+__device__ __forceinline__ void settle(Raw8<DT>& r, int col, int dim) {
+  if constexpr (!LAST) return;
+  if (col <= dim - 8) return;
+  const int shift = -dim & 7;
+  u32x4& w = r.w[0];
+  if (shift & 4) w = u32x4{w[2], w[3], 0, 0};
+  if (shift & 2) w = u32x4{w[1], w[2], w[3], 0};
+  if (shift & 1)
+    w = u32x4{__builtin_amdgcn_alignbit(w[1], w[0], 16), __builtin_amdgcn_alignbit(w[2], w[1], 16),
+              __builtin_amdgcn_alignbit(w[3], w[2], 16), w[3] >> 16};
+}
+
+// Whether rows of type DT are loaded so by L lanes in S steps: where they have eight
+// columns (layouts of more than 16), and registers have room for it (not float32's
+// nor those of 1,024 lanes).
+template <int DT, int L, int S>
+constexpr bool kLast = DT != ST_SCORE_F32 && L * S > 2 && L != 1024;
 
 template <int DT>
 __device__ __forceinline__ void load_columns(const void* row, int col, int dim, float v[8]) {
@@ -146,14 +173,26 @@ __device__ __forceinline__ void load_columns_typed(const void* row, int col, int
     load_columns<ST_SCORE_BF16>(row, col, dim, v);
 }
 
+typedef uint32_t u32x2_by2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32_by2 __attribute__((aligned(2)));
+
 template <int DT>
 __device__ __forceinline__ void store_columns(void* row, int col, int dim, const float v[8]) {
   if (col + 8 <= dim) {
     store8<DT>(row, col, v);
-  } else {
+  } else if constexpr (DT == ST_SCORE_F32) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (col + i < dim) store_score<DT>(row, col + i, v[i]);
+  } else if (col < dim) {
+    // four, two and one of the last columns
+    const int left = dim & 7;
+    const auto pick = [](bool b, float x, float y) { return b ? x : y; };  // by value: an array indexed goes to memory
+    uint16_t* to = static_cast<uint16_t*>(row) + col;
+    if (left & 4) *reinterpret_cast<u32x2_by2*>(to) = u32x2_by2{score_bits2<DT>(v[0], v[1]), score_bits2<DT>(v[2], v[3])};
+    if (left & 2) *reinterpret_cast<u32_by2*>(to + (left & 4)) = score_bits2<DT>(pick(left & 4, v[4], v[0]), pick(left & 4, v[5], v[1]));
+    if (left & 1)
+      store_score<DT>(to, left & 6, pick(left & 4, pick(left & 2, v[6], v[4]), pick(left & 2, v[2], v[0])));
   }
 }
 
@@ -253,12 +292,12 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
     const int64_t row = min(base + within, a.rows - 1);
     const char* x = static_cast<const char*>(a.x) + row * a.x_stride * kScoreBytes<DT>;
 #pragma unroll
-    for (int s = 0; s < S; ++s) next_x[s] = load_raw_columns<DT>(x, (s * L + lane) * 8, a.dim);
+    for (int s = 0; s < S; ++s) next_x[s] = load_raw_columns<DT, kLast<DT, L, S>>(x, (s * L + lane) * 8, a.dim);
     if constexpr (!CODES) {
       if (a.residual) {
         const char* residual = static_cast<const char*>(a.residual) + row * a.residual_stride * kScoreBytes<HT>;
 #pragma unroll
-        for (int s = 0; s < S; ++s) next_residual[s] = load_raw_columns<HT>(residual, (s * L + lane) * 8, a.dim);
+        for (int s = 0; s < S; ++s) next_residual[s] = load_raw_columns<HT, kLast<HT, L, S>>(residual, (s * L + lane) * 8, a.dim);
       }
     }
   };
@@ -269,13 +308,17 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
     const int64_t row = live ? at : a.rows - 1;
     if constexpr (!kNext) fetch(base);
     char* sum = static_cast<char*>(a.sum) + row * a.dim * kScoreBytes<HT>;
+    // Whether all lanes of this wave have eight columns of the row in step s.
+    auto whole = [&](int s) { return (s * L + (L > 64 ? wave_lane + 64 : L)) * 8 <= a.dim; };
     float h[S][8];
     // h of step s
     auto values = [&](int s, float (&v)[8]) {
       const int col = (s * L + lane) * 8;
+      if (!whole(s)) settle<DT, kLast<DT, L, S>>(next_x[s], col, a.dim);
       unpack8<DT>(next_x[s], v);
       if constexpr (!CODES) {
         if (!a.residual) return;
+        if (!whole(s)) settle<HT, kLast<HT, L, S>>(next_residual[s], col, a.dim);
         float more[8];
         unpack8<HT>(next_residual[s], more);
         uint32_t keeps = 0xFF;
@@ -291,8 +334,6 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
     const void *weight = a.weight, *bias = a.bias;
     if constexpr (!kHold) asm volatile("" : "+s"(weight), "+s"(bias));  // else the compiler holds them after all, and spills
 
-    // Whether all lanes of this wave have eight columns of the row in step s.
-    auto whole = [&](int s) { return (s * L + (L > 64 ? wave_lane + 64 : L)) * 8 <= a.dim; };
     float mean = 0.0f, rest = 0.0f, r = 1.0f;
     float total[1] = {0.0f};
 #pragma unroll
@@ -423,10 +464,12 @@ __global__ __launch_bounds__(norm_threads(L), norm_backward_waves(L, S)) void no
     const char* hs = static_cast<const char*>(a.h) + row * a.h_stride * kScoreBytes<HT>;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      next_g[s] = load_raw_columns<DT>(gy, (s * L + lane) * 8, a.dim);
-      next_h[s] = load_raw_columns<HT>(hs, (s * L + lane) * 8, a.dim);
+      next_g[s] = load_raw_columns<DT, kLast<DT, L, S>>(gy, (s * L + lane) * 8, a.dim);
+      next_h[s] = load_raw_columns<HT, kLast<HT, L, S>>(hs, (s * L + lane) * 8, a.dim);
     }
   };
+  // as in norm_kernel
+  auto whole = [&](int s) { return (s * L + (L > 64 ? wave_lane + 64 : L)) * 8 <= a.dim; };
   int turn = 0;
   if constexpr (kNext) fetch(first);
   for (int64_t base = first; base < a.rows; base += step, turn ^= 1) {
@@ -438,6 +481,10 @@ __global__ __launch_bounds__(norm_threads(L), norm_backward_waves(L, S)) void no
     float g[S][8], n[S][8];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
+      if (!whole(s)) {
+        settle<DT, kLast<DT, L, S>>(next_g[s], (s * L + lane) * 8, a.dim);
+        settle<HT, kLast<HT, L, S>>(next_h[s], (s * L + lane) * 8, a.dim);
+      }
       unpack8<DT>(next_g[s], g[s]);
       unpack8<HT>(next_h[s], n[s]);
     }
@@ -450,7 +497,7 @@ __global__ __launch_bounds__(norm_threads(L), norm_backward_waves(L, S)) void no
       if constexpr (!kHold) load_weights(weight, s, w[0]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) n[s][i] = kRest<HT> ? ((n[s][i] - mean) - rest) * r : fmaf(n[s][i], r, -mean * r);
-      if ((s * L + (L > 64 ? wave_lane + 64 : L)) * 8 > a.dim)
+      if (!whole(s))
 #pragma unroll
         for (int i = 0; i < 8; ++i) n[s][i] = (s * L + lane) * 8 + i < a.dim ? n[s][i] : 0.0f;
       if (kSums && live) {
