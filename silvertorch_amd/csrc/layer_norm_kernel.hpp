@@ -11,7 +11,7 @@
 // it, so that rows far from 0 lose no digits.  HBM bounds both directions: 100
 // million bfloat16 elements take 76 to 88 us forward and 118 to 136 us backward in
 // rows of 64 to 16,384 columns, odd lengths among them, but 105 and 145 in rows of 24
-// and 110 and 235 in rows of 32,768 (all without a warm cache).
+// and 97 to 136 and 214 to 260 in longer ones (all without a warm cache).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -58,7 +58,7 @@ struct NormLayout {
 };
 constexpr NormLayout kNormLayouts[] = {{1, 1},   {1, 2},   {1, 3},   {2, 2},   {2, 3},   {4, 2},   {4, 3},  {8, 2},
                                        {8, 3},   {16, 2},  {16, 3},  {32, 2},  {32, 3},  {64, 2},  {64, 3}, {128, 2},
-                                       {128, 3}, {256, 2}, {256, 3}, {512, 2}, {512, 3}, {1024, 2}, {1024, 4}};
+                                       {128, 3}, {256, 2}, {256, 3}, {512, 2}, {512, 3}, {1024, 2}, {1024, 3}, {1024, 4}};
 // Where codes are the result, instructions bound it, a good part of them the same
 // for any number of columns a lane has: 16,384 x 4,096 with 256 lanes 62 us.
 constexpr NormLayout kCodeLayouts[] = {{2, 1},  {4, 1},  {8, 1},   {16, 1},  {16, 2}, {16, 4},
@@ -154,10 +154,11 @@ __device__ __forceinline__ void settle(Raw8<DT>& r, int col, int dim) {
 }
 
 // Whether rows of type DT are loaded so by L lanes in S steps: where they have eight
-// columns (layouts of more than 16), and registers have room for it (not float32's
-// nor those of 1,024 lanes).
+// columns (layouts of more than 16), and registers have room for it (not float32's;
+// 1,024 lanes in three steps, 4,999 x 20,001 151 and 267 us, so 136 and 259, but in
+// two or four they spill: 6,103 x 16,384 backward 124 us, so 175).
 template <int DT, int L, int S>
-constexpr bool kLast = DT != ST_SCORE_F32 && L * S > 2 && L != 1024;
+constexpr bool kLast = DT != ST_SCORE_F32 && L * S > 2 && (L != 1024 || S == 3);
 
 template <int DT>
 __device__ __forceinline__ void load_columns(const void* row, int col, int dim, float v[8]) {
@@ -253,7 +254,7 @@ template <int DT, int HT, int L, int S, bool CODES>
 __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
   constexpr int kRows = norm_rows(L);
   // Weights stay in registers from row to row where there is room for them.
-  constexpr bool kHold = CODES ? L * S <= 2048 : S <= 3;
+  constexpr bool kHold = L * S <= 2048 && (CODES || S <= 3);
   __shared__ float room[L > 64 ? 4 * (L / 64) : 1];
   const int lane = threadIdx.x % L, wave_lane = __builtin_amdgcn_readfirstlane(lane);  // of the wave's first
   const DropoutKey key = a.dropout.state ? dropout_key(a.dropout.state) : DropoutKey{};
@@ -280,8 +281,8 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
 
   // A wave's rows go through the loop together; what a lane of a row past the
   // last computes is not stored.  The next row is on its way while one is worked on,
-  // where there are registers for it.
-  constexpr bool kNext = L * S <= 2048;
+  // where there are registers for it (3,051 x 32,768 111 us without, 97 with).
+  constexpr bool kNext = L * S <= 2048 || (HT != ST_SCORE_F32 && !CODES);
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / (L < 64 ? 64 : L) * (L < 64 ? 64 / L : 1);
   const int within = L < 64 ? threadIdx.x % 64 / L : 0;
