@@ -155,10 +155,11 @@ __device__ __forceinline__ void settle(Raw8<DT>& r, int col, int dim) {
 
 // Whether rows of type DT are loaded so by L lanes in S steps: where they have eight
 // columns (layouts of more than 16), and registers have room for it (not float32's;
-// 1,024 lanes in three steps, 4,999 x 20,001 151 and 267 us, so 136 and 259, but in
-// two or four they spill: 6,103 x 16,384 backward 124 us, so 175).
+// of 1,024 lanes bfloat16's in three steps, 4,999 x 20,001 151 and 267 us, so 136 and
+// 259, but in two or four they spill, 6,103 x 16,384 backward 124 us, so 175, and
+// float16's in three, 244 us, so 332).
 template <int DT, int L, int S>
-constexpr bool kLast = DT != ST_SCORE_F32 && L * S > 2 && (L != 1024 || S == 3);
+constexpr bool kLast = DT != ST_SCORE_F32 && L * S > 2 && (L != 1024 || (S == 3 && DT == ST_SCORE_BF16));
 
 template <int DT>
 __device__ __forceinline__ void load_columns(const void* row, int col, int dim, float v[8]) {
@@ -177,11 +178,11 @@ __device__ __forceinline__ void load_columns_typed(const void* row, int col, int
 typedef uint32_t u32x2_by2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u32_by2 __attribute__((aligned(2)));
 
-template <int DT>
+template <int DT, bool LAST = false>
 __device__ __forceinline__ void store_columns(void* row, int col, int dim, const float v[8]) {
   if (col + 8 <= dim) {
     store8<DT>(row, col, v);
-  } else if constexpr (DT == ST_SCORE_F32) {
+  } else if constexpr (!LAST) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (col + i < dim) store_score<DT>(row, col + i, v[i]);
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
           // the norm is of the sum as it is returned
           v[i] = score_of_bits<HT>(score_bits<HT>(dropout_add(more[i], v[i], (keeps >> i) & 1, a.dropout.times)));
         }
-        if (live) store_columns<HT>(sum, col, a.dim, v);
+        if (live) store_columns<HT, kLast<HT, L, S>>(sum, col, a.dim, v);
       }
     };
     const void *weight = a.weight, *bias = a.bias;
@@ -393,7 +394,7 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         result(s, h[s]);
-        if (live) store_columns<DT>(y, (s * L + lane) * 8, a.dim, h[s]);
+        if (live) store_columns<DT, kLast<DT, L, S>>(y, (s * L + lane) * 8, a.dim, h[s]);
       }
     } else {
       float most[1] = {0.0f};
@@ -529,14 +530,14 @@ __global__ __launch_bounds__(norm_threads(L), norm_backward_waves(L, S)) void no
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[s][i] += more[i];
       }
-      if (a.gh && live) store_columns<HT>(static_cast<char*>(a.gh) + row * a.dim * kScoreBytes<HT>, col, a.dim, g[s]);
+      if (a.gh && live) store_columns<HT, kLast<HT, L, S>>(static_cast<char*>(a.gh) + row * a.dim * kScoreBytes<HT>, col, a.dim, g[s]);
       if (a.gx) {
         if (a.dropout.state) {
           const uint32_t keeps = dropout_keeps(key, static_cast<uint64_t>(row) * a.dim + col, a.dropout.dropped);
 #pragma unroll
           for (int i = 0; i < 8; ++i) g[s][i] = (keeps >> i) & 1 ? g[s][i] * a.dropout.times : 0.0f;
         }
-        if (live) store_columns<DT>(static_cast<char*>(a.gx) + row * a.dim * kScoreBytes<DT>, col, a.dim, g[s]);
+        if (live) store_columns<DT, kLast<DT, L, S>>(static_cast<char*>(a.gx) + row * a.dim * kScoreBytes<DT>, col, a.dim, g[s]);
       }
     }
   }
