@@ -204,6 +204,41 @@ def test_layer_norm_many_rows(rows, dim):
     assert all(torch.equal(a, c) for a, c in zip(grads, again))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim", [(70_001, 20), (90_001, 100), (40_003, 201), (9001, 1001), (3001, 5004), (1201, 16_001),
+                                      (1201, 17_001), (1201, 24_576), (1101, 25_001), (1101, 32_768)])
+def test_layer_norm_rows_in_turns(rows, dim, dtype):
+    """Rows that a workgroup takes one after another have the bits of rows in calls of their own; the bias's gradient is
+    the sum of the parts' (the whole and all parts are off by 64 + rows roundings of the magnitudes each at most)."""
+    H.note(f"[tower] layer_norm in turns {rows} x {dim} {dtype}")
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x, gy = (torch.randn((rows, dim), generator=g, device="cuda").to(dtype) for _ in range(2))
+    res = torch.randn((rows, dim), generator=g, device="cuda").to(dtype)
+    w, b = (torch.randn(dim, generator=g, device="cuda").requires_grad_() for _ in range(2))
+
+    def both(part):
+        leaves = [x[part].detach().requires_grad_(), res[part].detach().requires_grad_()]
+        y = st.layer_norm(leaves[0], w, b)
+        z, total = st.dropout_add_layer_norm(*leaves, w, b)
+        grads = torch.autograd.grad(y, [leaves[0], w, b], gy[part])
+        more = torch.autograd.grad([z, total], leaves, [gy[part], gy[part]])
+        codes = st.layer_norm_int8(x[part], w.detach(), b.detach()) + st.int8_quantize(x[part])
+        return [y.detach(), z.detach(), total.detach(), grads[0], *more, *codes], grads[1:]
+
+    whole, sums = both(slice(0, rows))
+    step = 128
+    parts = [both(slice(at, min(at + step, rows))) for at in range(0, min(rows, 10 * step), step)]
+    parts.append(both(slice(rows - 37, rows)))
+    ends = [(at, min(at + step, rows)) for at in range(0, min(rows, 10 * step), step)] + [(rows - 37, rows)]
+    for (lo, hi), (own, _) in zip(ends, parts):
+        for i, (a, c) in enumerate(zip(whole, own)):
+            assert torch.equal(a[lo:hi], c), (i, lo)
+    if rows <= 10 * step:
+        magnitude = gy.double().abs().sum(0)
+        total = sum(p[1][1].double() for p in parts[:-1])
+        assert ((sums[1].double() - total).abs() <= 2 * (64 + rows) * U * magnitude).all()
+
+
 def test_layer_norm_forms():
     """Without weight or bias, of any shape and stride, no rows, one wanted gradient, CPU tensors."""
     H.note("[tower] layer_norm forms")
