@@ -498,7 +498,7 @@ __global__ __launch_bounds__(norm_threads(L), norm_backward_waves(L, S)) void no
     for (int s = 0; s < S; ++s) {
       if constexpr (!kHold) load_weights(weight, s, w[0]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) n[s][i] = kRest<HT> ? ((n[s][i] - mean) - rest) * r : fmaf(n[s][i], r, -mean * r);
+      for (int i = 0; i < 8; ++i) n[s][i] = kRest<HT> ? ((n[s][i] - mean) - rest) * r : (n[s][i] - mean) * r;
       if (!whole(s))
 #pragma unroll
         for (int i = 0; i < 8; ++i) n[s][i] = (s * L + lane) * 8 + i < a.dim ? n[s][i] : 0.0f;
@@ -588,7 +588,7 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(NormBackwardArgs a) {
     const float mean = a.stats[kNormStats * row], rest = a.stats[kNormStats * row + 1], r = a.stats[kNormStats * row + 2];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      gw[i] = fmaf(g[i], kRest<HT> ? ((h[i] - mean) - rest) * r : fmaf(h[i], r, -mean * r), gw[i]);
+      gw[i] = fmaf(g[i], kRest<HT> ? ((h[i] - mean) - rest) * r : (h[i] - mean) * r, gw[i]);
       gb[i] += g[i];
     }
   }
