@@ -244,11 +244,6 @@ __device__ __forceinline__ void join_row(float (&x)[N], float* room, F f) {
 constexpr auto kAdd = [](float a, float b) { return a + b; };
 constexpr auto kMost = [](float a, float b) { return fmaxf(a, b); };
 
-// Whether what the mean's rounding left (2^-24 of it) counts: beside steps of
-// 16-bit values it does not.
-template <int HT>
-constexpr bool kRest = HT == ST_SCORE_F32;
-
 // HT: the type of h.  CODES: the result goes to 8 bits with a scale for each
 // row, from its 32-bit values.
 template <int DT, int HT, int L, int S, bool CODES>
@@ -350,7 +345,7 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
       join_row<L>(total, room, kAdd);
       mean = __fdiv_rn(total[0], static_cast<float>(a.dim));
       // the squares about the rounded mean, and what its rounding left
-      float left[kRest<HT> ? 2 : 1] = {};
+      float left[2] = {};
 #pragma unroll
       for (int s = 0; s < S; ++s) {
 #pragma unroll
@@ -361,17 +356,14 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           left[0] = fmaf(h[s][i], h[s][i], left[0]);
-          if constexpr (kRest<HT>) left[1] += h[s][i];
+          left[1] += h[s][i];
         }
       }
       join_row<L>(left, room + (L > 64 ? L / 64 : 0), kAdd);
-      float squares = left[0];
-      if constexpr (kRest<HT>) {
-        rest = __fdiv_rn(left[1], static_cast<float>(a.dim));
-        // a maximum with 0 would turn NaN into it
-        squares = fmaf(-rest, left[1], squares);
-        squares = squares < 0.0f ? 0.0f : squares;
-      }
+      rest = __fdiv_rn(left[1], static_cast<float>(a.dim));
+      // a maximum with 0 would turn NaN into it
+      float squares = fmaf(-rest, left[1], left[0]);
+      squares = squares < 0.0f ? 0.0f : squares;
       r = __fdiv_rn(1.0f, __fsqrt_rn(fmaf(squares, 1.0f / static_cast<float>(a.dim), a.eps)));
       if (a.stats && live && lane == 0) {
         a.stats[kNormStats * row] = mean;
@@ -385,7 +377,7 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
       if constexpr (!kHold) load_weights(weight, bias, s, w[0], b[0]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float n = kRest<HT> ? fmaf(v[i], r, -rest * r) : v[i] * r;
+        const float n = fmaf(v[i], r, -rest * r);
         v[i] = fmaf(n, w[kHold ? s : 0][i], b[kHold ? s : 0][i]);
       }
     };
@@ -498,7 +490,7 @@ __global__ __launch_bounds__(norm_threads(L), norm_backward_waves(L, S)) void no
     for (int s = 0; s < S; ++s) {
       if constexpr (!kHold) load_weights(weight, s, w[0]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) n[s][i] = kRest<HT> ? ((n[s][i] - mean) - rest) * r : (n[s][i] - mean) * r;
+      for (int i = 0; i < 8; ++i) n[s][i] = ((n[s][i] - mean) - rest) * r;
       if (!whole(s))
 #pragma unroll
         for (int i = 0; i < 8; ++i) n[s][i] = (s * L + lane) * 8 + i < a.dim ? n[s][i] : 0.0f;
@@ -588,7 +580,7 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(NormBackwardArgs a) {
     const float mean = a.stats[kNormStats * row], rest = a.stats[kNormStats * row + 1], r = a.stats[kNormStats * row + 2];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      gw[i] = fmaf(g[i], kRest<HT> ? ((h[i] - mean) - rest) * r : (h[i] - mean) * r, gw[i]);
+      gw[i] = fmaf(g[i], ((h[i] - mean) - rest) * r, gw[i]);
       gb[i] += g[i];
     }
   }
