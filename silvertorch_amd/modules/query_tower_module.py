@@ -16,7 +16,9 @@ class QueryTowerModule(nn.Module):
     ``h = in(dropout(x))``, then per layer ``h = h + dropout(down(relu(up(norm(h)))))``, then ``out(norm(h))``.
     A layer's end and the next norm are one pass (``dropout_add_layer_norm``).  Dropout stores no mask: it draws from
     ``rng`` (seed, next offset), a buffer on the module's device that every training pass advances, also when a graph
-    replays it.
+    replays it.  A pass that is computed twice (activation checkpointing) is given its state, for both to drop the same
+    elements: ``checkpoint(tower, x, tower.next_state(), use_reentrant=False)``.  Without one it is refused where it is
+    computed again, in the backward pass.
 
     Args:
         features: columns of the input.
@@ -43,12 +45,24 @@ class QueryTowerModule(nn.Module):
         self.register_buffer("places", torch.stack([torch.zeros(layers + 1, dtype=torch.int64),
                                                     torch.arange(layers + 1)], 1), persistent=False)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def next_state(self) -> torch.Tensor:
+        """The state (int64 [2]) of one training pass; ``rng`` goes on to the next one's."""
+        state = self.rng.clone()
+        self.rng[1] += len(self.places)
+        return state
+
+    def forward(self, x: torch.Tensor, state: torch.Tensor | None = None) -> torch.Tensor:
+        """`state`: dropout's of this pass, from `next_state`; without it, a training pass takes the next one."""
         ops = torch.ops.st
         p, states = 0.0, [None] * len(self.places)
         if self.training and self.dropout > 0:
-            p, states = self.dropout, (self.rng + self.places).unbind()
-            self.rng[1] += len(self.places)
+            if state is None:
+                if torch._C._current_graph_task_id() != -1:
+                    raise RuntimeError("a training pass inside a backward pass (activation checkpointing computes it "
+                                       "again) would drop other elements than its first run: give it a state, "
+                                       "checkpoint(tower, x, tower.next_state())")
+                state = self.next_state()
+            p, states = self.dropout, (state + self.places).unbind()
             x = ops.dropout(x, p, states[0])
         h = self.enter(x)
         y = ops.layer_norm(h, self.norm_weights[0], self.norm_biases[0], self.eps)
