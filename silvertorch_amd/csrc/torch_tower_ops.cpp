@@ -5,7 +5,10 @@
 // As in torch_head_ops.cpp, GPU tensors run on their device's current stream and
 // CPU tensors are copied to the current GPU and the results back.  What a tower
 // is trained through carries its gradients (Autograd key); the 8-bit operators
-// refuse to be differentiated.
+// refuse to be differentiated.  Below that key every kernel is called through the
+// dispatcher, so that a dispatch mode sees it: a pass that keeps something for its
+// gradients is an operator of its own (_with_state, _with_stats), and so is
+// layer_norm_backward.
 #include <torch/library.h>
 
 #include "torch_autograd.hpp"
@@ -29,6 +32,7 @@ using st_torch::with_adjacent_columns;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using Pair = std::tuple<Tensor, Tensor>;
+using Four = std::tuple<Tensor, Tensor, Tensor, Tensor>;
 
 constexpr int64_t kMaxNormColumns = 32768;
 
@@ -102,10 +106,28 @@ Pair dropout_any(const Tensor& x, double p, const Tensor& state, bool with_used)
   return {y.cpu(), back(used, false)};
 }
 
+Tensor dropout(const Tensor& x, double p, const Tensor& state) { return std::get<0>(dropout_any(x, p, state, false)); }
+
+Pair dropout_with_state(const Tensor& x, double p, const Tensor& state) { return dropout_any(x, p, state, true); }
+
+using DropoutOp = Tensor(const Tensor&, double, const Tensor&);
+using DropoutKeepOp = Pair(const Tensor&, double, const Tensor&);
+
+Tensor dropout_below(const Tensor& x, double p, const Tensor& state) {
+  static const auto op = find_op<DropoutOp>("st::dropout");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, p, state);
+}
+
+Pair dropout_with_state_below(const Tensor& x, double p, const Tensor& state) {
+  static const auto op = find_op<DropoutKeepOp>("st::dropout_with_state");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, p, state);
+}
+
 struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, const Tensor& state) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    auto [y, used] = dropout_any(x, p, state, true);
+    auto [y, used] = dropout_with_state_below(x, p, state);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({used});
     ctx->saved_data["p"] = p;
@@ -113,21 +135,14 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     Tensor grad;
-    if (grads[0].defined()) {
-      at::AutoDispatchBelowADInplaceOrView below;
-      grad = std::get<0>(dropout_any(grads[0], ctx->saved_data["p"].toDouble(), ctx->get_saved_variables()[0], false));
-    }
+    if (grads[0].defined()) grad = dropout_below(grads[0], ctx->saved_data["p"].toDouble(), ctx->get_saved_variables()[0]);
     return {differentiable_once(grad, grads[0], Tensor(), grads, "dropout"), Tensor(), Tensor()};
   }
 };
 
-Tensor dropout(const Tensor& x, double p, const Tensor& state) { return std::get<0>(dropout_any(x, p, state, false)); }
-
 Tensor dropout_autograd(const Tensor& x, double p, const Tensor& state) {
   refuse_tangents({&x}, "dropout");
-  if (requires_grad({&x})) return DropoutFunction::apply(x, p, state);
-  at::AutoDispatchBelowADInplaceOrView below;
-  return dropout(x, p, state);
+  return requires_grad({&x}) ? DropoutFunction::apply(x, p, state) : dropout_below(x, p, state);
 }
 
 // ------------------------------------------ layer norm
@@ -213,23 +228,57 @@ NormOut norm_any(const NormIn& in, bool with_grad, const char* op) {
   return o;
 }
 
-struct NormGrads {
-  Tensor x, residual, weight, bias;
-};
+Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  return norm_any({x, Tensor(), given(weight), given(bias), Tensor(), 0.0, eps}, false, "layer_norm").y;
+}
 
-struct NormWanted {
-  bool x, residual, weight, bias;
-};
+Pair layer_norm_with_stats(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  NormOut o = norm_any({x, Tensor(), given(weight), given(bias), Tensor(), 0.0, eps}, true, "layer_norm");
+  return {o.y, o.stats};
+}
 
-// h: x, or the sum.  The gradients come on h's device.
-NormGrads norm_gradients(const Tensor& h_in, at::ScalarType y_type, const Tensor& weight_in, at::ScalarType weights,
-                         const Tensor& stats_in, double p, const Tensor& used_in, const Tensor& grad_y,
-                         const Tensor& grad_sum, const NormWanted& want) {
-  at::AutoDispatchBelowADInplaceOrView below;
+Pair dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& bias,
+                            double p, const OptTensor& state, double eps) {
+  NormOut o = norm_any({x, residual, given(weight), given(bias), given(state), p, eps}, false, "dropout_add_layer_norm");
+  return {o.y, o.sum};
+}
+
+Four dropout_add_layer_norm_with_stats(const Tensor& x, const Tensor& residual, const OptTensor& weight,
+                                       const OptTensor& bias, double p, const OptTensor& state, double eps) {
+  NormOut o = norm_any({x, residual, given(weight), given(bias), given(state), p, eps}, true, "dropout_add_layer_norm");
+  return {o.y, o.sum, o.stats, o.used};
+}
+
+void check_gradients(const Tensor& h, at::ScalarType y_type, const Tensor& weight, at::ScalarType weights,
+                     const Tensor& stats, double p, const Tensor& used, const Tensor& grad_y, const Tensor& grad_sum) {
+  check_weights(h, weight, Tensor(), 1.0, "layer_norm_backward");
+  score_type(y_type, "x");
+  score_type(weights, "weight and bias");
+  TORCH_CHECK(h.scalar_type() == y_type || h.scalar_type() == at::kFloat, "the sum must be of x's type or float32, got ",
+              h.scalar_type());
+  TORCH_CHECK(stats.dim() == 2 && stats.size(0) == h.numel() / h.size(-1) && stats.size(1) == ST_NORM_STATS &&
+                  stats.scalar_type() == at::kFloat && stats.device() == h.device(),
+              "stats must be float32 [rows, ", ST_NORM_STATS, "] of the forward pass, got ", stats.sizes());
+  for (const Tensor* t : {&grad_y, &grad_sum})
+    TORCH_CHECK(!t->defined() || (t->sizes() == h.sizes() && t->device() == h.device()),
+                "gradients must be of the results' shape ", h.sizes(), " and device");
+  check_dropout(h, p, used, "layer_norm_backward");
+  TORCH_CHECK(p == 0.0 || used.defined(), "dropout needs the state that was used");
+}
+
+// h: x, or the sum; used: the state that the forward pass used, if it dropped.  The
+// gradients come on h's device, undefined where they are not wanted.
+Four layer_norm_backward(const OptTensor& grad_y_in, const OptTensor& grad_sum_in, const Tensor& h_in,
+                         const OptTensor& weight_opt, const Tensor& stats_in, const OptTensor& used_opt, double p,
+                         at::ScalarType y_type, at::ScalarType weights, std::array<bool, 4> wanted) {
+  const Tensor grad_y = given(grad_y_in), grad_sum = given(grad_sum_in), weight_in = given(weight_opt), used_in = given(used_opt);
+  check_gradients(h_in, y_type, weight_in, weights, stats_in, p, used_in, grad_y, grad_sum);
   const bool on_gpu = h_in.is_cuda();
   const at::Device dev = on_gpu ? h_in.device() : gpu_for_cpu_call();
   c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
-  const Tensor h = as_rows(placed(h_in, dev)), stats = placed(stats_in, dev), used = placed(used_in, dev);
+  const Tensor h = as_rows(placed(h_in, dev)), stats = placed(stats_in, dev).contiguous();
+  Tensor used;
+  if (used_in.defined()) used = placed(used_in, dev).contiguous();
   const int64_t rows = h.size(0), dim = h.size(1);
   const auto options = h.options();
   Tensor weight;
@@ -237,23 +286,62 @@ NormGrads norm_gradients(const Tensor& h_in, at::ScalarType y_type, const Tensor
   // without a gradient of its own the norm's result has one of zeros
   const Tensor gy = grad_y.defined() ? grad_rows(grad_y, y_type, dev) : at::zeros(h_in.sizes(), options.dtype(y_type));
   const Tensor gsum = grad_rows(grad_sum, h.scalar_type(), dev);
-  NormGrads g;
-  if (want.x) g.x = at::empty(h_in.sizes(), options.dtype(y_type));
-  if (want.residual) g.residual = at::empty(h_in.sizes(), options);
-  if (want.weight) g.weight = at::empty({dim}, options.dtype(weights));
-  if (want.bias) g.bias = at::empty({dim}, options.dtype(weights));
-  Tensor ws;
-  if (want.weight || want.bias)
+  Tensor gx, gr, gw, gb, ws;
+  if (wanted[0]) gx = at::empty(h_in.sizes(), options.dtype(y_type));
+  if (wanted[1]) gr = at::empty(h_in.sizes(), options);
+  if (wanted[2]) gw = at::empty({dim}, options.dtype(weights));
+  if (wanted[3]) gb = at::empty({dim}, options.dtype(weights));
+  if (wanted[2] || wanted[3])
     ws = at::empty({st_layer_norm_workspace_bytes(rows, dim)}, options.dtype(at::kByte));
   check_st(st_layer_norm_backward(bytes_or_null(gy), score_type(y_type, "x"), bytes_or_null(gsum), bytes_or_null(h),
                                   score_type(h.scalar_type(), "residual"), rows, dim, h.stride(0), bytes_or_null(weight),
                                   score_type(weights, "weight"), data_or_null<float>(stats), used.defined() ? p : 0.0,
-                                  data_or_null<int64_t>(used), bytes_or_null(ws), bytes_or_null(g.x),
-                                  bytes_or_null(g.residual), bytes_or_null(g.weight), bytes_or_null(g.bias),
-                                  current_stream(h)),
-           "layer_norm");
-  for (Tensor* t : {&g.x, &g.residual, &g.weight, &g.bias}) *t = back(*t, on_gpu);
-  return g;
+                                  data_or_null<int64_t>(used), bytes_or_null(ws), bytes_or_null(gx),
+                                  bytes_or_null(gr), bytes_or_null(gw), bytes_or_null(gb), current_stream(h)),
+           "layer_norm_backward");
+  return {back(gx, on_gpu), back(gr, on_gpu), back(gw, on_gpu), back(gb, on_gpu)};
+}
+
+using NormOp = Tensor(const Tensor&, const OptTensor&, const OptTensor&, double);
+using NormKeepOp = Pair(const Tensor&, const OptTensor&, const OptTensor&, double);
+using ResidualOp = Pair(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, double, const OptTensor&, double);
+using ResidualKeepOp = Four(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, double, const OptTensor&, double);
+using NormBackwardOp = Four(const OptTensor&, const OptTensor&, const Tensor&, const OptTensor&, const Tensor&,
+                            const OptTensor&, double, at::ScalarType, at::ScalarType, std::array<bool, 4>);
+
+Tensor norm_below(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  static const auto op = find_op<NormOp>("st::layer_norm");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, weight, bias, eps);
+}
+
+Pair norm_with_stats_below(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  static const auto op = find_op<NormKeepOp>("st::layer_norm_with_stats");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, weight, bias, eps);
+}
+
+Pair residual_below(const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& bias, double p,
+                    const OptTensor& state, double eps) {
+  static const auto op = find_op<ResidualOp>("st::dropout_add_layer_norm");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, residual, weight, bias, p, state, eps);
+}
+
+Four residual_with_stats_below(const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& bias,
+                               double p, const OptTensor& state, double eps) {
+  static const auto op = find_op<ResidualKeepOp>("st::dropout_add_layer_norm_with_stats");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, residual, weight, bias, p, state, eps);
+}
+
+Four norm_backward_below(AutogradContext* ctx, const Tensor& grad_y, const Tensor& grad_sum, const Tensor& h,
+                         const Tensor& weight, const Tensor& stats, const Tensor& used, std::array<bool, 4> wanted) {
+  static const auto op = find_op<NormBackwardOp>("st::layer_norm_backward");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(if_defined(grad_y), if_defined(grad_sum), h, if_defined(weight), stats, if_defined(used),
+                 ctx->saved_data["p"].toDouble(), static_cast<at::ScalarType>(ctx->saved_data["y"].toInt()),
+                 static_cast<at::ScalarType>(ctx->saved_data["weights"].toInt()), wanted);
 }
 
 at::ScalarType weights_scalar_type(const Tensor& weight, const Tensor& bias) {
@@ -262,92 +350,71 @@ at::ScalarType weights_scalar_type(const Tensor& weight, const Tensor& bias) {
 
 // Gradients wanted of weight and bias: the graph's edges count the tensors that
 // were given, `first` of them ahead of the weight.
-NormWanted wanted(AutogradContext* ctx, size_t first) {
+std::array<bool, 4> wanted(AutogradContext* ctx, size_t first) {
   const bool weight = ctx->saved_data["weight"].toBool(), bias = ctx->saved_data["bias"].toBool();
   return {ctx->needs_input_grad(0), first > 1 && ctx->needs_input_grad(1), weight && ctx->needs_input_grad(first),
           bias && ctx->needs_input_grad(first + (weight ? 1 : 0))};
 }
 
-void keep(AutogradContext* ctx, const NormIn& in) {
+void keep(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& bias, double p) {
   ctx->set_materialize_grads(false);
-  ctx->saved_data["weight"] = in.weight.defined();
-  ctx->saved_data["bias"] = in.bias.defined();
-  ctx->saved_data["weights"] = static_cast<int64_t>(weights_scalar_type(in.weight, in.bias));
-  ctx->saved_data["y"] = static_cast<int64_t>(in.x.scalar_type());
-  ctx->saved_data["p"] = in.p;
+  ctx->saved_data["weight"] = weight.defined();
+  ctx->saved_data["bias"] = bias.defined();
+  ctx->saved_data["weights"] = static_cast<int64_t>(weights_scalar_type(weight, bias));
+  ctx->saved_data["y"] = static_cast<int64_t>(x.scalar_type());
+  ctx->saved_data["p"] = p;
 }
 
 struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    const NormIn in{x, Tensor(), given(weight), given(bias), Tensor(), 0.0, eps};
-    const NormOut o = norm_any(in, true, "layer_norm");
-    keep(ctx, in);
-    ctx->save_for_backward({x, in.weight, o.stats});
-    return o.y;
+    auto [y, stats] = norm_with_stats_below(x, weight, bias, eps);
+    keep(ctx, x, given(weight), given(bias), 0.0);
+    ctx->save_for_backward({x, given(weight), stats});
+    return y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    const NormGrads g = norm_gradients(saved[0], saved[0].scalar_type(), saved[1],
-                                       static_cast<at::ScalarType>(ctx->saved_data["weights"].toInt()), saved[2], 0.0,
-                                       Tensor(), grads[0], Tensor(), wanted(ctx, 1));
+    auto [gx, gr, gw, gb] =
+        norm_backward_below(ctx, grads[0], Tensor(), saved[0], saved[1], saved[2], Tensor(), wanted(ctx, 1));
     auto once = [&](const Tensor& t) { return differentiable_once(t, saved[0], saved[1], grads, "layer_norm"); };
-    return {once(g.x), once(g.weight), once(g.bias), Tensor()};
+    return {once(gx), once(gw), once(gb), Tensor()};
   }
 };
-
-Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
-  return norm_any({x, Tensor(), given(weight), given(bias), Tensor(), 0.0, eps}, false, "layer_norm").y;
-}
 
 Tensor layer_norm_autograd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
   const Tensor w = given(weight), b = given(bias);
   refuse_tangents_of({&x, &w, &b}, "layer_norm");
-  if (requires_grad({&x, &w, &b})) return LayerNormFunction::apply(x, weight, bias, eps);
-  at::AutoDispatchBelowADInplaceOrView below;
-  return layer_norm(x, weight, bias, eps);
+  return requires_grad({&x, &w, &b}) ? LayerNormFunction::apply(x, weight, bias, eps) : norm_below(x, weight, bias, eps);
 }
 
 struct ResidualFunction : torch::autograd::Function<ResidualFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const OptTensor& weight,
                                const OptTensor& bias, double p, const OptTensor& state, double eps) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    const NormIn in{x, residual, given(weight), given(bias), given(state), p, eps};
-    const NormOut o = norm_any(in, true, "dropout_add_layer_norm");
-    keep(ctx, in);
-    ctx->save_for_backward({o.sum, in.weight, o.stats, o.used});
-    return {o.y, o.sum};
+    auto [y, sum, stats, used] = residual_with_stats_below(x, residual, weight, bias, p, state, eps);
+    keep(ctx, x, given(weight), given(bias), used.defined() ? p : 0.0);
+    ctx->save_for_backward({sum, given(weight), stats, used});
+    return {y, sum};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(7);
-    const NormGrads g = norm_gradients(saved[0], static_cast<at::ScalarType>(ctx->saved_data["y"].toInt()), saved[1],
-                                       static_cast<at::ScalarType>(ctx->saved_data["weights"].toInt()), saved[2],
-                                       ctx->saved_data["p"].toDouble(), saved[3], grads[0], grads[1], wanted(ctx, 2));
+    auto [gx, gr, gw, gb] =
+        norm_backward_below(ctx, grads[0], grads[1], saved[0], saved[1], saved[2], saved[3], wanted(ctx, 2));
     auto once = [&](const Tensor& t) { return differentiable_once(t, saved[0], saved[1], grads, "dropout_add_layer_norm"); };
-    return {once(g.x), once(g.residual), once(g.weight), once(g.bias), Tensor(), Tensor(), Tensor()};
+    return {once(gx), once(gr), once(gw), once(gb), Tensor(), Tensor(), Tensor()};
   }
 };
-
-Pair dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& bias,
-                            double p, const OptTensor& state, double eps) {
-  NormOut o = norm_any({x, residual, given(weight), given(bias), given(state), p, eps}, false, "dropout_add_layer_norm");
-  return {o.y, o.sum};
-}
 
 Pair dropout_add_layer_norm_autograd(const Tensor& x, const Tensor& residual, const OptTensor& weight,
                                      const OptTensor& bias, double p, const OptTensor& state, double eps) {
   const Tensor w = given(weight), b = given(bias);
   refuse_tangents_of({&x, &residual, &w, &b}, "dropout_add_layer_norm");
-  if (requires_grad({&x, &residual, &w, &b})) {
-    const variable_list o = ResidualFunction::apply(x, residual, weight, bias, p, state, eps);
-    return {o[0], o[1]};
-  }
-  at::AutoDispatchBelowADInplaceOrView below;
-  return dropout_add_layer_norm(x, residual, weight, bias, p, state, eps);
+  if (!requires_grad({&x, &residual, &w, &b})) return residual_below(x, residual, weight, bias, p, state, eps);
+  const variable_list o = ResidualFunction::apply(x, residual, weight, bias, p, state, eps);
+  return {o[0], o[1]};
 }
 
 // ------------------------------------------ rows in 8 bits
@@ -569,6 +636,14 @@ TORCH_LIBRARY_FRAGMENT(st, m) {
   // (the sum's layer norm, residual + dropout(x))
   m.def("dropout_add_layer_norm(Tensor x, Tensor residual, Tensor? weight=None, Tensor? bias=None, float p=0.0, "
         "Tensor? state=None, float eps=1e-05) -> (Tensor, Tensor)");
+  // What the gradients call: (result, state that was used), (result, stats), (norm, sum, stats, state that was used or
+  // none), gradients of (x, residual, weight, bias) or none where not wanted.
+  m.def("dropout_with_state(Tensor x, float p, Tensor state) -> (Tensor, Tensor)");
+  m.def("layer_norm_with_stats(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor)");
+  m.def("dropout_add_layer_norm_with_stats(Tensor x, Tensor residual, Tensor? weight, Tensor? bias, float p, "
+        "Tensor? state, float eps) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("layer_norm_backward(Tensor? grad_y, Tensor? grad_sum, Tensor h, Tensor? weight, Tensor stats, Tensor? used, "
+        "float p, ScalarType y_type, ScalarType weight_type, bool[4] wanted) -> (Tensor, Tensor, Tensor, Tensor)");
   // codes int8 [..., D up to a multiple of 16], scales [...]
   m.def("int8_quantize(Tensor x) -> (Tensor, Tensor)");
   m.def("layer_norm_int8(Tensor x, Tensor? weight=None, Tensor? bias=None, float eps=1e-05) -> (Tensor, Tensor)");
@@ -581,6 +656,10 @@ TORCH_LIBRARY_IMPL(st, CUDA, m) {
   m.impl("layer_norm", TORCH_FN(layer_norm));
   m.impl("dropout", TORCH_FN(dropout));
   m.impl("dropout_add_layer_norm", TORCH_FN(dropout_add_layer_norm));
+  m.impl("dropout_with_state", TORCH_FN(dropout_with_state));
+  m.impl("layer_norm_with_stats", TORCH_FN(layer_norm_with_stats));
+  m.impl("dropout_add_layer_norm_with_stats", TORCH_FN(dropout_add_layer_norm_with_stats));
+  m.impl("layer_norm_backward", TORCH_FN(layer_norm_backward));
   m.impl("int8_quantize", TORCH_FN(int8_quantize_gpu));
   m.impl("layer_norm_int8", TORCH_FN(layer_norm_int8_gpu));
   m.impl("int8_matmul", TORCH_FN(int8_matmul_gpu));
@@ -590,6 +669,10 @@ TORCH_LIBRARY_IMPL(st, CPU, m) {
   m.impl("layer_norm", TORCH_FN(layer_norm));
   m.impl("dropout", TORCH_FN(dropout));
   m.impl("dropout_add_layer_norm", TORCH_FN(dropout_add_layer_norm));
+  m.impl("dropout_with_state", TORCH_FN(dropout_with_state));
+  m.impl("layer_norm_with_stats", TORCH_FN(layer_norm_with_stats));
+  m.impl("dropout_add_layer_norm_with_stats", TORCH_FN(dropout_add_layer_norm_with_stats));
+  m.impl("layer_norm_backward", TORCH_FN(layer_norm_backward));
   m.impl("int8_quantize", TORCH_FN(int8_quantize_cpu));
   m.impl("layer_norm_int8", TORCH_FN(layer_norm_int8_cpu));
   m.impl("int8_matmul", TORCH_FN(int8_matmul_cpu));
