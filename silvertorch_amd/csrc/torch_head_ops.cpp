@@ -4,7 +4,8 @@
 // As in torch_ops.cpp, GPU tensors run on their device's current stream and
 // CPU tensors are copied to the current GPU and the results back.  The two
 // operators a model is trained through carry their gradients (Autograd key);
-// the 4-bit ones refuse to be differentiated.
+// the 4-bit ones refuse to be differentiated.  Below that key every kernel is
+// called through the dispatcher, so that a dispatch mode sees it.
 #include <torch/library.h>
 
 #include "torch_autograd.hpp"
@@ -258,18 +259,95 @@ Tensor differentiable_once(const Tensor& grad, const Tensor& logits, const varia
                                    if_defined(outer[4]), std::string(op));
 }
 
+using Logprobs = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
+using LogprobsStats = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
+
+Logprobs target_logprobs(const Tensor& logits, const Tensor& targets, int64_t topk, const OptTensor& mask,
+                         double temperature) {
+  LogprobsOut o = logprobs_any(logits, targets, topk, mask.value_or(Tensor()), temperature, false);
+  return {o.logprobs, o.entropy, o.lse, o.top_ids, o.top_logprobs};
+}
+
+LogprobsStats target_logprobs_with_stats(const Tensor& logits, const Tensor& targets, int64_t topk,
+                                         const OptTensor& mask, double temperature) {
+  LogprobsOut o = logprobs_any(logits, targets, topk, mask.value_or(Tensor()), temperature, true);
+  return {o.logprobs, o.entropy, o.lse, o.top_ids, o.top_logprobs, o.stats};
+}
+
+// The gradients of logprobs, entropy, lse and top_logprobs, each absent where it is zero.
+Tensor target_logprobs_backward(const Tensor& logits, const Tensor& targets, int64_t topk, const OptTensor& packed_mask,
+                                double temperature, const Tensor& entropy_in, const Tensor& top_ids_in,
+                                const Tensor& stats_in, const OptTensor& g_logprobs, const OptTensor& g_entropy,
+                                const OptTensor& g_lse, const OptTensor& g_top) {
+  const Tensor mask = packed_mask.value_or(Tensor());
+  check_logprobs(logits, targets, topk, mask, temperature);
+  const int64_t n = logits.size(0);
+  auto check = [&](const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const char* what) {
+    TORCH_CHECK(t.sizes() == sizes && t.scalar_type() == type && t.device() == logits.device(), what, " must be ", type,
+                " of ", sizes, " on the scores' device, got ", t.scalar_type(), " of ", t.sizes());
+  };
+  check(entropy_in, {n}, at::kFloat, "entropy");
+  check(top_ids_in, {n, topk}, at::kLong, "top_ids");
+  check(stats_in, {n, 2}, at::kFloat, "stats");
+  for (const OptTensor* g : {&g_logprobs, &g_entropy, &g_lse, &g_top}) {
+    if (!g->has_value() || !(*g)->defined()) continue;
+    const bool of_rows = g != &g_top;
+    TORCH_CHECK((of_rows ? (*g)->sizes() == at::IntArrayRef({n}) : (*g)->sizes() == at::IntArrayRef({n, topk})) &&
+                    (*g)->device() == logits.device(),
+                "gradients must be of the results' shapes and device, got ", (*g)->sizes());
+  }
+  const bool on_gpu = logits.is_cuda();
+  const at::Device dev = on_gpu ? logits.device() : gpu_for_cpu_call();
+  const LogprobsIn in =
+      logprobs_in(logits.to(dev), targets.to(dev), topk, mask.defined() ? mask.to(dev) : mask, temperature);
+  c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+  auto there = [&](const Tensor& t) { return t.to(dev).contiguous(); };
+  const Tensor entropy = there(entropy_in), top_ids = there(top_ids_in), stats = there(stats_in);
+  auto given = [&](const OptTensor& g) { return gradient(g.value_or(Tensor()), dev); };
+  const Tensor gl = given(g_logprobs), ge = given(g_entropy), gs = given(g_lse), gt = given(g_top);
+  const Tensor& z = in.logits;
+  Tensor grad = at::empty(z.sizes(), z.options());
+  check_st(st_target_logprobs_backward(
+               bytes_or_null(z), in.type, z.size(0), z.size(1), z.stride(0), data_or_null<int64_t>(in.targets),
+               data_or_null<int64_t>(in.mask), in.mask_stride, in.mask_words, in.topk, in.temperature,
+               data_or_null<float>(entropy), data_or_null<float>(stats), data_or_null<int64_t>(top_ids),
+               data_or_null<float>(gl), data_or_null<float>(ge), data_or_null<float>(gs), data_or_null<float>(gt),
+               bytes_or_null(grad), current_stream(z)),
+           "target_logprobs");
+  return on_gpu ? grad : grad.cpu();
+}
+
+using LogprobsOp = Logprobs(const Tensor&, const Tensor&, int64_t, const OptTensor&, double);
+using LogprobsKeepOp = LogprobsStats(const Tensor&, const Tensor&, int64_t, const OptTensor&, double);
+using LogprobsBackwardOp = Tensor(const Tensor&, const Tensor&, int64_t, const OptTensor&, double, const Tensor&,
+                                  const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+                                  const OptTensor&);
+
+Logprobs logprobs_below(const Tensor& logits, const Tensor& targets, int64_t topk, const OptTensor& mask,
+                        double temperature) {
+  static const auto op = find_op<LogprobsOp>("st::target_logprobs");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(logits, targets, topk, mask, temperature);
+}
+
+LogprobsStats logprobs_with_stats_below(const Tensor& logits, const Tensor& targets, int64_t topk, const OptTensor& mask,
+                                        double temperature) {
+  static const auto op = find_op<LogprobsKeepOp>("st::target_logprobs_with_stats");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(logits, targets, topk, mask, temperature);
+}
+
 struct LogprobsFunction : torch::autograd::Function<LogprobsFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& targets, int64_t topk,
                                const OptTensor& packed_mask, double temperature) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor mask = packed_mask.value_or(Tensor());
-    LogprobsOut o = logprobs_any(logits, targets, topk, mask, temperature, true);
+    auto [logprobs, entropy, lse, top_ids, top_logprobs, stats] =
+        logprobs_with_stats_below(logits, targets, topk, packed_mask, temperature);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({logits, targets, mask, o.entropy, o.top_ids, o.stats});
+    ctx->save_for_backward({logits, targets, packed_mask.value_or(Tensor()), entropy, top_ids, stats});
     ctx->saved_data["topk"] = topk;
     ctx->saved_data["temperature"] = temperature;
-    ctx->mark_non_differentiable({o.top_ids});
-    return {o.logprobs, o.entropy, o.lse, o.top_ids, o.top_logprobs};
+    ctx->mark_non_differentiable({top_ids});
+    return {logprobs, entropy, lse, top_ids, top_logprobs};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -279,45 +357,19 @@ struct LogprobsFunction : torch::autograd::Function<LogprobsFunction> {
   }
 
   static Tensor logits_gradient(AutogradContext* ctx, const variable_list& saved, const variable_list& grads) {
+    static const auto op = find_op<LogprobsBackwardOp>("st::target_logprobs_backward");
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor& logits = saved[0];
-    const bool on_gpu = logits.is_cuda();
-    const at::Device dev = on_gpu ? logits.device() : gpu_for_cpu_call();
-    const LogprobsIn in = logprobs_in(logits.to(dev), saved[1].to(dev), ctx->saved_data["topk"].toInt(),
-                                      saved[2].defined() ? saved[2].to(dev) : saved[2],
-                                      ctx->saved_data["temperature"].toDouble());
-    c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
-    const Tensor entropy = saved[3].to(dev), top_ids = saved[4].to(dev), stats = saved[5].to(dev);
-    const Tensor gl = gradient(grads[0], dev), ge = gradient(grads[1], dev), gs = gradient(grads[2], dev),
-                 gt = gradient(grads[4], dev);
-    const Tensor& z = in.logits;
-    Tensor grad = at::empty(z.sizes(), z.options());
-    check_st(st_target_logprobs_backward(
-                 bytes_or_null(z), in.type, z.size(0), z.size(1), z.stride(0), data_or_null<int64_t>(in.targets),
-                 data_or_null<int64_t>(in.mask), in.mask_stride, in.mask_words, in.topk, in.temperature,
-                 data_or_null<float>(entropy), data_or_null<float>(stats), data_or_null<int64_t>(top_ids),
-                 data_or_null<float>(gl), data_or_null<float>(ge), data_or_null<float>(gs), data_or_null<float>(gt),
-                 bytes_or_null(grad), current_stream(z)),
-             "target_logprobs");
-    return on_gpu ? grad : grad.cpu();
+    return op.call(saved[0], saved[1], ctx->saved_data["topk"].toInt(), if_defined(saved[2]),
+                   ctx->saved_data["temperature"].toDouble(), saved[3], saved[4], saved[5], if_defined(grads[0]),
+                   if_defined(grads[1]), if_defined(grads[2]), if_defined(grads[4]));
   }
 };
-
-using Logprobs = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
-
-Logprobs target_logprobs(const Tensor& logits, const Tensor& targets, int64_t topk, const OptTensor& mask,
-                         double temperature) {
-  LogprobsOut o = logprobs_any(logits, targets, topk, mask.value_or(Tensor()), temperature, false);
-  return {o.logprobs, o.entropy, o.lse, o.top_ids, o.top_logprobs};
-}
 
 Logprobs target_logprobs_autograd(const Tensor& logits, const Tensor& targets, int64_t topk, const OptTensor& mask,
                                   double temperature) {
   refuse_tangents({&logits}, "target_logprobs");
-  if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    return target_logprobs(logits, targets, topk, mask, temperature);
-  }
+  if (!at::GradMode::is_enabled() || !logits.requires_grad())
+    return logprobs_below(logits, targets, topk, mask, temperature);
   const variable_list o = LogprobsFunction::apply(logits, targets, topk, mask, temperature);
   return {o[0], o[1], o[2], o[3], o[4]};
 }
@@ -431,6 +483,12 @@ TORCH_LIBRARY_FRAGMENT(st, m) {
   // (logprobs, entropy, lse, top_ids, top_logprobs)
   m.def("target_logprobs(Tensor logits, Tensor targets, int topk=0, Tensor? packed_mask=None, "
         "float temperature=1.0) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  // What its gradient calls: the same and the statistics; the gradient of the scores.
+  m.def("target_logprobs_with_stats(Tensor logits, Tensor targets, int topk, Tensor? packed_mask, float temperature) "
+        "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("target_logprobs_backward(Tensor logits, Tensor targets, int topk, Tensor? packed_mask, float temperature, "
+        "Tensor entropy, Tensor top_ids, Tensor stats, Tensor? g_logprobs, Tensor? g_entropy, Tensor? g_lse, "
+        "Tensor? g_top) -> Tensor");
   // (cluster_ids, weights, lse, counts, balance_loss)
   m.def("cluster_route(Tensor logits, int probes, Tensor? valid=None) "
         "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
@@ -440,6 +498,8 @@ TORCH_LIBRARY_IMPL(st, CUDA, m) {
   m.impl("int4_quantize", TORCH_FN(int4_quantize_gpu));
   m.impl("int4_matvec", TORCH_FN(int4_matvec_gpu));
   m.impl("target_logprobs", TORCH_FN(target_logprobs));
+  m.impl("target_logprobs_with_stats", TORCH_FN(target_logprobs_with_stats));
+  m.impl("target_logprobs_backward", TORCH_FN(target_logprobs_backward));
   m.impl("cluster_route", TORCH_FN(cluster_route));
 }
 
@@ -447,6 +507,8 @@ TORCH_LIBRARY_IMPL(st, CPU, m) {
   m.impl("int4_quantize", TORCH_FN(int4_quantize_cpu));
   m.impl("int4_matvec", TORCH_FN(int4_matvec_cpu));
   m.impl("target_logprobs", TORCH_FN(target_logprobs));
+  m.impl("target_logprobs_with_stats", TORCH_FN(target_logprobs_with_stats));
+  m.impl("target_logprobs_backward", TORCH_FN(target_logprobs_backward));
   m.impl("cluster_route", TORCH_FN(cluster_route));
 }
 
