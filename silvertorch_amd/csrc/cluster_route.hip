@@ -774,7 +774,9 @@ __global__ __launch_bounds__(kThreads<LPR>) void route_backward_kernel(RouteBack
     for (int j = 0; j < kOwn; ++j) {
       const int i = in_row + LPR * j;
       const bool is = i < k;
-      x.id[j] = is ? static_cast<int>(a.ids[r * k + i]) : -1;
+      // an id that is no cluster's is none, as -1 is
+      const int64_t given = is ? a.ids[r * k + i] : -1;
+      x.id[j] = given >= 0 && given < clusters ? static_cast<int>(given) : -1;
       x.weight[j] = is ? a.weights[r * k + i] : 0.0f;
       x.g[j] = is && a.g_weights != nullptr ? a.g_weights[r * k + i] : 0.0f;
     }

@@ -419,14 +419,84 @@ RouteOut route_any(const Tensor& logits, int64_t probes, const Tensor& valid) {
   return o;
 }
 
+using Route = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
+using RouteStats = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
+
+Route cluster_route(const Tensor& logits, int64_t probes, const OptTensor& valid) {
+  RouteOut o = route_any(logits, probes, valid.value_or(Tensor()));
+  return {o.ids, o.weights, o.lse, o.counts, o.loss};
+}
+
+RouteStats cluster_route_with_stats(const Tensor& logits, int64_t probes, const OptTensor& valid) {
+  RouteOut o = route_any(logits, probes, valid.value_or(Tensor()));
+  return {o.ids, o.weights, o.lse, o.counts, o.loss, o.stats, o.slopes};
+}
+
+// The gradients of weights, lse and the loss, each absent where it is zero.
+Tensor cluster_route_backward(const Tensor& logits, const Tensor& ids_in, const Tensor& weights_in,
+                              const Tensor& stats_in, const Tensor& slopes_in, const OptTensor& g_weights,
+                              const OptTensor& g_lse, const OptTensor& g_loss) {
+  TORCH_CHECK(ids_in.dim() == 2, "cluster_ids must be a 2-D tensor");
+  const int64_t probes = ids_in.size(1);
+  check_route(logits, probes, Tensor());
+  const int64_t n = logits.size(0), e = logits.size(1);
+  auto check = [&](const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const char* what) {
+    TORCH_CHECK(t.sizes() == sizes && t.scalar_type() == type && t.device() == logits.device(), what, " must be ", type,
+                " of ", sizes, " on the scores' device, got ", t.scalar_type(), " of ", t.sizes());
+  };
+  check(ids_in, {n, probes}, at::kLong, "cluster_ids");
+  check(weights_in, {n, probes}, at::kFloat, "weights");
+  check(stats_in, {n, 2}, at::kFloat, "stats");
+  check(slopes_in, {e}, at::kFloat, "slopes");
+  auto check_gradient = [&](const OptTensor& g, at::IntArrayRef sizes) {
+    TORCH_CHECK(!g.has_value() || !g->defined() || (g->sizes() == sizes && g->device() == logits.device()),
+                "gradients must be of the results' shapes and device");
+  };
+  check_gradient(g_weights, {n, probes});
+  check_gradient(g_lse, {n});
+  check_gradient(g_loss, {});
+  const bool on_gpu = logits.is_cuda();
+  const at::Device dev = on_gpu ? logits.device() : gpu_for_cpu_call();
+  c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+  const Tensor z = with_adjacent_columns(logits.to(dev));
+  auto there = [&](const Tensor& t) { return t.to(dev).contiguous(); };
+  const Tensor ids = there(ids_in), weights = there(weights_in), stats = there(stats_in), slopes = there(slopes_in);
+  auto given = [&](const OptTensor& g) { return gradient(g.value_or(Tensor()), dev); };
+  const Tensor gw = given(g_weights), gs = given(g_lse), gl = given(g_loss);
+  Tensor grad = at::empty(z.sizes(), z.options());
+  check_st(st_cluster_route_backward(bytes_or_null(z), score_type(z.scalar_type(), "logits"), z.size(0), z.size(1),
+                                     z.stride(0), probes, data_or_null<int64_t>(ids), data_or_null<float>(weights),
+                                     data_or_null<float>(stats), data_or_null<float>(slopes), data_or_null<float>(gw),
+                                     data_or_null<float>(gs), data_or_null<float>(gl), bytes_or_null(grad),
+                                     current_stream(z)),
+           "cluster_route");
+  return on_gpu ? grad : grad.cpu();
+}
+
+using RouteOp = Route(const Tensor&, int64_t, const OptTensor&);
+using RouteKeepOp = RouteStats(const Tensor&, int64_t, const OptTensor&);
+using RouteBackwardOp = Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                               const OptTensor&, const OptTensor&, const OptTensor&);
+
+Route route_below(const Tensor& logits, int64_t probes, const OptTensor& valid) {
+  static const auto op = find_op<RouteOp>("st::cluster_route");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(logits, probes, valid);
+}
+
+RouteStats route_with_stats_below(const Tensor& logits, int64_t probes, const OptTensor& valid) {
+  static const auto op = find_op<RouteKeepOp>("st::cluster_route_with_stats");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(logits, probes, valid);
+}
+
 struct RouteFunction : torch::autograd::Function<RouteFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t probes, const OptTensor& valid) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    RouteOut o = route_any(logits, probes, valid.value_or(Tensor()));
+    auto [ids, weights, lse, counts, loss, stats, slopes] = route_with_stats_below(logits, probes, valid);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({logits, o.ids, o.weights, o.stats, o.slopes});
-    ctx->mark_non_differentiable({o.ids, o.counts});
-    return {o.ids, o.weights, o.lse, o.counts, o.loss};
+    ctx->save_for_backward({logits, ids, weights, stats, slopes});
+    ctx->mark_non_differentiable({ids, counts});
+    return {ids, weights, lse, counts, loss};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -435,38 +505,16 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
   }
 
   static Tensor logits_gradient(const variable_list& saved, const variable_list& grads) {
+    static const auto op = find_op<RouteBackwardOp>("st::cluster_route_backward");
     at::AutoDispatchBelowADInplaceOrView below;
-    const bool on_gpu = saved[0].is_cuda();
-    const at::Device dev = on_gpu ? saved[0].device() : gpu_for_cpu_call();
-    c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
-    const Tensor z = with_adjacent_columns(saved[0].to(dev));
-    const Tensor ids = saved[1].to(dev), weights = saved[2].to(dev), stats = saved[3].to(dev),
-                 slopes = saved[4].to(dev);
-    const Tensor gw = gradient(grads[1], dev), gs = gradient(grads[2], dev), gl = gradient(grads[4], dev);
-    Tensor grad = at::empty(z.sizes(), z.options());
-    check_st(st_cluster_route_backward(bytes_or_null(z), score_type(z.scalar_type(), "logits"), z.size(0), z.size(1),
-                                       z.stride(0), ids.size(1), data_or_null<int64_t>(ids),
-                                       data_or_null<float>(weights), data_or_null<float>(stats),
-                                       data_or_null<float>(slopes), data_or_null<float>(gw), data_or_null<float>(gs),
-                                       data_or_null<float>(gl), bytes_or_null(grad), current_stream(z)),
-             "cluster_route");
-    return on_gpu ? grad : grad.cpu();
+    return op.call(saved[0], saved[1], saved[2], saved[3], saved[4], if_defined(grads[1]), if_defined(grads[2]),
+                   if_defined(grads[4]));
   }
 };
 
-using Route = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
-
-Route cluster_route(const Tensor& logits, int64_t probes, const OptTensor& valid) {
-  RouteOut o = route_any(logits, probes, valid.value_or(Tensor()));
-  return {o.ids, o.weights, o.lse, o.counts, o.loss};
-}
-
 Route cluster_route_autograd(const Tensor& logits, int64_t probes, const OptTensor& valid) {
   refuse_tangents({&logits}, "cluster_route");
-  if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    return cluster_route(logits, probes, valid);
-  }
+  if (!at::GradMode::is_enabled() || !logits.requires_grad()) return route_below(logits, probes, valid);
   const variable_list o = RouteFunction::apply(logits, probes, valid);
   return {o[0], o[1], o[2], o[3], o[4]};
 }
@@ -492,6 +540,11 @@ TORCH_LIBRARY_FRAGMENT(st, m) {
   // (cluster_ids, weights, lse, counts, balance_loss)
   m.def("cluster_route(Tensor logits, int probes, Tensor? valid=None) "
         "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  // What its gradient calls: the same with statistics and slopes; the gradient of the scores.
+  m.def("cluster_route_with_stats(Tensor logits, int probes, Tensor? valid) "
+        "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("cluster_route_backward(Tensor logits, Tensor cluster_ids, Tensor weights, Tensor stats, Tensor slopes, "
+        "Tensor? g_weights, Tensor? g_lse, Tensor? g_loss) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(st, CUDA, m) {
@@ -501,6 +554,8 @@ TORCH_LIBRARY_IMPL(st, CUDA, m) {
   m.impl("target_logprobs_with_stats", TORCH_FN(target_logprobs_with_stats));
   m.impl("target_logprobs_backward", TORCH_FN(target_logprobs_backward));
   m.impl("cluster_route", TORCH_FN(cluster_route));
+  m.impl("cluster_route_with_stats", TORCH_FN(cluster_route_with_stats));
+  m.impl("cluster_route_backward", TORCH_FN(cluster_route_backward));
 }
 
 TORCH_LIBRARY_IMPL(st, CPU, m) {
@@ -510,6 +565,8 @@ TORCH_LIBRARY_IMPL(st, CPU, m) {
   m.impl("target_logprobs_with_stats", TORCH_FN(target_logprobs_with_stats));
   m.impl("target_logprobs_backward", TORCH_FN(target_logprobs_backward));
   m.impl("cluster_route", TORCH_FN(cluster_route));
+  m.impl("cluster_route_with_stats", TORCH_FN(cluster_route_with_stats));
+  m.impl("cluster_route_backward", TORCH_FN(cluster_route_backward));
 }
 
 TORCH_LIBRARY_IMPL(st, Autograd, m) {

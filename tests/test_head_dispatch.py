@@ -53,12 +53,27 @@ def test_a_mode_sees_target_logprobs(grad):
             assert [a is not None for a in mode.args[8:]] == [True, False, False, True] and (mode.args[3] is None) == (m is None)
 
 
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_mode_sees_cluster_route(grad):
+    z = torch.ones((3, 70), requires_grad=grad)
+    with Answers() as mode:
+        out = st.cluster_route(z, 4, torch.tensor([True, False, True]))
+        if grad:
+            g, = torch.autograd.grad(out[1].sum() + out[4], z)
+            assert (g == 2).all()
+    assert mode.seen == (["cluster_route_with_stats", "cluster_route_backward"] if grad else ["cluster_route"])
+    if grad:
+        assert [a is not None for a in mode.args[5:]] == [True, False, True]
+
+
 def test_fake_scores_do_not_reach_a_kernel():
     for grad in (False, True):
         mode = FakeTensorMode()
         z, targets = torch.ones((3, 70), requires_grad=grad), torch.zeros(3, dtype=torch.long)
         with mode, pytest.raises(Exception, match=r"st\.|st::"):
             st.target_logprobs(mode.from_tensor(z), mode.from_tensor(targets), 4)
+        with mode, pytest.raises(Exception, match=r"st\.|st::"):
+            st.cluster_route(mode.from_tensor(z), 4)
 
 
 def test_target_logprobs_backward_refusals():
@@ -77,3 +92,23 @@ def test_target_logprobs_backward_refusals():
     refused("gradients must be", grads=(None, None, None, two))
     refused("gradients must be", grads=(None, None, one[:2], None))
     refused("temperature", temperature=0.0)
+
+
+def test_cluster_route_backward_refusals():
+    z = torch.zeros((3, 70))
+    ids, four, two, slopes = torch.zeros((3, 4), dtype=torch.long), torch.zeros((3, 4)), torch.zeros((3, 2)), torch.zeros(70)
+
+    def refused(message, logits=z, ids=ids, weights=four, stats=two, slopes=slopes, grads=(None, None, None)):
+        with pytest.raises(RuntimeError, match=message):
+            st.cluster_route_backward(logits, ids, weights, stats, slopes, *grads)
+
+    refused("logits must be a 2-D", logits=z[0])
+    refused("probes must be", ids=torch.zeros((3, 65), dtype=torch.long))
+    refused("cluster_ids must be", ids=ids.int())
+    refused("cluster_ids must be", ids=ids[:2])
+    refused("weights must be", weights=four[:, :3])
+    refused("stats must be", stats=four)
+    refused("slopes must be", slopes=slopes[:69])
+    refused("gradients must be", grads=(two, None, None))
+    refused("gradients must be", grads=(None, two, None))
+    refused("gradients must be", grads=(None, None, two))
