@@ -110,12 +110,6 @@ constexpr bool norm_columns_apart(int64_t dim) {
 #ifdef ST_NORM_TYPE
 namespace {
 
-__device__ __forceinline__ float load_typed(const void* p, int64_t i, int type) {
-  if (type == ST_SCORE_F32) return load_score<ST_SCORE_F32>(p, i);
-  if (type == ST_SCORE_F16) return load_score<ST_SCORE_F16>(p, i);
-  return load_score<ST_SCORE_BF16>(p, i);
-}
-
 // Columns [col, col + 8) of a row as they are stored; 0 past its end.  LAST: where
 // the row ends inside, its last eight for `settle`, one load; put together one by one,
 // those of 16-bit types had to be waited for before their row was due (20,000 x 5,004
