@@ -627,8 +627,8 @@ int st_dropout(const void* x, int type, int64_t elements, double p, const int64_
  * null) the gradients of x (y_type), of the residual (h_type), weight and bias
  * (weight_type), each null where it is not wanted; grad_x is grad_residual's value
  * through dropout with the state that was used.  h: x or sum.  workspace: device
- * memory of st_layer_norm_workspace_bytes(rows, dim) bytes, for the last two.  The
- * same inputs give the same bits.
+ * memory of st_layer_norm_workspace_bytes(rows, dim) bytes (asked for with the call's
+ * device current), for the last two.  The same inputs give the same bits.
  *
  * st_layer_norm_int8: the norm's rows in 8 bits, from their 32-bit values, as
  * st_int8_quantize would hold them.

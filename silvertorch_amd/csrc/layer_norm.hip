@@ -17,11 +17,11 @@ NormShape norm_forward<ST_SCORE_F16>(int dim, bool wide_sum, bool codes);
 template <>
 NormShape norm_forward<ST_SCORE_BF16>(int dim, bool wide_sum, bool codes);
 template <>
-NormShape norm_backward<ST_SCORE_F32>(int dim, bool wide_sum);
+const void* norm_backward<ST_SCORE_F32>(int dim, bool wide_sum);
 template <>
-NormShape norm_backward<ST_SCORE_F16>(int dim, bool wide_sum);
+const void* norm_backward<ST_SCORE_F16>(int dim, bool wide_sum);
 template <>
-NormShape norm_backward<ST_SCORE_BF16>(int dim, bool wide_sum);
+const void* norm_backward<ST_SCORE_BF16>(int dim, bool wide_sum);
 template <>
 const void* norm_columns<ST_SCORE_F32>(bool wide_sum);
 template <>
@@ -52,7 +52,7 @@ NormShape forward_shape_of(int type, int dim, bool wide_sum, bool codes) {
   return norm_forward<ST_SCORE_BF16>(dim, wide_sum, codes);
 }
 
-NormShape backward_shape_of(int type, int dim, bool wide_sum) {
+const void* backward_kernel_of(int type, int dim, bool wide_sum) {
   if (type == ST_SCORE_F32) return norm_backward<ST_SCORE_F32>(dim, false);
   if (type == ST_SCORE_F16) return norm_backward<ST_SCORE_F16>(dim, wide_sum);
   return norm_backward<ST_SCORE_BF16>(dim, wide_sum);
@@ -76,14 +76,15 @@ void launch_forward(NormArgs& a, int type, bool wide_sum, bool codes, hipStream_
   launch_kernel(shape.kernel, dim3(static_cast<unsigned>(grid)), shape.threads, &a, "norm_kernel", s);
 }
 
-// The backward kernel's workgroups: each adds two rows of sums in 32 bits to the
-// traffic, so there are no more of them than the chip holds at once, and each takes
-// four turns at least where that leaves one a CU.
+// The backward kernel's workgroups, for the workspace and the launch: each adds two
+// rows of sums in 32 bits to the traffic, so there are no more of them than the
+// current device holds at once, and each takes four turns at least where that leaves
+// one a CU.
 int64_t backward_groups(int64_t rows, int64_t dim) {
   const NormLayout l = kNormLayouts[norm_layout(dim)];
   const int64_t turns = (rows + norm_rows(l.lanes) - 1) / norm_rows(l.lanes);
-  const int64_t most = 256 * std::max(1, norm_backward_waves(l.lanes, l.steps) * 256 / norm_threads(l.lanes));
-  return std::max<int64_t>(1, std::min(most, std::max(std::min<int64_t>(turns, 256), turns / 4)));
+  const int64_t cus = cu_count(), most = cus * std::max(1, norm_backward_waves(l.lanes, l.steps) * 256 / norm_threads(l.lanes));
+  return std::max<int64_t>(1, std::min(most, std::max(std::min(turns, cus), turns / 4)));
 }
 
 // out[c] = sum over the parts, for C columns of gw and gb side by side: 1,024 / C
@@ -239,7 +240,6 @@ extern "C" int st_layer_norm_backward(const void* grad_y, int y_type, const void
     hipStream_t s = static_cast<hipStream_t>(stream);
     int64_t groups = 0;
     if (rows > 0) {
-      const NormShape shape = backward_shape_of(y_type, static_cast<int>(dim), h_type != y_type);
       groups = backward_groups(rows, dim);
       if (a.dropout.dropped == 0) a.dropout.state = nullptr;
       a.gy = grad_y;
@@ -257,7 +257,8 @@ extern "C" int st_layer_norm_backward(const void* grad_y, int y_type, const void
       a.inverse_dim = 1.0f / static_cast<float>(dim);
       const bool apart = norm_columns_apart(dim), wide = h_type != y_type;
       if (!apart || grad_x || grad_residual)
-        launch_kernel(shape.kernel, dim3(static_cast<unsigned>(groups)), shape.threads, &a, "norm_backward_kernel", s);
+        launch_kernel(backward_kernel_of(y_type, a.dim, wide), dim3(static_cast<unsigned>(groups)),
+                      norm_threads(kNormLayouts[norm_layout(dim)].lanes), &a, "norm_backward_kernel", s);
       if (apart && sums) {
         groups = std::min<int64_t>(groups, 128);  // times 2,048 columns each
         launch_kernel(columns_kernel_of(y_type, wide), dim3(static_cast<unsigned>((dim + 2047) / 2048), static_cast<unsigned>(groups)),

@@ -74,7 +74,8 @@ constexpr int norm_layout(int64_t dim, const NormLayout* layouts = kNormLayouts)
 constexpr int norm_threads(int lanes) { return lanes <= 64 ? 256 : lanes; }
 constexpr int norm_rows(int lanes) { return lanes <= 64 ? 256 / lanes : 1; }
 
-// Waves a SIMD that the backward kernel's registers leave room for.
+// Waves a SIMD that the backward kernel's registers leave room for (its launch
+// bounds hold them to it).
 constexpr int norm_backward_waves(int lanes, int steps) {
   return lanes == 1024 || steps == 1 ? 4 : lanes <= 256 && steps == 2 ? 3 : 2;
 }
@@ -96,7 +97,7 @@ NormShape norm_shape(K* kernel, int threads, int rows) {
 template <int DT>
 NormShape norm_forward(int dim, bool wide_sum, bool codes);
 template <int DT>
-NormShape norm_backward(int dim, bool wide_sum);
+const void* norm_backward(int dim, bool wide_sum);
 template <int DT>
 const void* norm_columns(bool wide_sum);
 
@@ -589,12 +590,6 @@ NormShape forward_shape() {
   return shape;
 }
 
-template <int DT, int HT, int L, int S>
-NormShape backward_shape() {
-  static const NormShape shape = norm_shape(norm_backward_kernel<DT, HT, L, S>, norm_threads(L), norm_rows(L));
-  return shape;
-}
-
 template <int DT, int HT, bool CODES, int I = 0>
 NormShape forward_for(int layout) {
   constexpr const NormLayout* layouts = CODES ? kCodeLayouts : kNormLayouts;
@@ -606,12 +601,13 @@ NormShape forward_for(int layout) {
 }
 
 template <int DT, int HT, int I = 0>
-NormShape backward_for(int layout) {
+const void* backward_for(int layout) {
   if constexpr (I < kNormLayoutCount) {
-    if (layout == I) return backward_shape<DT, HT, kNormLayouts[I].lanes, kNormLayouts[I].steps>();
+    if (layout == I)
+      return reinterpret_cast<const void*>(&norm_backward_kernel<DT, HT, kNormLayouts[I].lanes, kNormLayouts[I].steps>);
     return backward_for<DT, HT, I + 1>(layout);
   }
-  return {};
+  return nullptr;
 }
 
 }  // namespace
@@ -625,7 +621,7 @@ NormShape norm_forward<ST_NORM_TYPE>(int dim, bool wide_sum, bool codes) {
 }
 
 template <>
-NormShape norm_backward<ST_NORM_TYPE>(int dim, bool wide_sum) {
+const void* norm_backward<ST_NORM_TYPE>(int dim, bool wide_sum) {
   const int layout = norm_layout(dim);
   if (wide_sum) return backward_for<ST_NORM_TYPE, ST_SCORE_F32>(layout);
   return backward_for<ST_NORM_TYPE, ST_NORM_TYPE>(layout);
