@@ -807,6 +807,7 @@ extern "C" int st_int8_matmul(const int8_t* codes, const float* scales, int64_t 
     }
     if (x_type != ST_CODE_I8) {
       ST_CHECK(workspace, "null device pointer");
+      ST_CHECK(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be 16-byte aligned");
       int8_t* made = static_cast<int8_t*>(workspace);
       float* made_scales = reinterpret_cast<float*>(made + codes_bytes(tokens, columns));
       quantize(x, x_type, tokens, dim, x_stride, made, made_scales, s);
