@@ -355,7 +355,11 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
         }
       }
       join_row<L>(left, room + (L > 64 ? L / 64 : 0), kAdd);
-      rest = __fdiv_rn(left[1], static_cast<float>(a.dim));
+      // Divided, where float32's sums are not exact, so that rows of one value leave
+      // just what all their columns are off by; those of 16 bits are, up to 8,192
+      // columns, and the product takes ten instructions less (codes of 1,000,000 x 100
+      // bfloat16 105 -> 99 us).
+      rest = HT == ST_SCORE_F32 ? __fdiv_rn(left[1], static_cast<float>(a.dim)) : left[1] * (1.0f / static_cast<float>(a.dim));
       // a maximum with 0 would turn NaN into it
       float squares = fmaf(-rest, left[1], left[0]);
       squares = squares < 0.0f ? 0.0f : squares;
