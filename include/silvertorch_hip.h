@@ -621,7 +621,8 @@ int st_dropout(const void* x, int type, int64_t elements, double p, const int64_
  * r * dim + column; p is 0 without a residual.  weight and bias (weight_type; null
  * for 1 and 0).  y (x's type) and sum are contiguous.  stats (or null) [rows,
  * ST_NORM_STATS]: what the backward call needs.  Statistics are 32-bit: squares
- * of what a row is apart from its mean have to sum up below 2^128.
+ * of what a row is apart from its mean, as 32 bits round that, have to sum up below
+ * 2^128.
  *
  * st_layer_norm_backward: from grad_y (y_type, x's) and grad_sum (h_type, or
  * null) the gradients of x (y_type), of the residual (h_type), weight and bias

@@ -7,8 +7,9 @@
 //
 // Half words, not words: a block is 20 products of 32 x 32 bits, a quarter of
 // the vector units' rate each, and with a word an element they, not the bytes,
-// would bound bfloat16.  p = 0.1 is off by 7e-6 of itself for it; kept elements
-// are multiplied with 2^16 / (2^16 - dropped), so the expectation is exact.
+// would bound bfloat16.  p is off by 2^-17 at most for it (0.1 is 6,554 of 65,536,
+// 6e-5 of itself too much); kept elements are multiplied with 2^16 / (2^16 - dropped),
+// so the expectation is exact.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -8,10 +8,12 @@
 //
 // A row lies in registers from its one read on, 8 columns a lane and step: the
 // mean first, then what its rounding left and the squares of what is apart from
-// it, so that rows far from 0 lose no digits.  HBM bounds both directions: 100
-// million bfloat16 elements take 76 to 88 us forward and 118 to 136 us backward in
-// rows of 64 to 16,384 columns, odd lengths among them, but 105 and 145 in rows of 24
-// and 97 to 136 and 214 to 260 in longer ones (all without a warm cache).
+// it, so that rows far from 0 lose no digits: n is (h - mean) - rest times r in both
+// directions.  HBM bounds them: 100 million bfloat16 elements take 78 to 85 us forward
+// and 119 to 127 us backward in rows of 64 to 16,384 columns.  Longer: lengths that
+// are no multiple of 8, 83 to 95 and 122 to 139, with 160 backward at 5,001 and 5,003;
+// rows of 16 and 24, 97 and 104, 138 and 141; past 16,384 columns 97 to 144 and 212 to
+// 263 (all without a warm cache).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -51,8 +53,8 @@ struct NormBackwardArgs {
 
 // Lanes of a row and steps of 8 columns a lane: the first that holds a row.  Two or
 // three steps: what a row costs besides its columns is shared by more of them, and a
-// wave has more rows under way (500,000 x 200 bfloat16 in one step 107 and 165 us
-// forward and backward, in two 83 and 120).
+// wave has more rows under way (500,000 x 200 bfloat16 in one step 116 and 145 us
+// forward and backward, in two 84 and 123).
 struct NormLayout {
   int lanes, steps;
 };
@@ -60,7 +62,9 @@ constexpr NormLayout kNormLayouts[] = {{1, 1},   {1, 2},   {1, 3},   {2, 2},   {
                                        {8, 3},   {16, 2},  {16, 3},  {32, 2},  {32, 3},  {64, 2},  {64, 3}, {128, 2},
                                        {128, 3}, {256, 2}, {256, 3}, {512, 2}, {512, 3}, {1024, 2}, {1024, 3}, {1024, 4}};
 // Where codes are the result, instructions bound it, a good part of them the same
-// for any number of columns a lane has: 16,384 x 4,096 with 256 lanes 62 us.
+// for any number of columns a lane has: 24,414 x 4,096 bfloat16 with 256 lanes 72 us,
+// with 128 63.  Lengths just past a power of two leave lanes idle: 11,111 x 9,000 119
+// us, 12,207 x 8,192 61.
 constexpr NormLayout kCodeLayouts[] = {{2, 1},  {4, 1},  {8, 1},   {16, 1},  {16, 2}, {16, 4},
                                        {32, 4}, {64, 4}, {128, 4}, {256, 4}, {512, 4}, {1024, 4}};
 constexpr int kNormLayoutCount = sizeof(kNormLayouts) / sizeof(kNormLayouts[0]);
@@ -114,7 +118,7 @@ namespace {
 // Columns [col, col + 8) of a row as they are stored; 0 past its end.  LAST: where
 // the row ends inside, its last eight for `settle`, one load; put together one by one,
 // those of 16-bit types had to be waited for before their row was due (20,000 x 5,004
-// bfloat16 104 and 210 us forward and backward, so 77 and 121).
+// bfloat16 112 and 216 us forward and backward, so 79 and 126).
 template <int DT, bool LAST = false>
 __device__ __forceinline__ Raw8<DT> load_raw_columns(const void* row, int col, int dim) {
   Raw8<DT> r{};
@@ -150,9 +154,9 @@ __device__ __forceinline__ void settle(Raw8<DT>& r, int col, int dim) {
 
 // Whether rows of type DT are loaded so by L lanes in S steps: where they have eight
 // columns (layouts of more than 16), and registers have room for it (not float32's;
-// of 1,024 lanes bfloat16's in three steps, 4,999 x 20,001 151 and 267 us, so 136 and
-// 259, but in two or four they spill, 6,103 x 16,384 backward 124 us, so 175, and
-// float16's in three, 244 us, so 332).
+// of 1,024 lanes bfloat16's in three steps, 4,999 x 20,001 155 and 267 us, so 144 and
+// 263, but in two or four they spill, 6,103 x 16,384 backward 121 us, so 165, and
+// float16's in three, 5,000 x 20,000 215 us, so 335).
 template <int DT, int L, int S>
 constexpr bool kLast = DT != ST_SCORE_F32 && L * S > 2 && (L != 1024 || (S == 3 && DT == ST_SCORE_BF16));
 
@@ -272,7 +276,7 @@ __global__ __launch_bounds__(norm_threads(L)) void norm_kernel(NormArgs a) {
 
   // A wave's rows go through the loop together; what a lane of a row past the
   // last computes is not stored.  The next row is on its way while one is worked on,
-  // where there are registers for it (3,051 x 32,768 111 us without, 97 with).
+  // where there are registers for it (3,051 x 32,768 114 us without, 100 with).
   constexpr bool kNext = L * S <= 2048 || (HT != ST_SCORE_F32 && !CODES);
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / (L < 64 ? 64 : L) * (L < 64 ? 64 / L : 1);
