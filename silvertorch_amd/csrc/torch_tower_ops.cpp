@@ -254,6 +254,8 @@ void check_gradients(const Tensor& h, at::ScalarType y_type, const Tensor& weigh
   check_weights(h, weight, Tensor(), 1.0, "layer_norm_backward");
   score_type(y_type, "x");
   score_type(weights, "weight and bias");
+  TORCH_CHECK(!weight.defined() || weight.scalar_type() == weights, "weight must be of weight_type ", weights, ", got ",
+              weight.scalar_type());
   TORCH_CHECK(h.scalar_type() == y_type || h.scalar_type() == at::kFloat, "the sum must be of x's type or float32, got ",
               h.scalar_type());
   TORCH_CHECK(stats.dim() == 2 && stats.size(0) == h.numel() / h.size(-1) && stats.size(1) == ST_NORM_STATS &&

@@ -1,4 +1,7 @@
-"""Pointers that the tower's C entry points cannot take, refused before any device work."""
+"""What the tower's entry points cannot take, refused before any device work: pointers, types that do not agree."""
+
+import pytest
+import torch
 
 import silvertorch_amd.ops._load_ops  # noqa: F401
 from silvertorch_amd import capi
@@ -13,3 +16,11 @@ def test_int8_matmul_refuses_an_unaligned_workspace():
         assert call(workspace) != 0
         assert "the workspace must be 16-byte aligned" in L.st_last_error().decode()
     assert call(None) != 0 and "null device pointer" in L.st_last_error().decode()
+
+
+def test_layer_norm_backward_refuses_a_weight_of_another_type():
+    """The kernel would read it as weight_type."""
+    h, stats = torch.zeros((3, 10)), torch.zeros((3, 3))
+    for weight, weight_type in ((torch.ones(10).half(), torch.float32), (torch.ones(10), torch.bfloat16)):
+        with pytest.raises(RuntimeError, match="weight must be of weight_type"):
+            torch.ops.st.layer_norm_backward(h, None, h, weight, stats, None, 0.0, torch.float32, weight_type, [True] * 4)
