@@ -62,6 +62,8 @@ class QueryTowerModule(nn.Module):
                                        "again) would drop other elements than its first run: give it a state, "
                                        "checkpoint(tower, x, tower.next_state())")
                 state = self.next_state()
+            elif state.shape != (2,):
+                raise RuntimeError(f"state must hold seed and offset, got a tensor of {list(state.shape)}")
             p, states = self.dropout, (state + self.places).unbind()
             x = ops.dropout(x, p, states[0])
         h = self.enter(x)

@@ -69,3 +69,10 @@ def test_checkpointed_pass_without_dropout(plain, use_reentrant):
     checkpoint(tower, x, use_reentrant=use_reentrant).square().sum().backward()
     assert all(torch.equal(p.grad, g) for p, g in zip(tower.parameters(), want))
     assert tower.rng.tolist() == [9, 0]
+
+
+def test_states_of_other_shapes_are_refused(plain):
+    tower, x = _tower(), torch.zeros((5, 6), dtype=torch.float64)
+    for state in (tower.rng[:1], tower.places, tower.rng[0]):
+        with pytest.raises(RuntimeError, match="seed and offset"):
+            tower(x, state)
